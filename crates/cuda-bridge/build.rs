@@ -37,6 +37,7 @@ fn main() {
         .arg("-o")
         .arg(&lib)
         .arg(csrc.join("bridge.cu"))
+        .arg(csrc.join("paged.cu"))
         .args(["-ldl", "-lpthread"])
         .status()
         .expect("failed to run nvcc");

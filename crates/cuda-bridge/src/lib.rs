@@ -87,6 +87,55 @@ pub mod ffi {
         pub tokens: i64,
     }
 
+    /// A paged KV cache and a step's batch (device pointers).
+    #[repr(C)]
+    #[derive(Clone, Copy, Debug)]
+    pub struct cb_paged_kv {
+        pub k: *mut c_void,
+        pub v: *mut c_void,
+        pub table: *const i32,
+        pub len: *const i32,
+        pub row_start: *const i32,
+        pub dtype: i32,
+        pub pages: i32,
+        pub kv_heads: i32,
+        pub page_size: i32,
+        pub batch: i32,
+        pub table_stride: i32,
+        pub max_len: i32,
+        pub rows: i32,
+        pub max_new: i32,
+    }
+
+    #[repr(C)]
+    #[derive(Clone, Copy, Debug)]
+    pub struct cb_rope_config {
+        pub inv_freq: *const f64,
+        pub rot_dim: i32,
+        pub layout: i32,
+        pub amplitude: f32,
+    }
+
+    #[repr(C)]
+    #[derive(Clone, Copy, Debug)]
+    pub struct cb_rope_scaling {
+        pub base: f64,
+        pub kind: i32,
+        pub factor: f64,
+        pub original_len: f64,
+        pub fast_turns: f64,
+        pub slow_turns: f64,
+    }
+
+    pub const CB_DTYPE_F16: i32 = 1;
+    pub const CB_DTYPE_BF16: i32 = 2;
+    pub const CB_ROPE_HALF: i32 = 1;
+    pub const CB_ROPE_INTERLEAVED: i32 = 2;
+    pub const CB_ROPE_SCALE_NONE: i32 = 0;
+    pub const CB_ROPE_SCALE_LINEAR: i32 = 1;
+    pub const CB_ROPE_SCALE_BASE: i32 = 2;
+    pub const CB_ROPE_SCALE_PARTS: i32 = 3;
+
     pub enum cb_ctx {}
     pub enum cb_tokens {}
 
@@ -135,6 +184,14 @@ pub mod ffi {
         pub fn cb_attention_bwd_f16(q: *const c_void, k: *const c_void, v: *const c_void, o: *const c_void, dout: *const c_void, lse: *const f32, dqkv: *mut c_void, batch: i32, heads: i32, kv_heads: i32, seq: i32, stream: *mut c_void) -> cb_status;
         pub fn cb_lm_head_ce_f16(xf: *const c_void, embed: *const c_void, targets: *const u32, t: i32, dim: i32, vocab: i32, softcap: f32, per_token_loss: *mut f32, loss: *mut f32, stream: *mut c_void) -> cb_status;
         pub fn cb_lm_head_ce_f16_noalloc(xf: *const c_void, embed: *const c_void, targets: *const u32, t: i32, dim: i32, vocab: i32, softcap: f32, per_token_loss: *mut f32, loss: *mut f32, stream: *mut c_void) -> cb_status;
+        pub fn cb_rope_frequencies(rot_dim: i32, scaling: *const cb_rope_scaling, inv_freq: *mut f64, amplitude: *mut f32) -> cb_status;
+        pub fn cb_rope(rope: *const cb_rope_config, dtype: i32, x: *const c_void, x_stride: i64, y: *mut c_void, y_stride: i64, positions: *const i32, tokens: i32, heads: i32, head_dim: i32, inverse: i32, stream: *mut c_void) -> cb_status;
+        pub fn cb_paged_append(kv: *const cb_paged_kv, rope: *const cb_rope_config, heads: i32, q: *const c_void, q_stride: i64, q_out: *mut c_void, q_out_stride: i64, k: *const c_void, k_stride: i64, v: *const c_void, v_stride: i64, positions: *const i32, weights: *mut f32, slot_positions: *mut i32, stream: *mut c_void) -> cb_status;
+        pub fn cb_paged_attention_workspace(kv: *const cb_paged_kv, heads: i32, bytes: *mut usize) -> cb_status;
+        pub fn cb_paged_attention(kv: *const cb_paged_kv, q: *const c_void, q_stride: i64, heads: i32, scale: f32, out: *mut c_void, out_stride: i64, lse: *mut f32, workspace: *mut c_void, workspace_bytes: usize, stream: *mut c_void) -> cb_status;
+        pub fn cb_paged_attention_weights(kv: *const cb_paged_kv, q: *const c_void, q_stride: i64, heads: i32, scale: f32, lse: *const f32, weights: *mut f32, stream: *mut c_void) -> cb_status;
+        pub fn cb_paged_evict_workspace(kv: *const cb_paged_kv, budget: i32, bytes: *mut usize) -> cb_status;
+        pub fn cb_paged_evict(kv: *const cb_paged_kv, weights: *const f32, weights_out: *mut f32, positions: *const i32, positions_out: *mut i32, next_position: *const i32, budget: i32, sinks: i32, recent: i32, len_out: *mut i32, workspace: *mut c_void, workspace_bytes: usize, stream: *mut c_void) -> cb_status;
     }
 }
 

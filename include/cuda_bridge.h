@@ -442,6 +442,156 @@ cb_status cb_lm_head_ce_f16_noalloc(const void* xf, const void* embed, const uin
                                     int32_t T, int32_t dim, int32_t vocab, float softcap,
                                     float* per_token_loss, float* loss, void* stream);
 
+/* ---- Serving from a paged KV cache (kernel-level entry points; device pointers). ------
+ *
+ * K and V live in pages of page_size slots of one layer, [pages][kv_heads][page_size][128].
+ * A batch of sequences of any lengths uses them through a page table: slot s of sequence b
+ * is row s % page_size of page table[b][s / page_size]. A step brings new tokens, any
+ * number per sequence (none, one in decode, a chunk of a prompt): the rows row_start[b] ..
+ * row_start[b + 1] of the token arrays, which take the last slots of the sequence. One step
+ * of one layer is
+ *   cb_paged_append              rotate q and k, write k and v into the pages
+ *   cb_paged_attention           attention of the new tokens over the cache
+ *   cb_paged_attention_weights   (to evict later) add up the weight that every slot got
+ * and now and then cb_paged_evict cuts the sequences down to their heaviest slots. The
+ * tables and lengths are read on the device, so a captured CUDA graph serves every step
+ * whose sizes stay within the host-side bounds of the descriptor.
+ *
+ * All pointers are device memory of the current device (CB_ERR_INVALID_ARG otherwise),
+ * token arrays and caches 16-byte aligned, strides counted in elements and multiples of 8.
+ * Work is enqueued on `stream` (NULL = default stream) without allocation or
+ * synchronisation. Device-side values are held to the descriptor: a page id outside
+ * 0 .. pages - 1 stands for slots that are absent (not written, not seen by any query),
+ * slots from max_len on are absent, rows from `rows` on do not exist, and of a sequence
+ * with more than max_new new tokens the rows behind max_new are left alone. Rows behind
+ * the last sequence (padding) are neither read nor written. */
+
+#define CB_DTYPE_F16 1
+#define CB_DTYPE_BF16 2
+
+typedef struct cb_paged_kv {
+  void* k;                  /* [pages][kv_heads][page_size][128], dtype */
+  void* v;
+  const int32_t* table;     /* [batch][table_stride] page ids */
+  const int32_t* len;       /* [batch] slots in use, this step's new tokens included */
+  const int32_t* row_start; /* [batch + 1] first row of each sequence's new tokens; ascending */
+  int32_t dtype;            /* CB_DTYPE_F16 or CB_DTYPE_BF16: cache and token arrays */
+  int32_t pages;
+  int32_t kv_heads;
+  int32_t page_size;        /* 16, 32, 64 or 128 */
+  int32_t batch;
+  int32_t table_stride;     /* ids per table row, >= ceil(max_len / page_size) */
+  int32_t max_len;          /* no len is above this */
+  int32_t rows;             /* rows of the token arrays */
+  int32_t max_new;          /* no sequence has more new tokens than this; <= rows */
+} cb_paged_kv;
+
+/* Rotary positions: the first rot_dim elements of a head are rotated in pairs, pair i of
+ * position p by the angle p * inv_freq[i], the others pass. The model of this library uses
+ * CB_ROPE_INTERLEAVED over all 128 elements with base 10000 and no scaling. */
+#define CB_ROPE_HALF 1        /* pair i = elements i and i + rot_dim / 2 */
+#define CB_ROPE_INTERLEAVED 2 /* pair i = elements 2 i and 2 i + 1 */
+
+typedef struct cb_rope_config {
+  const double* inv_freq; /* device, [rot_dim / 2] radians per position */
+  int32_t rot_dim;        /* a multiple of 8, at most the head's size */
+  int32_t layout;         /* CB_ROPE_HALF or CB_ROPE_INTERLEAVED */
+  float amplitude;        /* factor of cos and sin (1 = a pure rotation) */
+} cb_rope_config;
+
+#define CB_ROPE_SCALE_NONE 0
+#define CB_ROPE_SCALE_LINEAR 1 /* every frequency divided by factor */
+#define CB_ROPE_SCALE_BASE 2   /* the base multiplied by factor^(rot_dim / (rot_dim - 2)) */
+#define CB_ROPE_SCALE_PARTS 3  /* frequencies that turn more than fast_turns times within
+                                  original_len positions are kept, those under slow_turns
+                                  divided by factor, a linear ramp over the pair index in
+                                  between; amplitude 0.1 ln(factor) + 1 */
+
+typedef struct cb_rope_scaling {
+  double base;         /* 10000 unless the model says otherwise */
+  int32_t kind;        /* CB_ROPE_SCALE_*; the fields below as that kind uses them */
+  double factor;       /* contexts this many times as long as those of the training */
+  double original_len; /* tokens of a context of the training */
+  double fast_turns;
+  double slow_turns;
+} cb_rope_scaling;
+
+/* Host call (no GPU): inv_freq[i] = base^(-2 i / rot_dim), i < rot_dim / 2, scaled. inv_freq:
+ * host [rot_dim / 2], to be copied to the device by the caller; amplitude (nullable): the
+ * factor for cb_rope_config. */
+cb_status cb_rope_frequencies(int32_t rot_dim, const cb_rope_scaling* scaling,
+                              double* inv_freq, float* amplitude);
+
+/* y = x rotated to its positions: x and y are [tokens][heads][head_dim] with x_stride and
+ * y_stride elements from token to token (heads are adjacent), positions device [tokens]
+ * (any sign). Angles are formed in 64 bits, products in 32. inverse = 1 rotates back and
+ * is the gradient: dx from dy (with the same amplitude). y == x with equal strides rotates
+ * in place; other overlaps are refused. head_dim: a multiple of 8, at most 512. */
+cb_status cb_rope(const cb_rope_config* rope, int32_t dtype, const void* x, int64_t x_stride,
+                  void* y, int64_t y_stride, const int32_t* positions, int32_t tokens,
+                  int32_t heads, int32_t head_dim, int32_t inverse, void* stream);
+
+/* Writes a step's new tokens into the cache. Per row r (token i of sequence b with n new
+ * tokens; its slot is len[b] - n + i): k [rows][kv_heads][128] rotated to positions[r] and
+ * v [rows][kv_heads][128] unchanged go to the slot, q [rows][heads][128] rotated goes to
+ * q_out. rope NULL: nothing is rotated. positions NULL: the slot is the position. q and
+ * q_out both NULL: only the cache is written (heads is then ignored); q_out == q with equal
+ * strides rotates in place. weights and slot_positions (each nullable, [pages][kv_heads]
+ * [page_size]) get 0 and the position for each new slot. */
+cb_status cb_paged_append(const cb_paged_kv* kv, const cb_rope_config* rope, int32_t heads,
+                          const void* q, int64_t q_stride, void* q_out, int64_t q_out_stride,
+                          const void* k, int64_t k_stride, const void* v, int64_t v_stride,
+                          const int32_t* positions, float* weights, int32_t* slot_positions,
+                          void* stream);
+
+/* Bytes of workspace that cb_paged_attention needs for this descriptor (host call, no GPU).
+ * It reads batch, kv_heads, max_len, rows and max_new only. */
+cb_status cb_paged_attention_workspace(const cb_paged_kv* kv, int32_t heads, size_t* bytes);
+
+/* Attention of a step's new tokens over the cache: query row r (token i of n of sequence b)
+ * sees the slots 0 .. len[b] - n + i (the new tokens' own K and V must be in the cache:
+ * cb_paged_append). out[r][h] = softmax(scale * q[r][h] . K) V with key head
+ * h / (heads / kv_heads). heads is a multiple of kv_heads. q and out: [rows][heads][128];
+ * out must not overlap q. lse (nullable, [rows][heads]): the base-2 log-sum-exp of the
+ * scaled scores, as cb_attention_fwd_lse_f16. A row that sees no slot gets out = 0 and
+ * lse = -inf. workspace: 16-byte aligned; its contents do not matter and none are kept, but
+ * calls (and replays of captured graphs) that may run at the same time need one each. */
+cb_status cb_paged_attention(const cb_paged_kv* kv, const void* q, int64_t q_stride,
+                             int32_t heads, float scale, void* out, int64_t out_stride,
+                             float* lse, void* workspace, size_t workspace_bytes, void* stream);
+
+/* Adds to weights ([pages][kv_heads][page_size]) the attention weight that each slot got
+ * from this step's queries: sum over the rows r that see it and the query heads h of its key
+ * head of 2^(scale * log2(e) * q[r][h] . K - lse[r][h]), lse from cb_paged_attention. Every
+ * sum is formed in 32 bits in a fixed order. A page that two sequences of the batch share
+ * collects from both (the order of the two additions is not fixed). */
+cb_status cb_paged_attention_weights(const cb_paged_kv* kv, const void* q, int64_t q_stride,
+                                     int32_t heads, float scale, const float* lse,
+                                     float* weights, void* stream);
+
+/* Bytes of workspace that cb_paged_evict needs (host call, no GPU; reads batch, kv_heads
+ * and max_len). */
+cb_status cb_paged_evict_workspace(const cb_paged_kv* kv, int32_t budget, size_t* bytes);
+
+/* Cuts every sequence down to at most `budget` slots, each key head by its own choice. Of a
+ * sequence with len[b] > budget slots it keeps those of positions below `sinks`, those of
+ * positions from next_position[b] - recent on, and then those of the largest weights (NaN
+ * counts as the smallest; among equals the lowest slot), budget in all; sinks + recent <=
+ * budget. The kept slots behind the budget move into the slots below it that became free,
+ * both in ascending order; the other kept slots stay where they are (attention does not
+ * depend on the slots' order). len_out[b] = min(len[b], budget). weights_out and
+ * positions_out get the values of all slots below len_out[b]; they may be the input arrays
+ * themselves (not overlap them in another way). K and V change in place. Slots from
+ * len_out[b] on are left as they were. len_out must not overlap len. The sequences of the
+ * batch must not share pages (the contents of shared pages are undefined afterwards).
+ * row_start, rows and max_new are not used (row_start may be NULL). workspace as in
+ * cb_paged_attention. */
+cb_status cb_paged_evict(const cb_paged_kv* kv, const float* weights, float* weights_out,
+                         const int32_t* positions, int32_t* positions_out,
+                         const int32_t* next_position, int32_t budget, int32_t sinks,
+                         int32_t recent, int32_t* len_out, void* workspace,
+                         size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

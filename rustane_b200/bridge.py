@@ -23,6 +23,16 @@ CB_ERR_NCCL = 7
 CB_INIT_NORMAL = 0
 CB_INIT_REFERENCE = 1
 
+CB_DTYPE_F16 = 1
+CB_DTYPE_BF16 = 2
+
+CB_ROPE_HALF = 1
+CB_ROPE_INTERLEAVED = 2
+CB_ROPE_SCALE_NONE = 0
+CB_ROPE_SCALE_LINEAR = 1
+CB_ROPE_SCALE_BASE = 2
+CB_ROPE_SCALE_PARTS = 3
+
 STATUS_NAMES = {
     CB_OK: "CB_OK",
     CB_ERR_INVALID_ARG: "CB_ERR_INVALID_ARG",
@@ -49,6 +59,9 @@ EXPORTED = [
     "cb_tokens_len", "cb_tokens_close", "cb_forward_loss_windows", "cb_eval_windows",
     "cb_enable_training", "cb_zero_grads", "cb_forward_backward", "cb_get_grads_f32",
     "cb_prefill", "cb_decode_step", "cb_decode_position",
+    "cb_rope_frequencies", "cb_rope", "cb_paged_append", "cb_paged_attention_workspace",
+    "cb_paged_attention", "cb_paged_attention_weights", "cb_paged_evict_workspace",
+    "cb_paged_evict",
 ]
 
 
@@ -83,6 +96,24 @@ class cb_eval_totals(C.Structure):
                 ("tokens", C.c_int64)]
 
 
+class cb_paged_kv(C.Structure):
+    _fields_ = ([(n, C.c_void_p) for n in ("k", "v", "table", "len", "row_start")]
+                + [(n, C.c_int32) for n in
+                   ("dtype", "pages", "kv_heads", "page_size", "batch", "table_stride",
+                    "max_len", "rows", "max_new")])
+
+
+class cb_rope_config(C.Structure):
+    _fields_ = [("inv_freq", C.c_void_p), ("rot_dim", C.c_int32), ("layout", C.c_int32),
+                ("amplitude", C.c_float)]
+
+
+class cb_rope_scaling(C.Structure):
+    _fields_ = [("base", C.c_double), ("kind", C.c_int32), ("factor", C.c_double),
+                ("original_len", C.c_double), ("fast_turns", C.c_double),
+                ("slow_turns", C.c_double)]
+
+
 _lib = None
 
 
@@ -98,6 +129,8 @@ def load_library(path: Path | None = None) -> C.CDLL:
     lib = C.CDLL(str(p))
     vp, i32, i64, u64, f32 = C.c_void_p, C.c_int32, C.c_int64, C.c_uint64, C.c_float
     pf, pu32, pi32 = C.POINTER(C.c_float), C.POINTER(C.c_uint32), C.POINTER(C.c_int32)
+    psize = C.POINTER(C.c_size_t)
+    pkv, prope = C.POINTER(cb_paged_kv), C.POINTER(cb_rope_config)
     sig = {
         "cb_version": (C.c_char_p, []),
         "cb_device_count": (i32, [pi32]),
@@ -144,6 +177,16 @@ def load_library(path: Path | None = None) -> C.CDLL:
         "cb_prefill": (i32, [vp, pu32, i32, i32, f32, pf]),
         "cb_decode_step": (i32, [vp, pu32, i32, pf, pu32]),
         "cb_decode_position": (i32, [vp, pi32]),
+        "cb_rope_frequencies": (i32, [i32, C.POINTER(cb_rope_scaling), C.POINTER(C.c_double), pf]),
+        "cb_rope": (i32, [prope, i32, vp, i64, vp, i64, vp, i32, i32, i32, i32, vp]),
+        "cb_paged_append": (i32, [pkv, prope, i32, vp, i64, vp, i64, vp, i64, vp, i64, vp, vp,
+                                  vp, vp]),
+        "cb_paged_attention_workspace": (i32, [pkv, i32, psize]),
+        "cb_paged_attention": (i32, [pkv, vp, i64, i32, f32, vp, i64, vp, vp, C.c_size_t, vp]),
+        "cb_paged_attention_weights": (i32, [pkv, vp, i64, i32, f32, vp, vp, vp]),
+        "cb_paged_evict_workspace": (i32, [pkv, i32, psize]),
+        "cb_paged_evict": (i32, [pkv, vp, vp, vp, vp, vp, i32, i32, i32, vp, vp, C.c_size_t,
+                                 vp]),
     }
     for name, (res, args) in sig.items():
         fn = getattr(lib, name)

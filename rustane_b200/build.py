@@ -14,13 +14,14 @@ PKG = Path(__file__).resolve().parent
 ROOT = PKG.parent
 CSRC = PKG / "csrc"
 LIB = PKG / "libcudabridge.so"
-SOURCES = [CSRC / "bridge.cu"]
+OBJ_DIR = PKG / "build"
+SOURCES = [CSRC / "bridge.cu", CSRC / "paged.cu"]
 HEADERS = sorted(CSRC.glob("*.cuh")) + sorted(CSRC.glob("*.h")) + [ROOT / "include" / "cuda_bridge.h"]
 
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a",
     "-O3", "-lineinfo", "-std=c++17",
-    "-Xcompiler", "-fPIC", "-shared",
+    "-Xcompiler", "-fPIC",
     "--expt-relaxed-constexpr",
 ]
 
@@ -49,6 +50,17 @@ def needs_build() -> bool:
     return any(p.stat().st_mtime > t for p in SOURCES + HEADERS if p.exists())
 
 
+def _object_is_current(obj: Path, cmd: str) -> bool:
+    """Whether an object is newer than everything its last compile read (nvcc's own list,
+    -MD) and was made by the same command."""
+    deps, made_by = obj.with_suffix(".d"), obj.with_suffix(".cmd")
+    if not (obj.exists() and deps.exists() and made_by.exists()) or made_by.read_text() != cmd:
+        return False
+    files = deps.read_text().replace("\\\n", " ").split(":", 1)[1].split()
+    t = obj.stat().st_mtime
+    return all(os.path.exists(f) and os.stat(f).st_mtime <= t for f in files)
+
+
 def build(force: bool = False, verbose: bool = False) -> Path:
     if not force and not needs_build():
         return LIB
@@ -58,8 +70,31 @@ def build(force: bool = False, verbose: bool = False) -> Path:
     extra = [f"-I{inc}"]
     if nccl_lib is not None:
         extra.append(f'-DCB_NCCL_DEFAULT_PATH="{nccl_lib}"')
-    cmd = [nvcc_path(), *NVCC_FLAGS, f"-I{ROOT / 'include'}", f"-I{CSRC}", *extra,
-           "-o", str(LIB), *map(str, SOURCES), "-ldl", "-lpthread"]
+    OBJ_DIR.mkdir(exist_ok=True)
+    running = []
+    for src in SOURCES:  # the sources compile side by side
+        obj = OBJ_DIR / (src.stem + ".o")
+        cmd = [nvcc_path(), *NVCC_FLAGS, f"-I{ROOT / 'include'}", f"-I{CSRC}", *extra,
+               "-MD", "-MF", str(obj.with_suffix(".d")), "-c", "-o", str(obj), str(src)]
+        line = " ".join(cmd)
+        if not force and _object_is_current(obj, line):
+            continue
+        if verbose:
+            print(line, file=sys.stderr)
+        obj.unlink(missing_ok=True)
+        running.append((obj, line, subprocess.Popen(cmd, stdout=subprocess.PIPE,
+                                                    stderr=subprocess.STDOUT, text=True)))
+    failed = []
+    for obj, line, p in running:
+        out, _ = p.communicate()
+        if p.returncode != 0:
+            failed.append(f"nvcc failed ({p.returncode}):\n{out}")
+        else:
+            obj.with_suffix(".cmd").write_text(line)
+    if failed:
+        raise RuntimeError("\n".join(failed))
+    cmd = [nvcc_path(), *NVCC_FLAGS, "-shared", "-o", str(LIB),
+           *(str(OBJ_DIR / (s.stem + ".o")) for s in SOURCES), "-ldl", "-lpthread"]
     if verbose:
         print(" ".join(cmd), file=sys.stderr)
     r = subprocess.run(cmd, capture_output=True, text=True)

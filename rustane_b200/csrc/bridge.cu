@@ -49,6 +49,7 @@
 #include "io.cuh"
 #include "ptx.cuh"
 #include "rowwise.cuh"
+#include "tensor_map.h"
 #include "weights.cuh"
 
 using namespace cb;
@@ -58,25 +59,6 @@ using namespace cb;
 namespace {
 
 // ------------------------------------------------------------ tensor maps
-typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*,
-                                  const cuuint64_t*, const cuuint64_t*, const cuuint32_t*,
-                                  const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
-                                  CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
-
-EncodeTiledFn encode_fn() {
-  static EncodeTiledFn fn = nullptr;
-  static std::once_flag once;
-  std::call_once(once, [] {
-    void* p = nullptr;
-    cudaDriverEntryPointQueryResult q;
-    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) ==
-            cudaSuccess &&
-        q == cudaDriverEntryPointSuccess)
-      fn = reinterpret_cast<EncodeTiledFn>(p);
-  });
-  return fn;
-}
-
 // fp16 tensor [depth][rows][k] (k contiguous) tiled as 64 x box_rows x 1 boxes, 128B swizzle.
 bool make_tmap(CUtensorMap* map, const void* ptr, uint64_t k, uint64_t rows, uint64_t depth,
                uint32_t box_rows) {

@@ -1,0 +1,497 @@
+// C entry points of the paged KV cache and of the rotary embedding (include/cuda_bridge.h,
+// "Serving from a paged KV cache"). Each call checks its arguments on the host, holds what
+// only the device knows to the descriptor's bounds in the kernels, and enqueues its kernels
+// without allocating or synchronising.
+#include <cuda.h>
+#include <cuda_runtime.h>
+
+#include <algorithm>
+#include <atomic>
+#include <cmath>
+#include <cstdint>
+#include <limits>
+
+#include "cuda_bridge.h"
+#include "paged_attention.cuh"
+#include "paged_common.cuh"
+#include "paged_evict.cuh"
+#include "paged_rope.cuh"
+#include "tensor_map.h"
+
+using namespace cb;
+
+namespace {
+
+constexpr int PG_SMS = 148;  // of a B200: the plans below are made for it, without a GPU
+constexpr int64_t INT_LIMIT = std::numeric_limits<int32_t>::max();
+
+// ------------------------------------------------------------------------ checks
+bool aligned(const void* p, uintptr_t a) { return (reinterpret_cast<uintptr_t>(p) & (a - 1)) == 0; }
+
+bool dtype_ok(int32_t d) { return d == CB_DTYPE_F16 || d == CB_DTYPE_BF16; }
+
+// Sizes of a descriptor (no pointers).
+bool kv_sizes_ok(const cb_paged_kv* kv) {
+  if (!kv || !dtype_ok(kv->dtype)) return false;
+  if (kv->page_size != 16 && kv->page_size != 32 && kv->page_size != 64 && kv->page_size != 128)
+    return false;
+  if (kv->pages <= 0 || kv->kv_heads <= 0 || kv->batch <= 0 || kv->table_stride <= 0 ||
+      kv->max_len <= 0 || kv->rows < 0 || kv->max_new < 0 || kv->max_new > kv->rows)
+    return false;
+  if (kv->max_len > (int64_t)kv->table_stride * kv->page_size) return false;
+  // cache rows are TMA coordinates (a tile's worth of head room)
+  return (double)kv->pages * kv->kv_heads * kv->page_size < (double)(INT_LIMIT - 1024) &&
+         kv->batch < INT_LIMIT - 64 && kv->max_len < INT_LIMIT / 2;
+}
+
+bool kv_pointers_ok(const cb_paged_kv* kv, bool rows_needed) {
+  if (!kv->k || !kv->v || !kv->table || !kv->len || (rows_needed && !kv->row_start)) return false;
+  return aligned(kv->k, 16) && aligned(kv->v, 16) && aligned(kv->table, 4) &&
+         aligned(kv->len, 4) && aligned(kv->row_start, 4);
+}
+
+bool heads_ok(const cb_paged_kv* kv, int32_t heads) {
+  return heads > 0 && heads % kv->kv_heads == 0 && (int64_t)kv->rows * heads <= INT_LIMIT &&
+         (int64_t)kv->max_new * heads <= INT_LIMIT;
+}
+
+// A token array: [rows][width] elements of two bytes.
+bool array_ok(const void* p, int64_t stride, int64_t width) {
+  return p && aligned(p, 16) && stride >= width && stride % 8 == 0 && stride <= (int64_t(1) << 40);
+}
+
+// Whether two token arrays share an element. Columns of one wider array do not.
+bool arrays_overlap(const void* a, int64_t a_stride, int64_t a_width, const void* b,
+                    int64_t b_stride, int64_t b_width, int64_t rows) {
+  const int64_t pa = reinterpret_cast<intptr_t>(a), pb = reinterpret_cast<intptr_t>(b);
+  const int64_t ea = pa + ((rows - 1) * a_stride + a_width) * 2;
+  const int64_t eb = pb + ((rows - 1) * b_stride + b_width) * 2;
+  if (ea <= pb || eb <= pa) return false;
+  if (a_stride != b_stride) return true;
+  const int64_t s = a_stride * 2, off = ((pb - pa) % s + s) % s;
+  return !(off >= a_width * 2 && off + b_width * 2 <= s);
+}
+
+bool ranges_overlap(const void* a, int64_t a_bytes, const void* b, int64_t b_bytes) {
+  const int64_t pa = reinterpret_cast<intptr_t>(a), pb = reinterpret_cast<intptr_t>(b);
+  return pa < pb + b_bytes && pb < pa + a_bytes;
+}
+
+// The current device is a B200 and every (non-null) pointer is memory of it.
+cb_status check_device(std::initializer_list<const void*> pointers) {
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess) {
+    cudaGetLastError();  // not the next call's error
+    return CB_ERR_CUDA;
+  }
+  static std::atomic<uint64_t> known{0};  // bit per device that was found to be one
+  if (dev >= 64 || !(known.load(std::memory_order_relaxed) >> dev & 1)) {
+    int major = 0, minor = 0;
+    if (cudaDeviceGetAttribute(&major, cudaDevAttrComputeCapabilityMajor, dev) != cudaSuccess ||
+        cudaDeviceGetAttribute(&minor, cudaDevAttrComputeCapabilityMinor, dev) != cudaSuccess) {
+      cudaGetLastError();
+      return CB_ERR_CUDA;
+    }
+    if (major != 10 || minor != 0) return CB_ERR_UNSUPPORTED;
+    if (dev < 64) known.fetch_or(uint64_t(1) << dev, std::memory_order_relaxed);
+  }
+  for (const void* p : pointers) {
+    if (!p) continue;
+    cudaPointerAttributes a;
+    if (cudaPointerGetAttributes(&a, p) != cudaSuccess) {
+      cudaGetLastError();
+      return CB_ERR_INVALID_ARG;
+    }
+    if (!(a.type == cudaMemoryTypeDevice && a.device == dev) && a.type != cudaMemoryTypeManaged)
+      return CB_ERR_INVALID_ARG;
+  }
+  return CB_OK;
+}
+
+PagedKV device_kv(const cb_paged_kv* kv) {
+  PagedKV d;
+  d.k = kv->k;
+  d.v = kv->v;
+  d.table = kv->table;
+  d.len = kv->len;
+  d.row_start = kv->row_start;
+  d.pages = kv->pages;
+  d.kv_heads = kv->kv_heads;
+  d.page_size = kv->page_size;
+  d.page_shift = kv->page_size == 16 ? 4 : kv->page_size == 32 ? 5 : kv->page_size == 64 ? 6 : 7;
+  d.batch = kv->batch;
+  d.table_stride = kv->table_stride;
+  d.max_len = kv->max_len;
+  d.rows = kv->rows;
+  d.max_new = kv->max_new;
+  return d;
+}
+
+cb_status status_of(cudaError_t e) {
+  if (e == cudaSuccess) return CB_OK;
+  cudaGetLastError();
+  return CB_ERR_CUDA;
+}
+
+// Dynamic shared memory above 48 KB is asked for once per kernel and device.
+template <typename F>
+cudaError_t allow_smem(F* kernel, int bytes, std::atomic<uint64_t>& done) {
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return e;
+  if (dev < 64 && (done.load(std::memory_order_acquire) >> dev & 1)) return cudaSuccess;
+  e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  if (e == cudaSuccess && dev < 64) done.fetch_or(uint64_t(1) << dev, std::memory_order_release);
+  return e;
+}
+
+// The cache as a [rows][128] matrix in boxes of box_rows x 64 elements, 128-byte swizzle.
+// (Both types are two bytes and out-of-range rows read as zero bytes: one element type does.)
+bool make_cache_map(CUtensorMap* map, const void* ptr, const cb_paged_kv* kv, uint32_t box_rows) {
+  EncodeTiledFn enc = encode_fn();
+  if (!enc) return false;
+  cuuint64_t dims[2] = {(cuuint64_t)PG_HD, (cuuint64_t)kv->pages * kv->kv_heads * kv->page_size};
+  cuuint64_t strides[1] = {PG_HD * 2};
+  cuuint32_t box[2] = {64, box_rows};
+  cuuint32_t estr[2] = {1, 1};
+  return enc(map, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2, const_cast<void*>(ptr), dims, strides, box,
+             estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+             CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
+
+// ------------------------------------------------------------------- attention plan
+struct AttentionPlan {
+  int64_t tiles;  // an upper bound: the device knows how many there are
+  int splits;
+  int keys;  // keys of a split
+  size_t parts;
+  size_t bytes() const { return splits > 1 ? parts * (PG_HD + 1) * sizeof(float) : 0; }
+};
+
+// Tiles of m query rows: no more than the rows need with one ragged tile per sequence, and
+// no more than batch x the tiles of the longest.
+int64_t tile_bound(const cb_paged_kv* kv, int group, int m) {
+  return std::min<int64_t>(kv->batch * ceil_div((int64_t)kv->max_new * group, m),
+                           ceil_div((int64_t)kv->rows * group, m) + kv->batch);
+}
+
+AttentionPlan plan_attention(const cb_paged_kv* kv, int32_t heads) {
+  AttentionPlan p;
+  p.tiles = tile_bound(kv, heads / kv->kv_heads, PR_ROWS);
+  // Two CTAs share an SM; four per SM in all leave the last ones little to wait for.
+  const int64_t want = 4 * PG_SMS, have = std::max<int64_t>(1, p.tiles * kv->kv_heads);
+  int64_t splits = std::min<int64_t>(ceil_div(want, have), ceil_div(kv->max_len, 256));
+  splits = std::max<int64_t>(1, splits);
+  p.keys = (int)(ceil_div(ceil_div(kv->max_len, splits), 16) * 16);
+  p.splits = (int)ceil_div(kv->max_len, p.keys);
+  p.parts = (size_t)kv->rows * heads * p.splits;
+  return p;
+}
+
+template <typename T>
+cb_status launch_attention(const cb_paged_kv* kv, const T* q, int64_t q_stride, int32_t heads,
+                           float scale, T* out, int64_t out_stride, float* lse, float* workspace,
+                           cudaStream_t st) {
+  const AttentionPlan p = plan_attention(kv, heads);
+  const int64_t grid = p.tiles * kv->kv_heads * p.splits;
+  if (grid > INT_LIMIT) return CB_ERR_UNSUPPORTED;
+  CUtensorMap tk, tv;
+  if (!make_cache_map(&tk, kv->k, kv, PR_BLOCK) || !make_cache_map(&tv, kv->v, kv, PR_BLOCK))
+    return CB_ERR_UNSUPPORTED;
+  static std::atomic<uint64_t> done{0};
+  cudaError_t e = allow_smem(paged_rows_kernel<T>, PR_SMEM, done);
+  if (e != cudaSuccess) return status_of(e);
+  const PagedKV d = device_kv(kv);
+  PagedParts parts{workspace, workspace ? workspace + p.parts * PG_HD : nullptr, p.splits, p.keys};
+  paged_rows_kernel<T><<<(unsigned)grid, PR_WARPS * 32, PR_SMEM, st>>>(
+      tk, tv, d, q, q_stride, heads, scale * 1.4426950408889634f, out, out_stride, lse, parts);
+  e = cudaPeekAtLastError();
+  if (e == cudaSuccess && p.splits > 1) {
+    const int64_t blocks = ceil_div((int64_t)kv->rows * heads, PC_WARPS);
+    paged_combine_kernel<T><<<(unsigned)blocks, PC_WARPS * 32, 0, st>>>(d, heads, parts, PR_ROWS,
+                                                                       out, out_stride, lse);
+    e = cudaPeekAtLastError();
+  }
+  return status_of(e);
+}
+
+// ---------------------------------------------------------------------- evict plan
+template <int THREADS, int PER>
+cudaError_t launch_evict(const PagedKV& kv, const EvictArgs& a, int ctas, cudaStream_t st) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)((int64_t)kv.batch * kv.kv_heads * ctas));
+  cfg.blockDim = dim3(THREADS);
+  cfg.stream = st;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = ctas;
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = ctas > 1 ? 1 : 0;
+  return cudaLaunchKernelEx(&cfg, paged_evict_kernel<THREADS, PER>, kv, a, ctas);
+}
+
+}  // namespace
+
+extern "C" {
+
+cb_status cb_rope_frequencies(int32_t rot_dim, const cb_rope_scaling* scaling, double* inv_freq,
+                              float* amplitude) {
+  if (!scaling || !inv_freq || rot_dim <= 0 || rot_dim % 8 != 0) return CB_ERR_INVALID_ARG;
+  const cb_rope_scaling& s = *scaling;
+  if (!(s.base > 1.0) || !std::isfinite(s.base)) return CB_ERR_INVALID_ARG;
+  if (s.kind < CB_ROPE_SCALE_NONE || s.kind > CB_ROPE_SCALE_PARTS) return CB_ERR_INVALID_ARG;
+  if (s.kind != CB_ROPE_SCALE_NONE && (!(s.factor >= 1.0) || !std::isfinite(s.factor)))
+    return CB_ERR_INVALID_ARG;
+  double base = s.base;
+  if (s.kind == CB_ROPE_SCALE_BASE) base *= std::pow(s.factor, (double)rot_dim / (rot_dim - 2));
+  double lo = 0.0, hi = 0.0;
+  if (s.kind == CB_ROPE_SCALE_PARTS) {
+    if (!(s.original_len > 0.0) || !(s.slow_turns > 0.0) || !(s.fast_turns >= s.slow_turns) ||
+        !std::isfinite(s.original_len) || !std::isfinite(s.fast_turns))
+      return CB_ERR_INVALID_ARG;
+    // the pair that turns `turns` times within original_len: p f = 2 pi turns
+    const double two_pi = 6.283185307179586;
+    auto pair = [&](double turns) {
+      return rot_dim * std::log(s.original_len / (turns * two_pi)) / (2.0 * std::log(base));
+    };
+    lo = std::max(0.0, std::floor(pair(s.fast_turns)));
+    hi = std::min(rot_dim - 1.0, std::ceil(pair(s.slow_turns)));
+  }
+  for (int i = 0; i < rot_dim / 2; ++i) {
+    double f = std::pow(base, -2.0 * i / rot_dim);
+    if (s.kind == CB_ROPE_SCALE_LINEAR) f /= s.factor;
+    if (s.kind == CB_ROPE_SCALE_PARTS) {
+      const double ramp = std::min(1.0, std::max(0.0, (i - lo) / std::max(hi - lo, 0.001)));
+      f = f / s.factor * ramp + f * (1.0 - ramp);
+    }
+    inv_freq[i] = f;
+  }
+  if (amplitude)
+    *amplitude = s.kind == CB_ROPE_SCALE_PARTS ? (float)(0.1 * std::log(s.factor) + 1.0) : 1.0f;
+  return CB_OK;
+}
+
+static bool rope_config_ok(const cb_rope_config* r, int32_t head_dim) {
+  return r && r->inv_freq && aligned(r->inv_freq, 8) && r->rot_dim > 0 && r->rot_dim % 8 == 0 &&
+         r->rot_dim <= head_dim &&
+         (r->layout == CB_ROPE_HALF || r->layout == CB_ROPE_INTERLEAVED) &&
+         std::isfinite(r->amplitude);
+}
+
+cb_status cb_rope(const cb_rope_config* rope, int32_t dtype, const void* x, int64_t x_stride,
+                  void* y, int64_t y_stride, const int32_t* positions, int32_t tokens,
+                  int32_t heads, int32_t head_dim, int32_t inverse, void* stream) {
+  if (!dtype_ok(dtype) || head_dim <= 0 || head_dim % 8 != 0 || head_dim > 512 || heads <= 0 ||
+      tokens < 0 || inverse < 0 || inverse > 1 || !rope_config_ok(rope, head_dim))
+    return CB_ERR_INVALID_ARG;
+  const int64_t width = (int64_t)heads * head_dim;
+  if (!positions || !aligned(positions, 4) || width > INT_LIMIT || !array_ok(x, x_stride, width) ||
+      !array_ok(y, y_stride, width))
+    return CB_ERR_INVALID_ARG;
+  if (tokens == 0) return CB_OK;
+  if (!(x == y && x_stride == y_stride) &&
+      arrays_overlap(x, x_stride, width, y, y_stride, width, tokens))
+    return CB_ERR_INVALID_ARG;
+  const cb_status s = check_device({x, y, positions, rope->inv_freq});
+  if (s != CB_OK) return s;
+  // Heads of a thread: enough to spread an angle's cost, few enough to fill the GPU.
+  const int64_t units = (int64_t)tokens * heads * (head_dim / 8);
+  const int per_thread = units >= (int64_t)PG_SMS * 2048 * 4 ? 4 : 1;
+  const int64_t threads = (int64_t)tokens * ceil_div(heads, per_thread) * (head_dim / 8);
+  const int64_t blocks = ceil_div(threads, ROPE_THREADS);
+  if (blocks > INT_LIMIT) return CB_ERR_UNSUPPORTED;
+  const bool half = rope->layout == CB_ROPE_HALF;
+  const float amp = rope->amplitude, amp_sin = inverse ? -amp : amp;
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  if (dtype == CB_DTYPE_F16)
+    rope_kernel<__half><<<(unsigned)blocks, ROPE_THREADS, 0, st>>>(
+        static_cast<const __half*>(x), x_stride, static_cast<__half*>(y), y_stride, positions,
+        rope->inv_freq, rope->rot_dim, half, amp, amp_sin, tokens, heads, head_dim, per_thread);
+  else
+    rope_kernel<__nv_bfloat16><<<(unsigned)blocks, ROPE_THREADS, 0, st>>>(
+        static_cast<const __nv_bfloat16*>(x), x_stride, static_cast<__nv_bfloat16*>(y), y_stride,
+        positions, rope->inv_freq, rope->rot_dim, half, amp, amp_sin, tokens, heads, head_dim,
+        per_thread);
+  return status_of(cudaPeekAtLastError());
+}
+
+cb_status cb_paged_append(const cb_paged_kv* kv, const cb_rope_config* rope, int32_t heads,
+                          const void* q, int64_t q_stride, void* q_out, int64_t q_out_stride,
+                          const void* k, int64_t k_stride, const void* v, int64_t v_stride,
+                          const int32_t* positions, float* weights, int32_t* slot_positions,
+                          void* stream) {
+  if (!kv_sizes_ok(kv) || !kv_pointers_ok(kv, true)) return CB_ERR_INVALID_ARG;
+  if (rope && !rope_config_ok(rope, PG_HD)) return CB_ERR_INVALID_ARG;
+  if (!q != !q_out || (q && !heads_ok(kv, heads))) return CB_ERR_INVALID_ARG;
+  if (!q) heads = 0;
+  const int64_t q_width = (int64_t)heads * PG_HD, kv_width = (int64_t)kv->kv_heads * PG_HD;
+  if (q && (!array_ok(q, q_stride, q_width) || !array_ok(q_out, q_out_stride, q_width)))
+    return CB_ERR_INVALID_ARG;
+  if (!array_ok(k, k_stride, kv_width) || !array_ok(v, v_stride, kv_width) ||
+      !aligned(positions, 4) || !aligned(weights, 4) || !aligned(slot_positions, 4))
+    return CB_ERR_INVALID_ARG;
+  if (kv->rows == 0 || kv->max_new == 0) return CB_OK;
+  const int64_t rows = kv->rows;
+  if (q && !(q == q_out && q_stride == q_out_stride) &&
+      arrays_overlap(q, q_stride, q_width, q_out, q_out_stride, q_width, rows))
+    return CB_ERR_INVALID_ARG;
+  if (q && (arrays_overlap(q_out, q_out_stride, q_width, k, k_stride, kv_width, rows) ||
+            arrays_overlap(q_out, q_out_stride, q_width, v, v_stride, kv_width, rows)))
+    return CB_ERR_INVALID_ARG;
+  const cb_status s =
+      check_device({kv->k, kv->v, kv->table, kv->len, kv->row_start, rope ? rope->inv_freq : nullptr,
+                    q, q_out, k, v, positions, weights, slot_positions});
+  if (s != CB_OK) return s;
+  const int all = heads + 2 * kv->kv_heads;
+  // Heads of a warp: two at a time; more of them where there are warps enough.
+  const int per_warp = rows * all / 8 >= (int64_t)PG_SMS * 64 ? 8 : 2;
+  const int64_t warps = rows * ceil_div(all, per_warp);
+  const int64_t blocks = ceil_div(warps, APPEND_WARPS);
+  if (blocks > INT_LIMIT) return CB_ERR_UNSUPPORTED;
+  const double* freq = rope ? rope->inv_freq : nullptr;
+  const int rot = rope ? rope->rot_dim : 0;
+  const bool half = rope && rope->layout == CB_ROPE_HALF;
+  const float amp = rope ? rope->amplitude : 1.0f;
+  const PagedKV d = device_kv(kv);
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  if (kv->dtype == CB_DTYPE_F16) {
+    using T = __half;
+    paged_append_kernel<T><<<(unsigned)blocks, APPEND_WARPS * 32, 0, st>>>(
+        d, static_cast<const T*>(q), q_stride, static_cast<T*>(q_out), q_out_stride, heads,
+        static_cast<const T*>(k), k_stride, static_cast<const T*>(v), v_stride, positions, freq, rot,
+        half, amp, weights, slot_positions, per_warp);
+  } else {
+    using T = __nv_bfloat16;
+    paged_append_kernel<T><<<(unsigned)blocks, APPEND_WARPS * 32, 0, st>>>(
+        d, static_cast<const T*>(q), q_stride, static_cast<T*>(q_out), q_out_stride, heads,
+        static_cast<const T*>(k), k_stride, static_cast<const T*>(v), v_stride, positions, freq, rot,
+        half, amp, weights, slot_positions, per_warp);
+  }
+  return status_of(cudaPeekAtLastError());
+}
+
+cb_status cb_paged_attention_workspace(const cb_paged_kv* kv, int32_t heads, size_t* bytes) {
+  if (!bytes || !kv_sizes_ok(kv) || !heads_ok(kv, heads)) return CB_ERR_INVALID_ARG;
+  *bytes = plan_attention(kv, heads).bytes();
+  return CB_OK;
+}
+
+cb_status cb_paged_attention(const cb_paged_kv* kv, const void* q, int64_t q_stride,
+                             int32_t heads, float scale, void* out, int64_t out_stride,
+                             float* lse, void* workspace, size_t workspace_bytes, void* stream) {
+  if (!kv_sizes_ok(kv) || !kv_pointers_ok(kv, true) || !heads_ok(kv, heads))
+    return CB_ERR_INVALID_ARG;
+  const int64_t width = (int64_t)heads * PG_HD;
+  if (!(scale > 0.0f) || !std::isfinite(scale) || !array_ok(q, q_stride, width) ||
+      !array_ok(out, out_stride, width) || !aligned(lse, 4) || !aligned(workspace, 16))
+    return CB_ERR_INVALID_ARG;
+  const size_t need = plan_attention(kv, heads).bytes();
+  if (need > 0 && (!workspace || workspace_bytes < need)) return CB_ERR_INVALID_ARG;
+  if (kv->rows == 0 || kv->max_new == 0) return CB_OK;
+  if (arrays_overlap(q, q_stride, width, out, out_stride, width, kv->rows))
+    return CB_ERR_INVALID_ARG;
+  const cb_status s = check_device({kv->k, kv->v, kv->table, kv->len, kv->row_start, q, out, lse,
+                                    need > 0 ? workspace : nullptr});
+  if (s != CB_OK) return s;
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  float* ws = need > 0 ? static_cast<float*>(workspace) : nullptr;
+  if (kv->dtype == CB_DTYPE_F16)
+    return launch_attention(kv, static_cast<const __half*>(q), q_stride, heads, scale,
+                            static_cast<__half*>(out), out_stride, lse, ws, st);
+  return launch_attention(kv, static_cast<const __nv_bfloat16*>(q), q_stride, heads, scale,
+                          static_cast<__nv_bfloat16*>(out), out_stride, lse, ws, st);
+}
+
+cb_status cb_paged_attention_weights(const cb_paged_kv* kv, const void* q, int64_t q_stride,
+                                     int32_t heads, float scale, const float* lse,
+                                     float* weights, void* stream) {
+  if (!kv_sizes_ok(kv) || !kv_pointers_ok(kv, true) || !heads_ok(kv, heads))
+    return CB_ERR_INVALID_ARG;
+  if (!(scale > 0.0f) || !std::isfinite(scale) || !array_ok(q, q_stride, (int64_t)heads * PG_HD) ||
+      !lse || !weights || !aligned(lse, 4) || !aligned(weights, 4))
+    return CB_ERR_INVALID_ARG;
+  if (kv->rows == 0 || kv->max_new == 0) return CB_OK;
+  const cb_status s =
+      check_device({kv->k, kv->table, kv->len, kv->row_start, q, lse, weights});
+  if (s != CB_OK) return s;
+  const int blocks = (int)ceil_div(kv->max_len, PW_KEYS);
+  const int64_t grid = (int64_t)kv->batch * blocks * kv->kv_heads;
+  if (grid > INT_LIMIT) return CB_ERR_UNSUPPORTED;
+  const PagedKV d = device_kv(kv);
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  const float scale_log2 = scale * 1.4426950408889634f;
+  if (kv->dtype == CB_DTYPE_F16)
+    paged_weights_kernel<__half><<<(unsigned)grid, PW_WARPS * 32, 0, st>>>(
+        d, static_cast<const __half*>(q), q_stride, heads, scale_log2, lse, weights, blocks);
+  else
+    paged_weights_kernel<__nv_bfloat16><<<(unsigned)grid, PW_WARPS * 32, 0, st>>>(
+        d, static_cast<const __nv_bfloat16*>(q), q_stride, heads, scale_log2, lse, weights, blocks);
+  return status_of(cudaPeekAtLastError());
+}
+
+static size_t evict_list(const cb_paged_kv* kv, int32_t budget) {
+  return (size_t)std::min(budget, kv->max_len);
+}
+
+cb_status cb_paged_evict_workspace(const cb_paged_kv* kv, int32_t budget, size_t* bytes) {
+  if (!bytes || !kv_sizes_ok(kv) || budget <= 0) return CB_ERR_INVALID_ARG;
+  *bytes = (size_t)kv->batch * kv->kv_heads * 2 * evict_list(kv, budget) * sizeof(int32_t);
+  return CB_OK;
+}
+
+cb_status cb_paged_evict(const cb_paged_kv* kv, const float* weights, float* weights_out,
+                         const int32_t* positions, int32_t* positions_out,
+                         const int32_t* next_position, int32_t budget, int32_t sinks,
+                         int32_t recent, int32_t* len_out, void* workspace,
+                         size_t workspace_bytes, void* stream) {
+  if (!kv_sizes_ok(kv) || !kv_pointers_ok(kv, false)) return CB_ERR_INVALID_ARG;
+  if (!weights || !weights_out || !positions || !positions_out || !next_position || !len_out ||
+      !workspace || budget <= 0 || sinks < 0 || recent < 0 || (int64_t)sinks + recent > budget)
+    return CB_ERR_INVALID_ARG;
+  if (!aligned(weights, 4) || !aligned(weights_out, 4) || !aligned(positions, 4) ||
+      !aligned(positions_out, 4) || !aligned(next_position, 4) || !aligned(len_out, 4) ||
+      !aligned(workspace, 16))
+    return CB_ERR_INVALID_ARG;
+  size_t need = 0;
+  cb_paged_evict_workspace(kv, budget, &need);
+  if (workspace_bytes < need) return CB_ERR_INVALID_ARG;
+  const int64_t meta = (int64_t)kv->pages * kv->kv_heads * kv->page_size * 4;
+  if ((weights != weights_out && ranges_overlap(weights, meta, weights_out, meta)) ||
+      (positions != positions_out && ranges_overlap(positions, meta, positions_out, meta)) ||
+      ranges_overlap(len_out, kv->batch * 4ll, kv->len, kv->batch * 4ll) ||
+      ranges_overlap(weights_out, meta, positions_out, meta))
+    return CB_ERR_INVALID_ARG;
+  if (kv->max_len > EV_MAX_LEN) return CB_ERR_UNSUPPORTED;
+  const cb_status s = check_device({kv->k, kv->v, kv->table, kv->len, weights, weights_out,
+                                    positions, positions_out, next_position, len_out, workspace});
+  if (s != CB_OK) return s;
+  const int64_t items = (int64_t)kv->batch * kv->kv_heads;
+  if (items * EV_MAX_CTAS > INT_LIMIT) return CB_ERR_UNSUPPORTED;
+  const PagedKV d = device_kv(kv);
+  const EvictArgs a{weights, weights_out, positions, positions_out, next_position, budget, sinks,
+                    recent, len_out, static_cast<int*>(workspace), (int)evict_list(kv, budget)};
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  // The smallest form that holds the longest sequence; long ones are spread over a cluster.
+  const int n = kv->max_len;
+  cudaError_t e;
+  if (n <= 256 * 4)
+    e = launch_evict<256, 4>(d, a, 1, st);
+  else if (n <= 1024 * 4)
+    e = launch_evict<1024, 4>(d, a, 1, st);
+  else if (n <= 1024 * 4 * 2)
+    e = launch_evict<1024, 4>(d, a, 2, st);
+  else if (n <= 1024 * 4 * 4)
+    e = launch_evict<1024, 4>(d, a, 4, st);
+  else if (n <= 1024 * 4 * 8)
+    e = launch_evict<1024, 4>(d, a, 8, st);
+  else
+    e = launch_evict<EV_MAX_THREADS, EV_MAX_PER_THREAD>(d, a, EV_MAX_CTAS, st);
+  return status_of(e);
+}
+
+}  // extern "C"

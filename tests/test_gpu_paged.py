@@ -1,0 +1,423 @@
+"""GPU tests of the paged-cache operators against 64-bit forms (tests/paged_ref.py), whose
+tolerances are derived there."""
+import ctypes as C
+import math
+
+import pytest
+import torch
+
+import paged_ref as R
+from paged_ref import Cache, ptr, stream
+from rustane_b200 import bridge as B
+
+pytestmark = pytest.mark.gpu
+SCALE = 1 / math.sqrt(128)
+
+
+def close(got, want, tol, what=""):
+    got, want = got.double(), want.double()
+    assert not bool(torch.isnan(got).any()), f"{what}: NaN"
+    inf = torch.isinf(want)
+    assert bool((got[inf] == want[inf]).all()), f"{what}: infinities differ"
+    over = ((got - want).abs() - tol)[~inf]
+    assert over.numel() == 0 or float(over.max()) <= 0.0, \
+        f"{what}: off by {float((got - want).abs()[~inf].max()):.3g}, over the bound by {float(over.max()):.3g}"
+
+
+# ------------------------------------------------------------------------------- rope
+def _inv(rot, scaling=0):
+    lib = B.load_library()
+    s = B.cb_rope_scaling(10000.0, scaling, 8.0, 4096.0, 32.0, 1.0)
+    inv, amp = (C.c_double * (rot // 2))(), C.c_float()
+    assert lib.cb_rope_frequencies(rot, C.byref(s), inv, C.byref(amp)) == 0
+    return torch.tensor(list(inv), dtype=torch.float64, device="cuda"), amp.value
+
+
+LAYOUT = {"half": B.CB_ROPE_HALF, "interleaved": B.CB_ROPE_INTERLEAVED}
+
+
+def _rope(lib, x, y, pos, inv, amp, layout, rot, inverse, hd, dtype, st=None):
+    t, w = x.shape
+    cfg = B.cb_rope_config(inv.data_ptr(), rot, LAYOUT[layout], amp)
+    return lib.cb_rope(C.byref(cfg), R.CODES[dtype], ptr(x), x.stride(0), ptr(y), y.stride(0),
+                       ptr(pos), t, w // hd, hd, int(inverse), st or stream())
+
+
+@pytest.mark.parametrize("layout", ["half", "interleaved"])
+@pytest.mark.parametrize("dtype,tokens,heads,hd,rot,scaling,far", [
+    ("f16", 1, 1, 8, 8, 0, 10),
+    ("bf16", 3, 5, 64, 24, 1, 5000),
+    ("f16", 129, 7, 128, 128, 0, 2_000_000),
+    ("bf16", 257, 12, 128, 64, 3, 2_000_000),
+    ("f16", 65, 3, 96, 96, 2, 100_000),
+    ("bf16", 33, 2, 512, 512, 3, 2 ** 31 - 1),
+    ("f16", 4096, 32, 128, 128, 3, 32768),   # enough work for four heads a thread
+    ("bf16", 2048, 53, 128, 120, 0, 32768),  # a head count that four does not divide
+])
+def test_rope_and_its_gradient(bridge_lib, layout, dtype, tokens, heads, hd, rot, scaling, far):
+    dt = R.DTYPES[dtype]
+    g = torch.Generator(device="cuda").manual_seed(tokens + rot)
+    inv, amp = _inv(rot, scaling)
+    x = torch.randn(tokens, heads * hd + 16, device="cuda", generator=g).to(dt)[:, :heads * hd]
+    pos = torch.randint(-far, far, (tokens,), device="cuda", generator=g).int()
+    wide = torch.full((tokens, heads * hd + 24), 7.0, device="cuda", dtype=dt)
+    y = wide[:, :heads * hd]
+    for inverse in (False, True):
+        assert _rope(bridge_lib, x, y, pos, inv, amp, layout, rot, inverse, hd, dtype) == 0
+        torch.cuda.synchronize()
+        want, size = R.rotate_ref(x.unflatten(1, (heads, hd)), pos, inv, amp, layout, rot, inverse)
+        close(y.unflatten(1, (heads, hd)), want, R.rotate_tol(want, size, dt), f"inverse {inverse}")
+        assert bool((wide[:, heads * hd:] == 7.0).all())
+    in_place = x.clone()
+    assert _rope(bridge_lib, in_place, in_place, pos, inv, amp, layout, rot, True, hd, dtype) == 0
+    torch.cuda.synchronize()
+    assert torch.equal(in_place, y)
+
+
+def test_rope_gradient_is_the_transpose_and_agrees_with_differences(bridge_lib):
+    """<R x, g> = <x, R^T g>, and the change of <R x, g> along a direction d is <d, R^T g>."""
+    g = torch.Generator(device="cuda").manual_seed(3)
+    inv, amp = _inv(64, 3)
+    x, up, d = (torch.randn(50, 4 * 128, device="cuda", generator=g).half() for _ in range(3))
+    pos = torch.randint(0, 100_000, (50,), device="cuda", generator=g).int()
+
+    def run(a, inverse):
+        y = torch.empty_like(a)
+        assert _rope(bridge_lib, a, y, pos, inv, amp, "half", 64, inverse, 128, "f16") == 0
+        return y.double()
+    back = run(up, True)
+    # both products round once per element: half a step of each of 25600 terms
+    terms = (run(x, False) * up.double()).abs().sum() + (x.double() * back).abs().sum()
+    assert abs((run(x, False) * up.double()).sum() - (x.double() * back).sum()) <= terms * 2.0 ** -11
+    moved = (x.double() + d.double()).half()
+    step = moved.double() - x.double()  # exact: the step that was taken
+    change = ((run(moved, False) - run(x, False)) * up.double()).sum()
+    terms = ((run(moved, False).abs() + run(x, False).abs()) * up.double().abs()).sum() \
+        + (step * back).abs().sum()
+    assert abs(change - (step * back).sum()) <= terms * 2.0 ** -11
+
+
+def test_rope_matches_the_model_table(bridge_lib):
+    """Interleaved, whole head, base 10000: the rotation that the model's forward uses."""
+    inv, amp = _inv(128)
+    t = torch.arange(512, device="cuda", dtype=torch.int32)
+    x = torch.zeros(512, 128, device="cuda", dtype=torch.float16)
+    x[:, 0::2] = 1.0
+    y = torch.empty_like(x)
+    assert _rope(bridge_lib, x, y, t, inv, amp, "interleaved", 128, False, 128, "f16") == 0
+    i = torch.arange(64, device="cuda", dtype=torch.float64)
+    a = t.double()[:, None] * 10000.0 ** (-2 * i / 128)
+    torch.cuda.synchronize()
+    assert float((y[:, 0::2].double() - torch.cos(a)).abs().max()) <= 2.0 ** -11
+    assert float((y[:, 1::2].double() - torch.sin(a)).abs().max()) <= 2.0 ** -11
+
+
+# ----------------------------------------------------------------------------- append
+def _append(lib, c, rope, q, q_out, k, v, pos=None, w=None, sp=None, heads=None, st=None):
+    d = c.desc()
+    return lib.cb_paged_append(C.byref(d), C.byref(rope) if rope else None,
+                               c.heads if heads is None else heads, ptr(q),
+                               q.stride(0) if q is not None else 0, ptr(q_out),
+                               q_out.stride(0) if q_out is not None else 0, ptr(k), k.stride(0),
+                               ptr(v), v.stride(0), ptr(pos), ptr(w), ptr(sp), st or stream())
+
+
+APPENDS = [
+    # lens, news, heads, kv_heads, page, dtype, layout, rot, explicit positions
+    ([1], [1], 1, 1, 16, "f16", "half", 128, False),
+    ([5, 16, 17], [5, 1, 0], 4, 2, 16, "bf16", "interleaved", 128, True),
+    ([100, 33, 1, 64], [37, 33, 0, 1], 8, 1, 32, "f16", "half", 40, True),
+    ([300, 129], [300, 64], 6, 6, 128, "bf16", "half", 64, False),
+    ([40 + i for i in range(70)], [i % 3 for i in range(70)], 3, 3, 64, "f16", "interleaved", 8, True),
+    ([900, 1024, 700], [900, 1000, 640], 16, 16, 64, "bf16", "half", 128, True),
+]
+
+
+@pytest.mark.parametrize("lens,news,heads,kv_heads,page,dtype,layout,rot,explicit", APPENDS)
+def test_append(bridge_lib, lens, news, heads, kv_heads, page, dtype, layout, rot, explicit):
+    c = Cache(lens, news, heads, kv_heads, page, dtype, seed=len(lens) + heads)
+    total = c.starts[-1]
+    qkv = c.tokens((heads + 2 * kv_heads) * 128, stride=(heads + 2 * kv_heads) * 128 + 8)
+    q, k, v = qkv.split([heads * 128, kv_heads * 128, kv_heads * 128], 1)
+    q_out = torch.full((c.rows, heads * 128), 5.0, device="cuda", dtype=c.dt)
+    inv, amp = _inv(rot, 3)
+    rope = B.cb_rope_config(inv.data_ptr(), rot, LAYOUT[layout], amp)
+    slots = torch.cat([torch.arange(n - m, n) for n, m in zip(lens, news)]).int().cuda()
+    pos = slots + 100_003 if explicit else slots
+    given = torch.cat([pos, pos[:1].expand(c.rows - total)]).contiguous() if explicit else None
+    w = torch.full((c.pages, kv_heads, page), 3.0, device="cuda")
+    sp = torch.full((c.pages, kv_heads, page), -7, device="cuda", dtype=torch.int32)
+    k0, v0 = c.k.clone(), c.v.clone()
+    assert _append(bridge_lib, c, rope, q, q_out, k, v, given, w, sp) == 0
+    torch.cuda.synchronize()
+
+    def want(x, h):
+        y, size = R.rotate_ref(x[:total].unflatten(1, (h, 128)), pos, inv, amp, layout, rot)
+        return y, R.rotate_tol(y, size, c.dt)
+    close(q_out[:total].unflatten(1, (heads, 128)), *want(q, heads), "q")
+    assert bool((q_out[total:] == 5.0).all())  # padding
+    want_k, tol_k = want(k, kv_heads)
+    touched = torch.zeros(c.pages, kv_heads, page, dtype=torch.bool, device="cuda")
+    for b in range(c.batch):
+        span = slice(c.starts[b], c.starts[b + 1])
+        at = c.place(b, torch.arange(lens[b] - news[b], lens[b], device="cuda"))
+        for h in range(kv_heads):
+            close(c.k[at[0], h, at[1]], want_k[span, h], tol_k[span, h], "k")
+            assert torch.equal(c.v[at[0], h, at[1]], v[span].unflatten(1, (kv_heads, 128))[:, h])
+            assert bool((w[at[0], h, at[1]] == 0).all())
+            assert torch.equal(sp[at[0], h, at[1]], pos[span])
+            touched[at[0], h, at[1]] = True
+    for pool, before in ((c.k, k0), (c.v, v0)):
+        assert torch.equal(torch.nan_to_num(pool[~touched], 9.0), torch.nan_to_num(before[~touched], 9.0))
+    assert bool((w[~touched] == 3.0).all()) and bool((sp[~touched] == -7).all())
+
+
+def test_append_in_place_without_rotation_and_without_q(bridge_lib):
+    c = Cache([30, 9], [7, 9], 4, 2, 16, "f16", seed=2)
+    total = c.starts[-1]
+    q, k, v = c.tokens(512), c.tokens(256), c.tokens(256)
+    q0 = q.clone()
+    inv, amp = _inv(128)
+    rope = B.cb_rope_config(inv.data_ptr(), 128, B.CB_ROPE_HALF, amp)
+    apart = torch.zeros_like(q)
+    assert _append(bridge_lib, c, rope, q, apart, k, v) == 0
+    k_turned = c.k.clone()
+    assert _append(bridge_lib, c, rope, q, q, k, v) == 0
+    torch.cuda.synchronize()
+    assert torch.equal(q[:total], apart[:total]) and bool(q[total:].isnan().all())
+    assert _append(bridge_lib, c, rope, None, None, k, v, heads=0) == 0
+    torch.cuda.synchronize()
+    assert torch.equal(torch.nan_to_num(c.k), torch.nan_to_num(k_turned))
+    assert _append(bridge_lib, c, None, q0, q, k, v) == 0
+    torch.cuda.synchronize()
+    assert torch.equal(q[:total], q0[:total])
+    at = c.place(1, torch.arange(9, device="cuda"))
+    assert torch.equal(c.k[at[0], 1, at[1]], k[7:16, 128:])
+
+
+# -------------------------------------------------------------------------- attention
+ATTENTION = [
+    # lens, news, heads, kv_heads, page
+    ([1], [1], 1, 1, 16),
+    ([17], [1], 2, 1, 16),
+    ([5], [5], 1, 1, 16),
+    ([64, 1, 33, 128], [1, 1, 1, 1], 12, 12, 16),
+    ([700, 3, 0, 259], [1, 1, 0, 1], 8, 2, 32),
+    ([513], [1], 32, 1, 64),             # 32 query heads to one key head
+    ([40, 90, 300], [3, 0, 5], 6, 2, 32),
+    ([130, 77], [130, 20], 5, 1, 16),    # a whole prompt, five heads to a key head
+    ([400, 129, 64, 2], [129, 129, 1, 2], 4, 4, 128),
+    ([1000, 1500], [200, 333], 7, 1, 64),
+    ([9000], [1], 4, 4, 64),             # split over many parts
+    ([5000, 20, 3000], [1, 1, 2], 8, 4, 16),
+    ([4100, 260], [150, 256], 8, 2, 32),  # split with many rows
+    ([65, 64, 63] * 30, [1] * 90, 2, 2, 16),
+    ([300] * 40, [i % 4 for i in range(40)], 3, 1, 16),
+]
+
+
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("lens,news,heads,kv_heads,page", ATTENTION)
+def test_attention(bridge_lib, lens, news, heads, kv_heads, page, dtype):
+    c = Cache(lens, news, heads, kv_heads, page, dtype, seed=heads + len(lens))
+    total = c.starts[-1]
+    q = c.tokens(heads * 128, stride=heads * 128 + 64, scale=1.5)
+    wide = torch.full((c.rows, heads * 128 + 40), 3.0, device="cuda", dtype=c.dt)
+    out = wide[:, :heads * 128]
+    lse = torch.full((c.rows, heads), 3.0, device="cuda")
+    assert R.attention(bridge_lib, c, q, SCALE, out, lse) == 0
+    want, want_lse, tol, lse_tol = R.attention_ref(c, q, SCALE)
+    close(out[:total].unflatten(1, (heads, 128)), want, tol, "out")
+    close(lse[:total], want_lse, lse_tol, "lse")
+    assert bool((out[total:] == 3.0).all()) and bool((lse[total:] == 3.0).all())
+    assert bool((wide[:, heads * 128:] == 3.0).all())
+    # the same call without lse, and the same bits again
+    again = torch.full((c.rows, heads * 128), 3.0, device="cuda", dtype=c.dt)
+    assert R.attention(bridge_lib, c, q, SCALE, again) == 0
+    assert torch.equal(again, out)
+
+
+@pytest.mark.parametrize("new", [1, 40])
+def test_attention_rows_without_slots(bridge_lib, new):
+    """A sequence whose length is below its new tokens: the first rows see nothing."""
+    c = Cache([50, 50], [new, new], 4, 2, 16, "f16", seed=4)
+    c.len[0] = new - 1  # token 0 sees no slot
+    c.lens[0] = new - 1
+    q = c.tokens(512)
+    out = torch.full((c.rows, 512), 3.0, device="cuda", dtype=c.dt)
+    lse = torch.full((c.rows, 4), 3.0, device="cuda")
+    assert R.attention(bridge_lib, c, q, SCALE, out, lse) == 0
+    assert bool((out[0] == 0).all()) and bool((lse[0] == -math.inf).all())
+    live = torch.isfinite(lse[:2 * new]).all(1)
+    assert live.tolist() == [False] + [True] * (2 * new - 1)
+    assert not bool(out[:2 * new].isnan().any())
+
+
+@pytest.mark.parametrize("new", [1, 70])
+def test_attention_skips_pages_outside_the_pool(bridge_lib, new):
+    """Page ids outside 0 .. pages - 1 stand for absent slots: the result is that of a cache
+    without them."""
+    c = Cache([96], [new], 4, 2, 16, "bf16", seed=5)
+    q = c.tokens(512)
+    c.table[0, 1], c.table[0, 3] = -5, c.pages
+    out = torch.zeros(c.rows, 512, device="cuda", dtype=c.dt)
+    lse = torch.zeros(c.rows, 4, device="cuda")
+    assert R.attention(bridge_lib, c, q, SCALE, out, lse) == 0
+    absent = torch.zeros(96, dtype=torch.bool, device="cuda")
+    absent[16:32] = absent[48:64] = True
+    for head in range(2):
+        x, size = R.scores(c, q, 0, head, SCALE, 2)
+        x = x.masked_fill(absent, -math.inf)
+        w = torch.softmax(x, -1)
+        v = c.slots(c.v, 0, head).double()
+        want = (w @ v).transpose(0, 1)
+        tol = 2.0 ** -8 * want.abs() + (2.0 ** -8 + 2.0 ** -12) * (w @ v.abs()).transpose(0, 1)
+        close(out[:new].unflatten(1, (4, 128))[:, head * 2:head * 2 + 2], want, tol)
+
+
+def test_attention_holds_to_the_descriptor(bridge_lib):
+    """Lengths above max_len, more new tokens than max_new and row starts out of range: what
+    lies behind the bounds is left alone."""
+    c = Cache([64, 64], [4, 4], 2, 2, 16, "f16", seed=6, max_len=64, max_new=2)
+    q = c.tokens(256)
+    good = torch.full((c.rows, 256), 3.0, device="cuda", dtype=c.dt)
+    assert R.attention(bridge_lib, c, q, SCALE, good) == 0
+    assert bool((good[2:4] == 3.0).all()) and bool((good[6:] == 3.0).all())
+    assert not bool((good[[0, 1, 4, 5]] == 3.0).all(1).any())
+    c.len[:] = 2 ** 31 - 1
+    c.row_start[:] = torch.tensor([-9, 4, 2 ** 31 - 1], dtype=torch.int32)
+    out = torch.full((c.rows, 256), 3.0, device="cuda", dtype=c.dt)
+    assert R.attention(bridge_lib, c, q, SCALE, out) == 0
+    assert bool((out[[2, 3, 6, 7]] == 3.0).all())
+
+
+def test_attention_extreme_scores(bridge_lib):
+    """Scores of thousands, one key far above the others, and equal keys."""
+    c = Cache([200, 200, 200], [1, 1, 17], 2, 1, 16, "f16", seed=7)
+    q = c.tokens(256, scale=8.0)
+    at = c.place(0, torch.arange(200, device="cuda"))
+    c.k[at[0], 0, at[1]] *= 30
+    at = c.place(1, torch.arange(200, device="cuda"))
+    c.k[at[0], 0, at[1]] = 1.0
+    at = c.place(2, torch.arange(150, 160, device="cuda"))
+    c.k[at[0], 0, at[1]] *= 60
+    out = torch.zeros(c.rows, 256, device="cuda", dtype=c.dt)
+    lse = torch.zeros(c.rows, 2, device="cuda")
+    assert R.attention(bridge_lib, c, q, SCALE, out, lse) == 0
+    want, want_lse, tol, lse_tol = R.attention_ref(c, q, SCALE)
+    total = c.starts[-1]
+    close(out[:total].unflatten(1, (2, 128)), want, tol, "out")
+    close(lse[:total], want_lse, lse_tol, "lse")
+
+
+# ---------------------------------------------------------------------------- weights
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("lens,news,heads,kv_heads,page", ATTENTION)
+def test_weights(bridge_lib, lens, news, heads, kv_heads, page, dtype):
+    c = Cache(lens, news, heads, kv_heads, page, dtype, seed=heads + len(lens))
+    q = c.tokens(heads * 128, stride=heads * 128 + 64, scale=1.5)
+    _, lse64, _, _ = R.attention_ref(c, q, SCALE)
+    lse = torch.full((c.rows, heads), math.nan, device="cuda")
+    lse[:c.starts[-1]] = lse64.float()
+    w = torch.rand(c.pages, kv_heads, page, device="cuda")
+    before = w.clone()
+    d = c.desc()
+    assert bridge_lib.cb_paged_attention_weights(C.byref(d), ptr(q), q.stride(0), heads, SCALE,
+                                                 ptr(lse), ptr(w), stream()) == 0
+    torch.cuda.synchronize()
+    want, tol = R.weights_ref(c, q, SCALE, lse, before)
+    close(w, want, tol, "weights")
+    assert torch.equal(w[~c.live], before[~c.live])
+    w2 = before.clone()
+    assert bridge_lib.cb_paged_attention_weights(C.byref(d), ptr(q), q.stride(0), heads, SCALE,
+                                                 ptr(lse), ptr(w2), stream()) == 0
+    torch.cuda.synchronize()
+    assert torch.equal(w, w2)  # a fixed order of additions
+
+
+# ------------------------------------------------------------------------------ evict
+def _evict(lib, c, w, wo, p, po, nxt, budget, sinks, recent, lo, st=None):
+    d = c.desc()
+    size = C.c_size_t()
+    assert lib.cb_paged_evict_workspace(C.byref(d), budget, C.byref(size)) == 0
+    ws = torch.full((size.value + 64,), 0x5a, dtype=torch.uint8, device="cuda")
+    rc = lib.cb_paged_evict(C.byref(d), ptr(w), ptr(wo), ptr(p), ptr(po), ptr(nxt), budget, sinks,
+                            recent, ptr(lo), ptr(ws), size.value, st or stream())
+    torch.cuda.synchronize()
+    assert bool((ws[size.value:] == 0x5a).all())
+    return rc
+
+
+EVICTS = [
+    # lens, kv_heads, page, budget, sinks, recent, values of the weights
+    ([1], 1, 16, 1, 0, 0, "random"),
+    ([2], 1, 16, 1, 1, 0, "random"),
+    ([33, 32, 31, 0], 2, 16, 32, 4, 8, "random"),
+    ([100, 257, 40], 3, 32, 37, 0, 0, "equal"),
+    ([513] * 5, 4, 16, 512, 4, 64, "random"),
+    ([1000, 700], 2, 64, 300, 100, 200, "few"),
+    ([1000, 700], 2, 64, 300, 0, 300, "odd"),
+    ([1024, 1025], 2, 128, 1, 0, 0, "odd"),
+    ([4096, 4097, 900], 1, 64, 2000, 4, 100, "few"),
+    ([9000, 16384], 2, 128, 4000, 0, 64, "random"),
+    ([20000], 1, 32, 19999, 8, 1000, "equal"),
+    ([40000, 33000], 1, 128, 1000, 4, 0, "random"),
+]
+
+
+@pytest.mark.parametrize("in_place", [False, True])
+@pytest.mark.parametrize("lens,kv_heads,page,budget,sinks,recent,values", EVICTS)
+def test_evict(bridge_lib, lens, kv_heads, page, budget, sinks, recent, values, in_place):
+    c = Cache(lens, [0] * len(lens), kv_heads, kv_heads, page, "bf16", seed=sum(lens) + budget)
+    shape = (c.pages, kv_heads, page)
+    g = torch.Generator(device="cuda").manual_seed(budget)
+    w = torch.rand(shape, device="cuda", generator=g)
+    if values == "equal":
+        w[:] = 0.25
+    if values == "few":
+        w = (w * 4).floor()
+    if values == "odd":
+        pick = torch.randint(0, 8, shape, device="cuda", generator=g)
+        for i, x in enumerate((math.nan, math.inf, -math.inf, -0.0, 0.0, -1.5)):
+            w[pick == i] = x
+    p = torch.full(shape, -3, device="cuda", dtype=torch.int32)
+    for b in range(c.batch):
+        for h in range(kv_heads):
+            at = c.place(b, torch.arange(lens[b], device="cuda"))
+            p[at[0], h, at[1]] = torch.randperm(lens[b], device="cuda", generator=g).int() * 2
+    nxt = c.len * 2
+    wo = w if in_place else torch.full_like(w, 9.0)
+    po = p if in_place else torch.full_like(p, 9)
+    lo = torch.full_like(c.len, -1)
+    before = {n: t.clone() for n, t in (("k", c.k), ("v", c.v), ("w", w), ("p", p), ("wo", wo), ("po", po))}
+    moves = R.evict_ref(c, w, p, nxt, budget, sinks, recent)
+    assert _evict(bridge_lib, c, w, wo, p, po, nxt, budget, sinks, recent, lo) == 0
+    assert lo.tolist() == [min(n, budget) for n in lens]
+    want = {n: before[n].clone() for n in ("k", "v", "wo", "po")}
+    for (b, h), source in moves.items():
+        to = c.place(b, torch.arange(len(source), device="cuda"))
+        fro = c.place(b, torch.tensor(source, device="cuda", dtype=torch.long))
+        for name, start in (("k", "k"), ("v", "v"), ("wo", "w"), ("po", "p")):
+            want[name][to[0], h, to[1]] = before[start][fro[0], h, fro[1]]
+    for name, got in (("k", c.k), ("v", c.v)):
+        assert torch.equal(got.view(torch.int16), want[name].view(torch.int16)), name
+    assert torch.equal(wo.view(torch.int32), want["wo"].view(torch.int32))
+    assert torch.equal(po, want["po"])
+
+
+def test_evict_with_pages_outside_the_pool(bridge_lib):
+    """Absent slots go first and nothing is read from or written to them."""
+    c = Cache([64, 64], [0, 0], 1, 1, 16, "f16", seed=9)
+    w = torch.rand(c.pages, 1, 16, device="cuda") + 1
+    p = torch.zeros(c.pages, 1, 16, device="cuda", dtype=torch.int32) + 50
+    bad = int(c.table[0, 1])
+    c.table[0, 1] = -1
+    nxt = torch.full((2,), 1000, device="cuda", dtype=torch.int32)
+    lo = torch.zeros_like(c.len)
+    k0, w0 = c.k.clone(), w.clone()
+    assert _evict(bridge_lib, c, w, w, p, p, nxt, 48, 0, 0, lo) == 0
+    assert lo.tolist() == [48, 48]
+    # the other 48 slots of sequence 0 stay: its holes are the absent ones, which take nothing
+    for page in c.page_lists[0]:
+        assert torch.equal(c.k[page], k0[page]) and torch.equal(w[page], w0[page])
+    assert bad in c.page_lists[0]
