@@ -13,6 +13,7 @@
 
 #include "cuda_bridge.h"
 #include "paged_attention.cuh"
+#include "paged_attention_tc.cuh"
 #include "paged_common.cuh"
 #include "paged_evict.cuh"
 #include "paged_rope.cuh"
@@ -164,6 +165,8 @@ int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
 // ------------------------------------------------------------------- attention plan
 struct AttentionPlan {
+  bool tc;        // the tcgen05 kernel (256 query rows a CTA), else the 16-row one
+  int tile_rows;
   int64_t tiles;  // an upper bound: the device knows how many there are
   int splits;
   int keys;  // keys of a split
@@ -180,12 +183,18 @@ int64_t tile_bound(const cb_paged_kv* kv, int group, int m) {
 
 AttentionPlan plan_attention(const cb_paged_kv* kv, int32_t heads) {
   AttentionPlan p;
-  p.tiles = tile_bound(kv, heads / kv->kv_heads, PR_ROWS);
-  // Two CTAs share an SM; four per SM in all leave the last ones little to wait for.
-  const int64_t want = 4 * PG_SMS, have = std::max<int64_t>(1, p.tiles * kv->kv_heads);
-  int64_t splits = std::min<int64_t>(ceil_div(want, have), ceil_div(kv->max_len, 256));
-  splits = std::max<int64_t>(1, splits);
-  p.keys = (int)(ceil_div(ceil_div(kv->max_len, splits), 16) * 16);
+  const int group = heads / kv->kv_heads;
+  p.tc = (int64_t)kv->max_new * group > PR_ROWS;
+  p.tile_rows = p.tc ? PT_ROWS : PR_ROWS;
+  p.tiles = tile_bound(kv, group, p.tile_rows);
+  const int64_t have = std::max<int64_t>(1, p.tiles * kv->kv_heads);
+  // 16-row kernel: two CTAs share an SM; four per SM in all leave the last ones little to
+  // wait for. tcgen05 kernel: one CTA per SM.
+  const int64_t want = p.tc ? PG_SMS : 4 * PG_SMS;
+  const int step = p.tc ? PT_KEYS : PR_BLOCK, least = p.tc ? 512 : 256;
+  const int64_t splits = std::max<int64_t>(
+      1, std::min<int64_t>(p.tc ? want / have : ceil_div(want, have), ceil_div(kv->max_len, least)));
+  p.keys = (int)(ceil_div(ceil_div(kv->max_len, splits), step) * step);
   p.splits = (int)ceil_div(kv->max_len, p.keys);
   p.parts = (size_t)kv->rows * heads * p.splits;
   return p;
@@ -198,20 +207,29 @@ cb_status launch_attention(const cb_paged_kv* kv, const T* q, int64_t q_stride, 
   const AttentionPlan p = plan_attention(kv, heads);
   const int64_t grid = p.tiles * kv->kv_heads * p.splits;
   if (grid > INT_LIMIT) return CB_ERR_UNSUPPORTED;
+  const int box = p.tc ? std::min(kv->page_size, PT_KEYS) : PR_BLOCK;
   CUtensorMap tk, tv;
-  if (!make_cache_map(&tk, kv->k, kv, PR_BLOCK) || !make_cache_map(&tv, kv->v, kv, PR_BLOCK))
+  if (!make_cache_map(&tk, kv->k, kv, box) || !make_cache_map(&tv, kv->v, kv, box))
     return CB_ERR_UNSUPPORTED;
-  static std::atomic<uint64_t> done{0};
-  cudaError_t e = allow_smem(paged_rows_kernel<T>, PR_SMEM, done);
-  if (e != cudaSuccess) return status_of(e);
   const PagedKV d = device_kv(kv);
+  const float scale_log2 = scale * 1.4426950408889634f;
   PagedParts parts{workspace, workspace ? workspace + p.parts * PG_HD : nullptr, p.splits, p.keys};
-  paged_rows_kernel<T><<<(unsigned)grid, PR_WARPS * 32, PR_SMEM, st>>>(
-      tk, tv, d, q, q_stride, heads, scale * 1.4426950408889634f, out, out_stride, lse, parts);
+  cudaError_t e;
+  if (p.tc) {
+    static std::atomic<uint64_t> done{0};
+    if ((e = allow_smem(paged_tile_kernel<T>, PT_SMEM, done)) != cudaSuccess) return status_of(e);
+    paged_tile_kernel<T><<<(unsigned)grid, PT_THREADS, PT_SMEM, st>>>(
+        tk, tv, d, q, q_stride, heads, scale_log2, out, out_stride, lse, parts, box);
+  } else {
+    static std::atomic<uint64_t> done{0};
+    if ((e = allow_smem(paged_rows_kernel<T>, PR_SMEM, done)) != cudaSuccess) return status_of(e);
+    paged_rows_kernel<T><<<(unsigned)grid, PR_WARPS * 32, PR_SMEM, st>>>(
+        tk, tv, d, q, q_stride, heads, scale_log2, out, out_stride, lse, parts);
+  }
   e = cudaPeekAtLastError();
   if (e == cudaSuccess && p.splits > 1) {
     const int64_t blocks = ceil_div((int64_t)kv->rows * heads, PC_WARPS);
-    paged_combine_kernel<T><<<(unsigned)blocks, PC_WARPS * 32, 0, st>>>(d, heads, parts, PR_ROWS,
+    paged_combine_kernel<T><<<(unsigned)blocks, PC_WARPS * 32, 0, st>>>(d, heads, parts, p.tile_rows,
                                                                        out, out_stride, lse);
     e = cudaPeekAtLastError();
   }
