@@ -17,6 +17,7 @@
 #include "paged_common.cuh"
 #include "paged_evict.cuh"
 #include "paged_rope.cuh"
+#include "paged_weights_tc.cuh"
 #include "tensor_map.h"
 
 using namespace cb;
@@ -236,6 +237,50 @@ cb_status launch_attention(const cb_paged_kv* kv, const T* q, int64_t q_stride, 
   return status_of(e);
 }
 
+// q as a [rows][heads][128] array in boxes of tokens x group x 64, 128-byte swizzle.
+bool make_q_map(CUtensorMap* map, const void* q, int64_t q_stride, int heads, int rows, int group,
+                int tokens) {
+  EncodeTiledFn enc = encode_fn();
+  if (!enc) return false;
+  cuuint64_t dims[3] = {(cuuint64_t)PG_HD, (cuuint64_t)heads, (cuuint64_t)rows};
+  cuuint64_t strides[2] = {PG_HD * 2, (cuuint64_t)q_stride * 2};
+  cuuint32_t box[3] = {64, (cuuint32_t)group, (cuuint32_t)tokens};
+  cuuint32_t estr[3] = {1, 1, 1};
+  return enc(map, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3, const_cast<void*>(q), dims, strides, box,
+             estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+             CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+template <typename T>
+cb_status launch_weights(const cb_paged_kv* kv, const T* q, int64_t q_stride, int32_t heads,
+                         float scale, const float* lse, float* weights, cudaStream_t st) {
+  const int group = heads / kv->kv_heads;
+  const PagedKV d = device_kv(kv);
+  const float scale_log2 = scale * 1.4426950408889634f;
+  // the tcgen05 kernel needs a token's whole group in a step
+  const bool tc = (int64_t)kv->max_new * group > PR_ROWS && group <= WT_ROWS;
+  const int blocks = (int)ceil_div(kv->max_len, tc ? WT_KEYS : PW_KEYS);
+  const int64_t grid = (int64_t)kv->batch * blocks * kv->kv_heads;
+  if (grid > INT_LIMIT) return CB_ERR_UNSUPPORTED;
+  if (!tc) {
+    paged_weights_kernel<T><<<(unsigned)grid, PW_WARPS * 32, 0, st>>>(
+        d, q, q_stride, heads, scale_log2, lse, weights, blocks);
+    return status_of(cudaPeekAtLastError());
+  }
+  const int box = std::min(kv->page_size, 128), tokens = WT_ROWS / group;
+  CUtensorMap tk, tq;
+  if (!make_cache_map(&tk, kv->k, kv, box) ||
+      !make_q_map(&tq, q, q_stride, heads, kv->rows, group, tokens))
+    return CB_ERR_UNSUPPORTED;
+  static std::atomic<uint64_t> done{0};
+  const cudaError_t e = allow_smem(paged_weights_tile_kernel<T>, WT_SMEM, done);
+  if (e != cudaSuccess) return status_of(e);
+  paged_weights_tile_kernel<T><<<(unsigned)grid, WT_THREADS, WT_SMEM, st>>>(
+      tk, tq, d, heads, scale_log2, lse, weights, blocks, box, tokens);
+  return status_of(cudaPeekAtLastError());
+}
+
 // ---------------------------------------------------------------------- evict plan
 template <int THREADS, int PER>
 cudaError_t launch_evict(const PagedKV& kv, const EvictArgs& a, int ctas, cudaStream_t st) {
@@ -437,19 +482,12 @@ cb_status cb_paged_attention_weights(const cb_paged_kv* kv, const void* q, int64
   const cb_status s =
       check_device({kv->k, kv->table, kv->len, kv->row_start, q, lse, weights});
   if (s != CB_OK) return s;
-  const int blocks = (int)ceil_div(kv->max_len, PW_KEYS);
-  const int64_t grid = (int64_t)kv->batch * blocks * kv->kv_heads;
-  if (grid > INT_LIMIT) return CB_ERR_UNSUPPORTED;
-  const PagedKV d = device_kv(kv);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  const float scale_log2 = scale * 1.4426950408889634f;
   if (kv->dtype == CB_DTYPE_F16)
-    paged_weights_kernel<__half><<<(unsigned)grid, PW_WARPS * 32, 0, st>>>(
-        d, static_cast<const __half*>(q), q_stride, heads, scale_log2, lse, weights, blocks);
-  else
-    paged_weights_kernel<__nv_bfloat16><<<(unsigned)grid, PW_WARPS * 32, 0, st>>>(
-        d, static_cast<const __nv_bfloat16*>(q), q_stride, heads, scale_log2, lse, weights, blocks);
-  return status_of(cudaPeekAtLastError());
+    return launch_weights(kv, static_cast<const __half*>(q), q_stride, heads, scale, lse, weights,
+                          st);
+  return launch_weights(kv, static_cast<const __nv_bfloat16*>(q), q_stride, heads, scale, lse,
+                        weights, st);
 }
 
 static size_t evict_list(const cb_paged_kv* kv, int32_t budget) {

@@ -1,0 +1,257 @@
+// Attention weight that every slot of a paged cache got from a chunk of new tokens, on the
+// 5th-generation tensor cores: w_k += sum_r 2^(s_rk - lse_r), for many query rows.
+//
+// The slots are the rows of the product (S^T = K Q^T): a thread owns one slot, reads the
+// scores of all query rows of a step from its own TMEM lane and adds up, so the sum needs no
+// exchange and its order is fixed. A CTA keeps the K of 256 slots of one key head (two tiles
+// of 128, one warpgroup each) and walks the query rows in steps of whole tokens, at most 128
+// rows: every Q step that is loaded serves both tiles. 384 threads:
+//   warp 0       TMA producer: K once, then the Q steps (three buffers)
+//   warp 1       TMEM owner; lane 0 issues S^T (128 x 128 x 128) into two buffers per tile
+//   warp 2       copies the steps' log-sum-exps and limits to shared memory
+//   warps 4-11   the sums
+#pragma once
+#include "paged_attention_tc.cuh"
+
+namespace cb {
+
+constexpr int WT_KEYS = 256;        // slots of a CTA
+constexpr int WT_ROWS = 128;        // query rows of a step, at most
+constexpr int WT_THREADS = 384;
+constexpr int WT_Q_BUFS = 3;
+constexpr int WT_L_BUFS = 4;
+constexpr int WT_K_OFF = 0;         // [tile][half of the head][128 slots][128 B]
+constexpr int WT_Q_OFF = 65536;     // [buffer][half][128 rows][128 B]
+constexpr int WT_L_OFF = WT_Q_OFF + WT_Q_BUFS * 32768;  // [buffer]: -lse [128], limit [128]
+constexpr int WT_BAR_OFF = WT_L_OFF + WT_L_BUFS * 1024;
+constexpr int WT_SMEM = WT_BAR_OFF + 256 + 1024;
+constexpr uint32_t WT_TMEM_COLS = 512;  // tile A: two buffers of 128 columns, tile B: two
+
+// 3-D tiled TMA load without a cache hint.
+__device__ __forceinline__ void tma_load_3d_plain(void* smem_dst, const CUtensorMap* map,
+                                                  uint64_t* bar, int32_t c0, int32_t c1,
+                                                  int32_t c2) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes"
+      " [%0], [%1, {%3, %4, %5}], [%2];" ::"r"(smem_u32(smem_dst)),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(smem_u32(bar)), "r"(c0), "r"(c1), "r"(c2)
+      : "memory");
+}
+
+// Grid: ((sequence * blocks of WT_KEYS slots) + block) * kv_heads + key head. tmQ: q as
+// [rows][heads][128] in boxes of step_tokens x group x 64.
+template <typename T>
+__global__ void __launch_bounds__(WT_THREADS, 1)
+    paged_weights_tile_kernel(const __grid_constant__ CUtensorMap tmK,
+                              const __grid_constant__ CUtensorMap tmQ, const PagedKV kv, int heads,
+                              float scale_log2, const float* __restrict__ lse,
+                              float* __restrict__ weights, int blocks, int box_rows,
+                              int step_tokens) {
+  extern __shared__ uint8_t wt_smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>(
+      (reinterpret_cast<uintptr_t>(wt_smem_raw) + 1023) & ~uintptr_t(1023));
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + WT_BAR_OFF);
+  uint64_t* k_full = bars;
+  uint64_t* q_full = bars + 1;    // [3]
+  uint64_t* q_empty = bars + 4;   // [3]
+  uint64_t* l_full = bars + 7;    // [4]
+  uint64_t* l_empty = bars + 11;  // [4]
+  uint64_t* s_full = bars + 15;   // [tile][2]
+  uint64_t* s_empty = bars + 19;  // [tile][2]
+  uint64_t* drain = bars + 23;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 24);
+  int* failed = reinterpret_cast<int*>(bars + 25);
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int group = heads / kv.kv_heads;
+  const int head = blockIdx.x % kv.kv_heads;
+  const int rest = blockIdx.x / kv.kv_heads;
+  const int b = rest / blocks;
+  const int key0 = (rest % blocks) * WT_KEYS;
+  const PagedSeq seq = paged_seq(kv, b);
+  if (seq.n == 0 || key0 >= seq.limit(seq.n - 1)) return;  // no query sees these slots
+  const int tiles = key0 + 128 < seq.limit(seq.n - 1) ? 2 : 1;
+  const int i0 = max(0, key0 - seq.past);  // the first token that sees one of them
+  const int steps = (seq.n - i0 + step_tokens - 1) / step_tokens;
+  const int step_rows = step_tokens * group;
+
+  if (threadIdx.x == 0) {
+    mbar_init(k_full, 1);
+    for (int i = 0; i < WT_Q_BUFS; ++i) {
+      mbar_init(&q_full[i], 1);
+      mbar_init(&q_empty[i], 1);
+    }
+    for (int i = 0; i < WT_L_BUFS; ++i) {
+      mbar_init(&l_full[i], 1);
+      mbar_init(&l_empty[i], 4 * tiles);
+      mbar_init(&s_full[i], 1);
+      mbar_init(&s_empty[i], 4);
+    }
+    mbar_init(drain, 1);
+    *failed = 0;
+    fence_mbar_init();
+    tma_prefetch_desc(&tmK);
+    tma_prefetch_desc(&tmQ);
+  }
+  if (warp == 1) {
+    tmem_alloc(tmem_slot, WT_TMEM_COLS);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+
+  if (warp == 0) {
+    // ---------------- producer
+    if (lane == 0) mbar_arrive_expect_tx(k_full, 32768 * tiles);
+    __syncwarp();
+    for (int s = 0; s < tiles; ++s) {
+      const int k = key0 + s * 128;
+      const int id = pt_step_id(kv, b, k, seq.end, box_rows, lane);
+      const int part = lane >> 1, half = lane & 1;
+      if (part * box_rows < 128) {
+        const int row = id >= 0 ? kv.page_row(id, head, k + part * box_rows) : kv.cache_rows();
+        tma_load_2d(smem + WT_K_OFF + s * 32768 + half * 16384 + part * box_rows * 128, &tmK, k_full,
+                    half * 64, row);
+      }
+    }
+    if (lane == 0) {
+      for (int j = 0; j < steps; ++j) {
+        const int buf = j % WT_Q_BUFS;
+        if (!mbar_wait(&q_empty[buf], ((j / WT_Q_BUFS) & 1) ^ 1u, failed)) break;
+        uint8_t* dst = smem + WT_Q_OFF + buf * 32768;
+        const int row = seq.row0 + i0 + j * step_tokens;
+        mbar_arrive_expect_tx(&q_full[buf], step_rows * 256);
+        tma_load_3d_plain(dst, &tmQ, &q_full[buf], 0, head * group, row);
+        tma_load_3d_plain(dst + 16384, &tmQ, &q_full[buf], 64, head * group, row);
+      }
+    }
+  } else if (warp == 1) {
+    if (lane == 0) {
+      // ---------------- matrix instructions
+      constexpr uint32_t idesc = pt_idesc<T>(false);
+      const uint32_t k_addr = smem_u32(smem + WT_K_OFF), q_addr = smem_u32(smem + WT_Q_OFF);
+      bool ok = mbar_wait(k_full, 0, failed);
+      for (int j = 0; ok && j < steps; ++j) {
+        const int buf = j % WT_Q_BUFS;
+        if (!(ok = mbar_wait(&q_full[buf], (j / WT_Q_BUFS) & 1, failed))) break;
+        for (int s = 0; ok && s < tiles; ++s) {
+          if (!(ok = mbar_wait(&s_empty[s * 2 + (j & 1)], ((j >> 1) & 1) ^ 1u, failed))) break;
+          tc_fence_after();
+#pragma unroll
+          for (int k = 0; k < 8; ++k) {
+            const uint32_t off = (uint32_t)((k >> 2) * 16384 + (k & 3) * 32);
+            umma_f16_ss(tmem + s * 256 + (j & 1) * 128, sw128_kmajor_desc(k_addr + s * 32768 + off),
+                        sw128_kmajor_desc(q_addr + buf * 32768 + off), idesc, k != 0);
+          }
+          umma_commit(&s_full[s * 2 + (j & 1)]);
+        }
+        umma_commit(&q_empty[buf]);
+      }
+      umma_commit(drain);
+      mbar_wait(drain, 0, failed);
+    }
+  } else if (warp == 2) {
+    // ---------------- log-sum-exps and limits of the steps' rows
+    for (int j = 0; j < steps; ++j) {
+      const int buf = j % WT_L_BUFS;
+      float x[4];
+      int lim[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int c = lane + 32 * e;
+        const int i = i0 + j * step_tokens + c / group;
+        const bool valid = c < step_rows && i < seq.n;
+        x[e] = valid ? -__ldg(lse + (int64_t)(seq.row0 + i) * heads + head * group + c % group) : 0.f;
+        lim[e] = valid ? seq.limit(i) : 0;
+      }
+      if (!mbar_wait(&l_empty[buf], ((j / WT_L_BUFS) & 1) ^ 1u, failed)) break;
+      float* dst = reinterpret_cast<float*>(smem + WT_L_OFF + buf * 1024);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        dst[lane + 32 * e] = x[e];
+        reinterpret_cast<int*>(dst)[128 + lane + 32 * e] = lim[e];
+      }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&l_full[buf]);
+    }
+  } else if (warp >= 4 && (warp - 4) >> 2 < tiles) {
+    // ---------------- sums: thread = slot
+    const int s = (warp - 4) >> 2, quad = warp & 3;
+    const int key = key0 + s * 128 + quad * 32 + lane;
+    const uint32_t t_s = tmem + s * 256 + ((uint32_t)(quad * 32) << 16);
+    const float2 sc2 = make_float2(scale_log2, scale_log2);
+    float2 acc[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+    bool ok = true;
+    for (int j = 0; j < steps; ++j) {
+      const int buf = j % WT_L_BUFS;
+      const int first = i0 + j * step_tokens;
+      // whole steps whose rows all see the tile's slots need no masks
+      const bool whole = step_rows == WT_ROWS && first + step_tokens <= seq.n &&
+                         key0 + s * 128 + 128 <= seq.limit(first);
+      const float4* nl = reinterpret_cast<const float4*>(smem + WT_L_OFF + buf * 1024);
+      const int4* lim = reinterpret_cast<const int4*>(nl + 32);
+      if (!mbar_wait(&l_full[buf], (j / WT_L_BUFS) & 1, failed) ||
+          !mbar_wait(&s_full[s * 2 + (j & 1)], (j >> 1) & 1, failed)) { ok = false; break; }
+      tc_fence_after();
+      // 32 query rows at a time, the next ones on their way
+      uint32_t u[2][32];
+      tmem_ld_32x32b_x32(t_s + (j & 1) * 128, u[0]);
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        tmem_ld_wait_regs(u[c & 1]);
+        if (c < 3) {
+          tmem_ld_32x32b_x32(t_s + (j & 1) * 128 + (c + 1) * 32, u[(c + 1) & 1]);
+        } else {
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&s_empty[s * 2 + (j & 1)]);
+        }
+        const uint32_t(&w)[32] = u[c & 1];
+        if (whole) {
+#pragma unroll
+          for (int e = 0; e < 32; e += 4) {
+            const float4 y = nl[c * 8 + e / 4];
+            float2 a = ffma2(make_float2(__uint_as_float(w[e]), __uint_as_float(w[e + 1])), sc2,
+                             make_float2(y.x, y.y));
+            float2 d = ffma2(make_float2(__uint_as_float(w[e + 2]), __uint_as_float(w[e + 3])), sc2,
+                             make_float2(y.z, y.w));
+            a.x = exp2_mufu(a.x);
+            a.y = exp2_mufu(a.y);
+            d.x = exp2_mufu(d.x);
+            d.y = exp2_mufu(d.y);
+            acc[0] = fadd2(acc[0], a);
+            acc[1] = fadd2(acc[1], d);
+          }
+        } else {
+#pragma unroll
+          for (int e = 0; e < 32; e += 4) {
+            const float4 y = nl[c * 8 + e / 4];
+            const int4 m = lim[c * 8 + e / 4];
+            acc[0].x += key < m.x ? exp2_mufu(fmaf(__uint_as_float(w[e]), scale_log2, y.x)) : 0.f;
+            acc[0].y += key < m.y ? exp2_mufu(fmaf(__uint_as_float(w[e + 1]), scale_log2, y.y)) : 0.f;
+            acc[1].x += key < m.z ? exp2_mufu(fmaf(__uint_as_float(w[e + 2]), scale_log2, y.z)) : 0.f;
+            acc[1].y += key < m.w ? exp2_mufu(fmaf(__uint_as_float(w[e + 3]), scale_log2, y.w)) : 0.f;
+          }
+        }
+      }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&l_empty[buf]);
+    }
+    if (ok && key < seq.limit(seq.n - 1)) {
+      const int id = kv.page_id(b, key);
+      if (id >= 0)
+        atomicAdd(weights + kv.page_row(id, head, key),
+                  (acc[0].x + acc[0].y) + (acc[1].x + acc[1].y));
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc(tmem, WT_TMEM_COLS);
+  }
+}
+
+}  // namespace cb
