@@ -535,16 +535,16 @@ cb_status cb_paged_evict(const cb_paged_kv* kv, const float* weights, float* wei
   // The smallest form that holds the longest sequence; long ones are spread over a cluster.
   const int n = kv->max_len;
   cudaError_t e;
-  if (n <= 256 * 4)
-    e = launch_evict<256, 4>(d, a, 1, st);
-  else if (n <= 1024 * 4)
-    e = launch_evict<1024, 4>(d, a, 1, st);
-  else if (n <= 1024 * 4 * 2)
-    e = launch_evict<1024, 4>(d, a, 2, st);
-  else if (n <= 1024 * 4 * 4)
-    e = launch_evict<1024, 4>(d, a, 4, st);
-  else if (n <= 1024 * 4 * 8)
-    e = launch_evict<1024, 4>(d, a, 8, st);
+  if (n <= 128 * 8)
+    e = launch_evict<128, 8>(d, a, 1, st);
+  else if (n <= 512 * 8)
+    e = launch_evict<512, 8>(d, a, 1, st);
+  else if (n <= 512 * 8 * 2)
+    e = launch_evict<512, 8>(d, a, 2, st);
+  else if (n <= 512 * 8 * 4)
+    e = launch_evict<512, 8>(d, a, 4, st);
+  else if (n <= 512 * 8 * 8)
+    e = launch_evict<512, 8>(d, a, 8, st);
   else
     e = launch_evict<EV_MAX_THREADS, EV_MAX_PER_THREAD>(d, a, EV_MAX_CTAS, st);
   return status_of(e);

@@ -2,16 +2,19 @@
 //
 // One cluster of CTAs per (sequence, key head). Every slot gets a 32-bit key whose unsigned
 // order is the order of keeping: all ones for the positions that must stay, else the
-// weight's bits made monotone (NaN lowest). The budget-th largest key is found two bits a
-// pass by counting (16 passes over keys that stay in registers: no atomics, so no pile-up on
-// the few exponents that weights have, and the result does not depend on any order). Keys
-// above it stay, of those equal to it the lowest slots. Then the i-th slot below the budget
-// that is not kept (a hole) takes the i-th kept slot behind the budget (a mover); the
-// numbering is a scan over ballots. Holes and movers are disjoint ranges of slots, so all
-// rows move at once and in place. Reading the weights and positions and moving the rows is
-// the work that cannot be left out: the kernel is bound by the latency of the passes for
-// short sequences and by the moved rows for long ones, which is why a long sequence gets
-// several CTAs (they share the counts through distributed shared memory).
+// weight's bits made monotone (NaN lowest). Which slots go:
+//   - up to EV_FEW of them (a decode step drops one): the smallest key, of equals the highest
+//     slot, is looked for that many times;
+//   - more: the budget-th largest key is found two bits a pass by counting (at most 16
+//     passes over keys that stay in registers, fewer once a pass hits the budget exactly).
+//     Keys above it stay, of those equal to it the lowest slots. Counting needs no atomics on
+//     a histogram, which would pile up on the few exponents that weights have.
+// Either way the result does not depend on any order of execution. Then the i-th slot below
+// the budget that is not kept (a hole) takes the i-th kept slot behind the budget (a mover).
+// Holes and movers are disjoint ranges of slots, so all rows move at once and in place.
+// Reading the weights and positions and moving the rows is the work that cannot be left out;
+// a long sequence gets several CTAs (they share the counts through distributed shared
+// memory), because one SM moves rows at a small part of the memory's rate.
 #pragma once
 #include "paged_common.cuh"
 
@@ -35,12 +38,15 @@ __device__ __forceinline__ uint32_t evict_key(float w) {
   return bits >> 31 ? ~bits : bits | 0x80000000u;
 }
 
-// Per-block counts of up to three predicates per element, in one word each.
+constexpr int EV_FEW = 8;
+
 template <int THREADS, int PER>
 struct EvictShared {
   static constexpr int WARPS = THREADS / 32;
-  uint32_t part[3][WARPS];
-  uint32_t cluster[2][3];  // this CTA's counts, read by the others; two buffers in turn
+  uint32_t count[3][3];    // sums of three counts over the block, three buffers in turn
+  uint32_t least[2][2];    // this CTA's smallest key and its highest slot, two buffers
+  uint32_t warp_key[WARPS], warp_slot[WARPS];
+  int few[EV_FEW];         // the slots that go, when they are few
   uint32_t scan[PER * WARPS];
   uint32_t scan2[PER * WARPS];
   uint32_t warp_sum[32], warp_sum2[32];
@@ -100,77 +106,168 @@ __global__ void __launch_bounds__(THREADS)
   const int new_len = min(n, a.budget);
   if (rank == 0 && head == 0 && t == 0) a.len_out[b] = new_len;
 
-  auto meta = [&](int slot, int id) { return (size_t)kv.page_row(id, head, slot); };
-  const bool out_of_place_w = a.weights_out != a.weights;
-  const bool out_of_place_p = a.positions_out != a.positions;
+  const bool copy_w = a.weights_out != a.weights, copy_p = a.positions_out != a.positions;
   const int base = rank * THREADS * PER;
 
-  if (n <= a.budget) {  // everything stays (the whole cluster takes this branch)
-    for (int s = base + t; s < min(n, base + THREADS * PER); s += THREADS) {
-      const int id = kv.page_id(b, s);
-      if (id < 0) continue;
-      const size_t at = meta(s, id);
-      if (out_of_place_w) a.weights_out[at] = a.weights[at];
-      if (out_of_place_p) a.positions_out[at] = a.positions[at];
-    }
-    return;
-  }
-
-  // ---- the keys
+  // ---- the keys. Written to another array, weights and positions of every slot below the
+  // new length are copied at once (a hole's are overwritten when its mover comes).
   uint32_t key[PER];
   {
     const int recent_from = __ldg(a.next_position + b) - a.recent;
+    constexpr int BATCH = PER < 8 ? PER : 8;  // loads in flight
 #pragma unroll
-    for (int e = 0; e < PER; ++e) {
-      const int s = base + e * THREADS + t;
-      key[e] = 0;  // no slot, or one that is absent: kept last
-      if (s < n) {
-        const int id = kv.page_id(b, s);
-        if (id >= 0) {
-          const size_t at = meta(s, id);
-          const int p = a.positions[at];
-          const bool must = p < a.sinks || (a.recent > 0 && p >= recent_from);
-          key[e] = must ? 0xffffffffu : evict_key(a.weights[at]);
+    for (int e0 = 0; e0 < PER; e0 += BATCH) {
+      int at[BATCH], p[BATCH];
+      float w[BATCH];
+#pragma unroll
+      for (int e = 0; e < BATCH; ++e) {
+        const int s = base + (e0 + e) * THREADS + t;
+        const int id = s < n ? kv.page_id(b, s) : -1;
+        at[e] = id >= 0 ? kv.page_row(id, head, s) : -1;
+      }
+#pragma unroll
+      for (int e = 0; e < BATCH; ++e) {
+        p[e] = at[e] >= 0 ? a.positions[at[e]] : 0;
+        w[e] = at[e] >= 0 ? a.weights[at[e]] : 0.f;
+      }
+#pragma unroll
+      for (int e = 0; e < BATCH; ++e) {
+        const int s = base + (e0 + e) * THREADS + t;
+        const bool must = p[e] < a.sinks || (a.recent > 0 && p[e] >= recent_from);
+        // 0: no slot, or one that is absent (kept last)
+        key[e0 + e] = at[e] < 0 ? 0u : must ? 0xffffffffu : evict_key(w[e]);
+        if (at[e] >= 0 && s < new_len) {
+          if (copy_w) a.weights_out[at[e]] = w[e];
+          if (copy_p) a.positions_out[at[e]] = p[e];
         }
       }
     }
   }
+  if (n <= a.budget) return;  // everything stays (the whole cluster ends here)
 
-  // Sums of this block's three counts over the cluster; `before` those of lower ranks only.
+  auto cluster_barrier = [&] {
+    __syncwarp();
+    if (ctas > 1) cluster_sync(); else __syncthreads();
+  };
+  // One row, by a warp: lanes 0-15 K, 16-31 V, lane 0 also the weight and the position.
+  auto pool = [&](int at) {
+    return static_cast<uint4*>(lane < 16 ? kv.k : kv.v) + (size_t)at * (PG_HD / 8) + (lane & 15);
+  };
+
+  // ---- few slots go: look for each
+  if (n - a.budget <= EV_FEW) {
+    const int go = n - a.budget;
+    uint32_t gone = 0;
+    for (int round = 0; round < go; ++round) {
+      uint32_t k = 0xffffffffu, top = 0;  // the smallest key, and its highest slot + 1
+#pragma unroll
+      for (int e = 0; e < PER; ++e) {
+        const int s = base + e * THREADS + t;
+        if (s < n && !(gone >> e & 1u) && key[e] <= k) {
+          k = key[e];
+          top = (uint32_t)s + 1;
+        }
+      }
+      uint32_t least = __reduce_min_sync(0xffffffffu, k);
+      uint32_t slot = __reduce_max_sync(0xffffffffu, k == least ? top : 0u);
+      if (lane == 0) {
+        sm.warp_key[warp] = least;
+        sm.warp_slot[warp] = slot;
+      }
+      __syncthreads();
+      k = lane < WARPS ? sm.warp_key[lane] : 0xffffffffu;
+      top = lane < WARPS ? sm.warp_slot[lane] : 0u;
+      least = __reduce_min_sync(0xffffffffu, k);
+      slot = __reduce_max_sync(0xffffffffu, k == least ? top : 0u);
+      if (ctas > 1) {
+        uint32_t* mine = sm.least[round & 1];
+        if (t == 0) {
+          mine[0] = least;
+          mine[1] = slot;
+        }
+        __syncwarp();
+        cluster_sync();
+        // (a buffer is written again two rounds later, behind another cluster barrier)
+        k = lane < ctas ? ld_cluster_u32(mapa_shared(smem_u32(mine), lane)) : 0xffffffffu;
+        top = lane < ctas ? ld_cluster_u32(mapa_shared(smem_u32(mine + 1), lane)) : 0u;
+        least = __reduce_min_sync(0xffffffffu, k);
+        slot = __reduce_max_sync(0xffffffffu, k == least ? top : 0u);
+      } else {
+        __syncthreads();
+      }
+      const int out = (int)slot - 1, local = out - base;
+      if (local >= 0 && local < THREADS * PER && local % THREADS == t) gone |= 1u << (local / THREADS);
+      if (t == 0) sm.few[round] = out;
+    }
+    // no CTA leaves while another may still read its least; and the copies of phase one are done
+    cluster_barrier();
+    if (rank != 0) return;
+    for (int i = warp; i < go; i += WARPS) {
+      const int src = new_len + i;
+      int nth = 0, dst = -1;
+      bool stays = true;
+      for (int j = 0; j < go; ++j) {
+        const int f = sm.few[j];
+        stays &= f != src;
+      }
+      if (!stays) continue;
+      for (int c = 0; c < i; ++c) {  // kept slots behind the budget that come before this one
+        bool kept = true;
+        for (int j = 0; j < go; ++j) kept &= sm.few[j] != new_len + c;
+        nth += kept;
+      }
+      for (int j = 0; j < go; ++j) {  // the hole of that number
+        int lower = 0;
+        for (int g = 0; g < go; ++g) lower += sm.few[g] < sm.few[j];
+        if (sm.few[j] < new_len && lower == nth) dst = sm.few[j];
+      }
+      const int src_id = kv.page_id(b, src), dst_id = dst >= 0 ? kv.page_id(b, dst) : -1;
+      if (src_id < 0 || dst_id < 0) continue;  // a slot that is absent
+      const int from = kv.page_row(src_id, head, src), at = kv.page_row(dst_id, head, dst);
+      *pool(at) = *pool(from);
+      if (lane == 0) a.weights_out[at] = a.weights[from];
+      if (lane == 1) a.positions_out[at] = a.positions[from];
+    }
+    return;
+  }
+
+  // Sums of three counts of this block over the cluster; `before`: over lower ranks only.
+  // Three buffers in turn: the one cleared here was last read two barriers ago.
   int turn = 0;
   auto cluster_counts = [&](uint32_t (&c)[3], uint32_t (&before)[3]) {
+    const int clear = turn == 2 ? 0 : turn + 1;
 #pragma unroll
     for (int j = 0; j < 3; ++j) {
-      c[j] = __reduce_add_sync(0xffffffffu, c[j]);
-      if (lane == 0) sm.part[j][warp] = c[j];
+      const uint32_t w = __reduce_add_sync(0xffffffffu, c[j]);
+      if (lane == 0 && w) atomicAdd(&sm.count[turn][j], w);
     }
-    __syncthreads();
-#pragma unroll
-    for (int j = 0; j < 3; ++j) {
-      c[j] = __reduce_add_sync(0xffffffffu, lane < WARPS ? sm.part[j][lane] : 0u);
-      before[j] = 0;
-    }
+    if (t < 3) sm.count[clear][t] = 0;
+    cluster_barrier();
     if (ctas > 1) {
-      if (t < 3) sm.cluster[turn][t] = t == 0 ? c[0] : t == 1 ? c[1] : c[2];
-      __syncwarp();
-      cluster_sync();
-      // A buffer is written again two calls later, behind another cluster barrier.
-      uint32_t got = 0;
 #pragma unroll
       for (int j = 0; j < 3; ++j) {
-        got = lane < ctas ? ld_cluster_u32(mapa_shared(smem_u32(&sm.cluster[turn][j]), lane)) : 0u;
+        const uint32_t got =
+            lane < ctas ? ld_cluster_u32(mapa_shared(smem_u32(&sm.count[turn][j]), lane)) : 0u;
         c[j] = __reduce_add_sync(0xffffffffu, got);
         before[j] = __reduce_add_sync(0xffffffffu, lane < rank ? got : 0u);
       }
-      turn ^= 1;
     } else {
-      __syncthreads();
+#pragma unroll
+      for (int j = 0; j < 3; ++j) {
+        c[j] = *const_cast<volatile uint32_t*>(&sm.count[turn][j]);
+        before[j] = 0;
+      }
     }
+    turn = clear;
   };
+  if (t < 3) sm.count[0][t] = 0;
+  __syncthreads();
 
   // ---- the budget-th largest key: the largest T with at least `budget` keys >= T
   uint32_t T = 0, dummy[3];
-  for (int shift = 30; shift >= 0; shift -= 2) {
+  bool exact = false;  // just `budget` keys >= T
+  const uint32_t want = (uint32_t)a.budget;
+  for (int shift = 30; shift >= 0 && !exact; shift -= 2) {
     uint32_t c[3] = {0, 0, 0};
     const uint32_t t1 = T | (1u << shift), t2 = T | (2u << shift), t3 = T | (3u << shift);
 #pragma unroll
@@ -180,40 +277,44 @@ __global__ void __launch_bounds__(THREADS)
       c[2] += key[e] >= t3;
     }
     cluster_counts(c, dummy);
-    const uint32_t want = (uint32_t)a.budget;
-    T = c[2] >= want ? t3 : c[1] >= want ? t2 : c[0] >= want ? t1 : T;
+    if (c[2] >= want) {
+      T = t3;
+      exact = c[2] == want;
+    } else if (c[1] >= want) {
+      T = t2;
+      exact = c[1] == want;
+    } else if (c[0] >= want) {
+      T = t1;
+      exact = c[0] == want;
+    }
   }
-
-  // ---- how many keys equal to T stay, and where this thread's equals lie among all
-  uint32_t above[3] = {0, 0, 0}, above_before[3];
-#pragma unroll
-  for (int e = 0; e < PER; ++e) {
-    const bool slot = base + e * THREADS + t < n;
-    above[0] += key[e] > T;
-    above[1] += slot && key[e] == T;
-  }
-  cluster_counts(above, above_before);
-  const uint32_t equals_kept = (uint32_t)a.budget - above[0];
 
   uint32_t keep = 0;  // bit e: this thread's element e stays
-  if (above[1] == equals_kept) {
+  if (exact) {
 #pragma unroll
     for (int e = 0; e < PER; ++e)
-      if (base + e * THREADS + t < n && key[e] >= T) keep |= 1u << e;
+      if (key[e] >= T) keep |= 1u << e;
   } else {
+    // of the keys equal to T only some stay, the lowest slots: number them
+    uint32_t above[3] = {0, 0, 0}, above_before[3];
 #pragma unroll
     for (int e = 0; e < PER; ++e) {
-      const unsigned eq = __ballot_sync(0xffffffffu, base + e * THREADS + t < n && key[e] == T);
+      const bool equal = base + e * THREADS + t < n && key[e] == T;
+      above[0] += key[e] > T;
+      above[1] += equal;
+      const unsigned eq = __ballot_sync(0xffffffffu, equal);
       if (lane == 0) sm.scan[e * WARPS + warp] = __popc(eq);
     }
+    cluster_counts(above, above_before);
+    const uint32_t equals_kept = want - above[0];
     block_scan<THREADS>(sm.scan, PER * WARPS, sm.warp_sum);
 #pragma unroll
     for (int e = 0; e < PER; ++e) {
-      const bool slot = base + e * THREADS + t < n;
-      const unsigned eq = __ballot_sync(0xffffffffu, slot && key[e] == T);
+      const bool equal = base + e * THREADS + t < n && key[e] == T;
+      const unsigned eq = __ballot_sync(0xffffffffu, equal);
       const uint32_t place =
           above_before[1] + sm.scan[e * WARPS + warp] + __popc(eq & ((1u << lane) - 1));
-      if (slot && (key[e] > T || (key[e] == T && place < equals_kept))) keep |= 1u << e;
+      if (key[e] > T || (equal && place < equals_kept)) keep |= 1u << e;
     }
     __syncthreads();
   }
@@ -226,11 +327,11 @@ __global__ void __launch_bounds__(THREADS)
     const bool kept = keep >> e & 1u;
     const unsigned hole = __ballot_sync(0xffffffffu, s < new_len && !kept);
     const unsigned mover = __ballot_sync(0xffffffffu, s >= new_len && kept);
+    own[0] += s < new_len && !kept;
+    own[1] += s >= new_len && kept;
     if (lane == 0) {
       sm.scan[e * WARPS + warp] = __popc(hole);
       sm.scan2[e * WARPS + warp] = __popc(mover);
-      own[0] += __popc(hole);
-      own[1] += __popc(mover);
     }
   }
   cluster_counts(own, first);
@@ -250,45 +351,46 @@ __global__ void __launch_bounds__(THREADS)
       holes[first[0] + sm.scan[e * WARPS + warp] + __popc(hole & below)] = s;
     if (s >= new_len && kept)
       movers[first[1] + sm.scan2[e * WARPS + warp] + __popc(mover & below)] = s;
-    if (s < new_len && kept && (out_of_place_w || out_of_place_p)) {
-      const int id = kv.page_id(b, s);
-      if (id >= 0) {
-        const size_t at = meta(s, id);
-        if (out_of_place_w) a.weights_out[at] = a.weights[at];
-        if (out_of_place_p) a.positions_out[at] = a.positions[at];
+  }
+  cluster_barrier();  // the lists are whole; no CTA reads another's counts behind this
+
+  // ---- move: a warp takes 16 rows at a time, whose places its lanes look up together
+  const int stride = ctas * WARPS * 16;
+  for (int i0 = (rank * WARPS + warp) * 16; i0 < moves; i0 += stride) {
+    int from = -1, at = -1;
+    if (lane < 16 && i0 + lane < moves) {
+      const int src = __ldcg(movers + i0 + lane), dst = __ldcg(holes + i0 + lane);
+      const int src_id = kv.page_id(b, src), dst_id = kv.page_id(b, dst);
+      if (src_id >= 0 && dst_id >= 0) {  // else a slot that is absent
+        from = kv.page_row(src_id, head, src);
+        at = kv.page_row(dst_id, head, dst);
       }
     }
-  }
-  __syncwarp();
-  if (ctas > 1) cluster_sync(); else __syncthreads();  // the lists are whole
-
-  // ---- move: a warp takes four rows at a time, lanes 0-15 K and 16-31 V
-  constexpr int ROWS = 4;
-  const int stride = ctas * WARPS * ROWS;
-  for (int i0 = (rank * WARPS + warp) * ROWS; i0 < moves; i0 += stride) {
-    uint4 x[ROWS];
-    int64_t to[ROWS];
-#pragma unroll
-    for (int j = 0; j < ROWS; ++j) {
-      to[j] = -1;
-      if (i0 + j >= moves) continue;
-      const int src = __ldcg(movers + i0 + j), dst = __ldcg(holes + i0 + j);
-      const int src_id = kv.page_id(b, src), dst_id = kv.page_id(b, dst);
-      if (src_id < 0 || dst_id < 0) continue;  // a slot that is absent
-      const size_t from = meta(src, src_id), at = meta(dst, dst_id);
-      const uint4* pool = static_cast<const uint4*>(lane < 16 ? kv.k : kv.v);
-      x[j] = pool[from * (PG_HD / 8) + (lane & 15)];
-      to[j] = (int64_t)at;
-      if (lane == 0) a.weights_out[at] = a.weights[from];
-      if (lane == 1) a.positions_out[at] = a.positions[from];
+    float w = 0.f;
+    int p = 0;
+    if (from >= 0) {
+      w = a.weights[from];
+      p = a.positions[from];
     }
 #pragma unroll
-    for (int j = 0; j < ROWS; ++j)
-      if (to[j] >= 0)
-        static_cast<uint4*>(lane < 16 ? kv.k : kv.v)[to[j] * (PG_HD / 8) + (lane & 15)] = x[j];
+    for (int half = 0; half < 16; half += 8) {
+      uint4 x[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const int row = __shfl_sync(0xffffffffu, from, half + j);
+        if (row >= 0) x[j] = *pool(row);
+      }
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const int row = __shfl_sync(0xffffffffu, at, half + j);
+        if (row >= 0) *pool(row) = x[j];
+      }
+    }
+    if (from >= 0) {
+      a.weights_out[at] = w;
+      a.positions_out[at] = p;
+    }
   }
-  // no CTA leaves while another may still read its counts: the last reads of them lie
-  // before the barrier above
 }
 
 }  // namespace cb

@@ -421,3 +421,28 @@ def test_evict_with_pages_outside_the_pool(bridge_lib):
     for page in c.page_lists[0]:
         assert torch.equal(c.k[page], k0[page]) and torch.equal(w[page], w0[page])
     assert bad in c.page_lists[0]
+
+
+@pytest.mark.parametrize("over", [1, 2, 7, 8, 9])
+@pytest.mark.parametrize("budget,page", [(5, 16), (700, 16), (5000, 64), (20000, 128)])
+def test_evict_of_a_few_slots(bridge_lib, over, budget, page):
+    """Up to eight slots are looked for one by one, more of them by a threshold; equal
+    weights, the highest slots of which go."""
+    lens = [budget + over, budget, budget + 1]
+    c = Cache(lens, [0] * 3, 2, 2, page, "f16", seed=over)
+    g = torch.Generator(device="cuda").manual_seed(over)
+    w = torch.randint(0, max(2, budget // 50), (c.pages, 2, page), device="cuda", generator=g).float()
+    p = torch.randint(0, 10 * budget, w.shape, device="cuda", generator=g).int()
+    nxt = torch.full((3,), 10 * budget, device="cuda", dtype=torch.int32)
+    moves = R.evict_ref(c, w, p, nxt, budget, 1, budget // 4)
+    lo = torch.zeros_like(c.len)
+    k0, w0, p0 = c.k.clone(), w.clone(), p.clone()
+    assert _evict(bridge_lib, c, w, w, p, p, nxt, budget, 1, budget // 4, lo) == 0
+    assert lo.tolist() == [budget] * 3
+    for (b, h), source in moves.items():
+        to = c.place(b, torch.arange(len(source), device="cuda"))
+        fro = c.place(b, torch.tensor(source, device="cuda", dtype=torch.long))
+        k0[to[0], h, to[1]], w0[to[0], h, to[1]], p0[to[0], h, to[1]] = (
+            x[fro[0], h, fro[1]].clone() for x in (k0, w0, p0))
+    assert torch.equal(c.k.view(torch.int16), k0.view(torch.int16))
+    assert torch.equal(w, w0) and torch.equal(p, p0)
