@@ -166,13 +166,16 @@ int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
 // ------------------------------------------------------------------- attention plan
 struct AttentionPlan {
-  bool tc;        // the tcgen05 kernel (256 query rows a CTA), else the 16-row one
-  int tile_rows;
+  bool tc;        // the tcgen05 kernel, else the 16-row one
   int64_t tiles;  // an upper bound: the device knows how many there are
-  int splits;
-  int keys;  // keys of a split
-  size_t parts;
-  size_t bytes() const { return splits > 1 ? parts * (PG_HD + 1) * sizeof(float) : 0; }
+  int splits;     // 16-row kernel: parts of a tile, and their keys
+  int keys;
+  size_t parts;   // partial results: rows of 128 (and a log-sum-exp)
+  int ctas;       // tcgen05 kernel
+  size_t bytes() const {
+    if (tc) return parts * (PG_HD + 1) * sizeof(float) + ctas * sizeof(PtJoin);
+    return splits > 1 ? parts * (PG_HD + 1) * sizeof(float) : 0;
+  }
 };
 
 // Tiles of m query rows: no more than the rows need with one ragged tile per sequence, and
@@ -183,19 +186,20 @@ int64_t tile_bound(const cb_paged_kv* kv, int group, int m) {
 }
 
 AttentionPlan plan_attention(const cb_paged_kv* kv, int32_t heads) {
-  AttentionPlan p;
+  AttentionPlan p = {};
   const int group = heads / kv->kv_heads;
   p.tc = (int64_t)kv->max_new * group > PR_ROWS;
-  p.tile_rows = p.tc ? PT_ROWS : PR_ROWS;
-  p.tiles = tile_bound(kv, group, p.tile_rows);
+  p.tiles = tile_bound(kv, group, p.tc ? PT_ROWS : PR_ROWS);
   const int64_t have = std::max<int64_t>(1, p.tiles * kv->kv_heads);
-  // 16-row kernel: two CTAs share an SM; four per SM in all leave the last ones little to
-  // wait for. tcgen05 kernel: one CTA per SM.
-  const int64_t want = p.tc ? PG_SMS : 4 * PG_SMS;
-  const int step = p.tc ? PT_KEYS : PR_BLOCK, least = p.tc ? 512 : 256;
+  if (p.tc) {  // one CTA per SM, or as many as there can be steps
+    p.ctas = (int)std::min<double>(PG_SMS, (double)have * ceil_div(kv->max_len, PT_KEYS));
+    p.parts = (size_t)p.ctas * 2 * PT_ROWS;
+    return p;
+  }
+  // Two CTAs share an SM; four per SM in all leave the last ones little to wait for.
   const int64_t splits = std::max<int64_t>(
-      1, std::min<int64_t>(p.tc ? want / have : ceil_div(want, have), ceil_div(kv->max_len, least)));
-  p.keys = (int)(ceil_div(ceil_div(kv->max_len, splits), step) * step);
+      1, std::min<int64_t>(ceil_div(4 * PG_SMS, have), ceil_div(kv->max_len, 256)));
+  p.keys = (int)(ceil_div(ceil_div(kv->max_len, splits), PR_BLOCK) * PR_BLOCK);
   p.splits = (int)ceil_div(kv->max_len, p.keys);
   p.parts = (size_t)kv->rows * heads * p.splits;
   return p;
@@ -206,32 +210,37 @@ cb_status launch_attention(const cb_paged_kv* kv, const T* q, int64_t q_stride, 
                            float scale, T* out, int64_t out_stride, float* lse, float* workspace,
                            cudaStream_t st) {
   const AttentionPlan p = plan_attention(kv, heads);
-  const int64_t grid = p.tiles * kv->kv_heads * p.splits;
-  if (grid > INT_LIMIT) return CB_ERR_UNSUPPORTED;
   const int box = p.tc ? std::min(kv->page_size, PT_KEYS) : PR_BLOCK;
   CUtensorMap tk, tv;
   if (!make_cache_map(&tk, kv->k, kv, box) || !make_cache_map(&tv, kv->v, kv, box))
     return CB_ERR_UNSUPPORTED;
   const PagedKV d = device_kv(kv);
   const float scale_log2 = scale * 1.4426950408889634f;
-  PagedParts parts{workspace, workspace ? workspace + p.parts * PG_HD : nullptr, p.splits, p.keys};
+  float* part_lse = workspace ? workspace + p.parts * PG_HD : nullptr;
   cudaError_t e;
   if (p.tc) {
     static std::atomic<uint64_t> done{0};
     if ((e = allow_smem(paged_tile_kernel<T>, PT_SMEM, done)) != cudaSuccess) return status_of(e);
-    paged_tile_kernel<T><<<(unsigned)grid, PT_THREADS, PT_SMEM, st>>>(
+    const PtParts parts{workspace, part_lse, reinterpret_cast<PtJoin*>(part_lse + p.parts)};
+    paged_tile_kernel<T><<<p.ctas, PT_THREADS, PT_SMEM, st>>>(
         tk, tv, d, q, q_stride, heads, scale_log2, out, out_stride, lse, parts, box);
-  } else {
-    static std::atomic<uint64_t> done{0};
-    if ((e = allow_smem(paged_rows_kernel<T>, PR_SMEM, done)) != cudaSuccess) return status_of(e);
-    paged_rows_kernel<T><<<(unsigned)grid, PR_WARPS * 32, PR_SMEM, st>>>(
-        tk, tv, d, q, q_stride, heads, scale_log2, out, out_stride, lse, parts);
+    if ((e = cudaPeekAtLastError()) != cudaSuccess) return status_of(e);
+    paged_join_kernel<T><<<dim3(p.ctas, PT_ROWS / PJ_ROWS), PJ_WARPS * 32, 0, st>>>(
+        parts, heads, heads / kv->kv_heads, out, out_stride, lse);
+    return status_of(cudaPeekAtLastError());
   }
+  const int64_t grid = p.tiles * kv->kv_heads * p.splits;
+  if (grid > INT_LIMIT) return CB_ERR_UNSUPPORTED;
+  static std::atomic<uint64_t> done{0};
+  if ((e = allow_smem(paged_rows_kernel<T>, PR_SMEM, done)) != cudaSuccess) return status_of(e);
+  const PagedParts parts{workspace, part_lse, p.splits, p.keys};
+  paged_rows_kernel<T><<<(unsigned)grid, PR_WARPS * 32, PR_SMEM, st>>>(
+      tk, tv, d, q, q_stride, heads, scale_log2, out, out_stride, lse, parts);
   e = cudaPeekAtLastError();
   if (e == cudaSuccess && p.splits > 1) {
     const int64_t blocks = ceil_div((int64_t)kv->rows * heads, PC_WARPS);
-    paged_combine_kernel<T><<<(unsigned)blocks, PC_WARPS * 32, 0, st>>>(d, heads, parts, p.tile_rows,
-                                                                       out, out_stride, lse);
+    paged_combine_kernel<T><<<(unsigned)blocks, PC_WARPS * 32, 0, st>>>(d, heads, parts, out,
+                                                                       out_stride, lse);
     e = cudaPeekAtLastError();
   }
   return status_of(e);

@@ -272,12 +272,11 @@ __global__ void __launch_bounds__(PR_WARPS * 32, 2)
 }
 
 // Joins the parts of every row: out = sum_s 2^(lse_s - lse) o_s, lse = log2 sum_s 2^lse_s.
-// One warp per (row, head). tile_rows: query rows of a tile of the kernel that wrote the
-// parts; a tile has as many parts as its last row's slots need.
+// One warp per (row, head). A tile has as many parts as its last row's slots need.
 constexpr int PC_WARPS = 4;
 template <typename T>
 __global__ void __launch_bounds__(PC_WARPS * 32)
-    paged_combine_kernel(const PagedKV kv, int heads, const PagedParts parts, int tile_rows,
+    paged_combine_kernel(const PagedKV kv, int heads, const PagedParts parts,
                          T* __restrict__ out, int64_t out_stride, float* __restrict__ lse) {
   using H = Half16<T>;
   const int lane = threadIdx.x & 31;
@@ -296,7 +295,7 @@ __global__ void __launch_bounds__(PC_WARPS * 32)
   if (i < 0 || i >= seq.n) return;
   const int group = heads / kv.kv_heads;
   const int f = i * group + h % group;
-  const int last = min((f / tile_rows + 1) * tile_rows, seq.n * group) - 1;
+  const int last = min((f / PR_ROWS + 1) * PR_ROWS, seq.n * group) - 1;
   const int tile_end = max(0, seq.limit(last / group));
   const int n = min(parts.splits, max(1, (tile_end + parts.keys - 1) / parts.keys));
 

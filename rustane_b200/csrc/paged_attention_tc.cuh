@@ -7,16 +7,25 @@
 // cores' rate. 384 threads:
 //   warp 0       TMA producer: K and V steps, two buffers each; a page of the step per lane
 //                and half of the head (128-byte swizzle)
-//   warp 1       TMEM owner (512 columns); lane 0 issues the matrix instructions:
+//   warp 1       TMEM owner (512 columns); issues the matrix instructions:
 //                  S = Q K^T  (128 x 128 x 128) and O += P V  (P read from TMEM)
 //                in the order PV_A(j) S_A(j+1) PV_B(j) S_B(j+1): while one tile's products
-//                run, the other tile's softmax does
+//                run, the other tile's softmax does. PV starts when the first 64 keys' P are
+//                there, beside the exponentials of the others.
 //   warps 4-7    softmax of tile A, one thread per query row: 128 scores of a step in
 //   warps 8-11   registers (tile B likewise), running maximum and sum in 32 bits, P written
 //                over S. O in TMEM is rescaled only when the maximum has grown by 2^8 (P stays
 //                below 2^8, which both types hold).
 // A tile's S(j+1) is issued behind its PV(j), so "S(j+1) is full" also says that O may be
-// rescaled and that P(j) is no longer read: no further barriers are needed.
+// rescaled and that P(j) is no longer read. Steps of 64 keys with two S buffers a tile, and
+// two threads per row, hide the products' latency as well, but a step costs a warp about 60
+// instructions whatever its keys: both took 2.3 us for 128 keys.
+//
+// Sequences of a step differ in length and the number of tiles is rarely a multiple of the
+// SMs, so the steps of all tiles (sequence, key head, tile in this order: neighbours share
+// K and V in L2) are laid end to end and every CTA takes an equal share of them. A CTA that
+// has all steps of a tile writes its output; of a tile that is cut, each CTA writes its part
+// (at most two per CTA: its first and its last tile) and paged_join_kernel joins them.
 #pragma once
 #include "paged_attention.cuh"
 
@@ -25,62 +34,315 @@ namespace cb {
 constexpr int PT_SUB = 128;            // rows of a tile
 constexpr int PT_ROWS = 2 * PT_SUB;    // query rows of a CTA
 constexpr int PT_KEYS = 128;           // keys of a step
+constexpr int PT_BUFS = 2;             // K steps, and V steps, in flight
+constexpr int PT_STEP_BYTES = PT_KEYS * PG_HD * 2;
 constexpr int PT_THREADS = 384;
 constexpr int PT_Q_OFF = 0;            // [tile][half of the head][128 rows][128 B]
 constexpr int PT_K_OFF = 65536;        // [buffer][half][128 keys][128 B]
-constexpr int PT_V_OFF = 131072;
-constexpr int PT_BAR_OFF = 196608;
-constexpr int PT_SMEM = PT_BAR_OFF + 256 + 1024;
+constexpr int PT_V_OFF = PT_K_OFF + PT_BUFS * PT_STEP_BYTES;
+constexpr int PT_BAR_OFF = PT_V_OFF + PT_BUFS * PT_STEP_BYTES;
+constexpr int PT_SHARE_OFF = PT_BAR_OFF + 256;
+constexpr int PT_SMEM = PT_SHARE_OFF + 8192 + 64 + PT_THREADS / 32 * 64 + 1024;
 constexpr uint32_t PT_TMEM_COLS = 512;  // S_A, S_B, O_A, O_B: 128 columns each
 constexpr float PT_RESCALE = 8.0f;
 
 template <typename T>
-__device__ __forceinline__ constexpr uint32_t pt_idesc(bool b_mn) {
+__device__ __forceinline__ constexpr uint32_t pt_idesc(int n, bool b_mn) {
   // A and B formats: 0 = fp16, 1 = bf16
-  const uint32_t fmt = sizeof(T) == 2 && __is_same(T, __nv_bfloat16) ? (1u << 7) | (1u << 10) : 0u;
-  return (b_mn ? umma_idesc_f16_bmn(128, 128) : umma_idesc_f16(128, 128)) | fmt;
+  const uint32_t fmt = __is_same(T, __nv_bfloat16) ? (1u << 7) | (1u << 10) : 0u;
+  return (b_mn ? umma_idesc_f16_bmn(128, n) : umma_idesc_f16(128, n)) | fmt;
 }
 
-// Loads the Q rows f0 + r (r = 0 .. 127) of a key head into a K-major swizzled tile, one
-// thread per row; rows behind the sequence's last are zero.
+// Matrix instructions are issued by a whole warp with one lane's predicate, not by a branch
+// of one lane: the operands are warp-uniform then, and the descriptors (their low words;
+// the high word is the same for all) move on by additions. From a one-lane branch an
+// instruction took about 130 cycles to issue, twice its time in the tensor cores.
+constexpr uint32_t PT_DESC_HI = 64u | (1u << 14) | (2u << 29);  // 1024-byte groups, 128-byte swizzle
+__device__ __forceinline__ uint32_t pt_desc_k(uint32_t smem_addr) {  // K-major
+  return ((smem_addr & 0x3FFFFu) >> 4) | (1u << 16);
+}
+__device__ __forceinline__ uint32_t pt_desc_mn(uint32_t smem_addr, uint32_t lbo_bytes) {
+  return ((smem_addr & 0x3FFFFu) >> 4) | ((lbo_bytes >> 4) << 16);
+}
+__device__ __forceinline__ uint32_t pt_elect() {
+  uint32_t is;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+               : "=r"(is));
+  return is;
+}
+__device__ __forceinline__ void pt_mma_ss(uint32_t leader, uint32_t d, uint32_t a_lo, uint32_t b_lo,
+                                          uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\t.reg .b64 a, b;\n\t"
+      "setp.ne.b32 q, %0, 0;\n\tsetp.ne.b32 p, %6, 0;\n\t"
+      "mov.b64 a, {%2, %4};\n\tmov.b64 b, {%3, %4};\n\t"
+      "@q tcgen05.mma.cta_group::1.kind::f16 [%1], a, b, %5, p;\n\t}" ::"r"(leader),
+      "r"(d), "r"(a_lo), "r"(b_lo), "r"(PT_DESC_HI), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+__device__ __forceinline__ void pt_mma_ts(uint32_t leader, uint32_t d, uint32_t a_tmem,
+                                          uint32_t b_lo, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\t.reg .b64 b;\n\t"
+      "setp.ne.b32 q, %0, 0;\n\tsetp.ne.b32 p, %6, 0;\n\t"
+      "mov.b64 b, {%3, %4};\n\t"
+      "@q tcgen05.mma.cta_group::1.kind::f16 [%1], [%2], b, %5, p;\n\t}" ::"r"(leader),
+      "r"(d), "r"(a_tmem), "r"(b_lo), "r"(PT_DESC_HI), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+__device__ __forceinline__ void pt_commit(uint32_t leader, uint64_t* bar) {
+  asm volatile(
+      "{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %0, 0;\n\t"
+      "@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%1];\n\t}" ::"r"(
+          leader),
+      "r"(smem_u32(bar))
+      : "memory");
+}
+
+// Loads a warp's 32 query rows f0 + r (r = first .. first + 31) of a key head into a K-major
+// swizzled tile; rows behind the sequence's last are zero. Half a warp takes a row, so a load
+// meets whole lines (a row per lane took 2.6 us for the block's 256 rows).
 template <typename T>
 __device__ __forceinline__ void pt_load_q(uint8_t* tile, const T* __restrict__ q, int64_t q_stride,
-                                          const PagedSeq& seq, int head, int group, int f, int r) {
-  const int i = f / group;
-  uint4 x[16];
-  if (i < seq.n) {
-    const uint4* src = reinterpret_cast<const uint4*>(
-        q + (int64_t)(seq.row0 + i) * q_stride + (int64_t)(head * group + f - i * group) * PG_HD);
-#pragma unroll
-    for (int c = 0; c < 16; ++c) x[c] = __ldg(src + c);
-  } else {
-#pragma unroll
-    for (int c = 0; c < 16; ++c) x[c] = make_uint4(0, 0, 0, 0);
+                                          const PagedSeq& seq, int head, int group, int f0,
+                                          int first, int lane) {
+  const int c = lane & 15;
+  int r = first + (lane >> 4);
+  int i = (f0 + r) / group, g = f0 + r - i * group;
+#pragma unroll 2
+  for (int it = 0; it < 16; ++it) {
+    uint8_t* dst = tile + (c >> 3) * 16384 + r * 128 + (((c & 7) ^ (r & 7)) << 4);
+    if (i < seq.n)
+      cp_async_16(smem_u32(dst), q + (int64_t)(seq.row0 + i) * q_stride +
+                                     (int64_t)(head * group + g) * PG_HD + c * 8);
+    else
+      *reinterpret_cast<uint4*>(dst) = make_uint4(0, 0, 0, 0);
+    r += 2;
+    g += 2;
+    while (g >= group) {  // two rows on
+      g -= group;
+      ++i;
+    }
   }
-#pragma unroll
-  for (int c = 0; c < 16; ++c)
-    *reinterpret_cast<uint4*>(tile + (c >> 3) * 16384 + r * 128 + (((c & 7) ^ (r & 7)) << 4)) = x[c];
+  cp_async_commit();
+  cp_async_wait<0>();
 }
 
-// Producer side of a step: the lanes of a warp load the pages of keys key0 .. key0 + 127 into
-// a [half][128][128 B] buffer (box_rows keys each; absent pages and slots behind the table
+// Producer side of a step: the lanes of a warp load the pages of KEYS keys from key0 on into
+// a [half][KEYS][128 B] buffer (box_rows keys each; absent pages and slots behind the table
 // read as zero). id: the lane's page id of this step.
+template <int KEYS>
 __device__ __forceinline__ void pt_load_step(const CUtensorMap* map, uint8_t* dst, uint64_t* bar,
                                              const PagedKV& kv, int head, int key0, int id,
                                              int box_rows, int lane) {
-  if (lane == 0) mbar_arrive_expect_tx(bar, 32768);
+  if (lane == 0) mbar_arrive_expect_tx(bar, KEYS * 256);
   __syncwarp();
   const int part = lane >> 1, half = lane & 1;
-  if (part * box_rows < PT_KEYS) {
+  if (part * box_rows < KEYS) {
     const int row = id >= 0 ? kv.page_row(id, head, key0 + part * box_rows) : kv.cache_rows();
-    tma_load_2d(dst + half * 16384 + part * box_rows * 128, map, bar, half * 64, row);
+    tma_load_2d(dst + half * KEYS * 128 + part * box_rows * 128, map, bar, half * 64, row);
   }
 }
+template <int KEYS>
 __device__ __forceinline__ int pt_step_id(const PagedKV& kv, int b, int key0, int end,
                                           int box_rows, int lane) {
   const int key = key0 + (lane >> 1) * box_rows;
-  return (lane >> 1) * box_rows < PT_KEYS && key < end ? kv.page_id(b, key) : -1;
+  return (lane >> 1) * box_rows < KEYS && key < end ? kv.page_id(b, key) : -1;
 }
+
+// ------------------------------------------------------------------- the shares
+constexpr int PT_CHUNK = 1024;     // sequences whose steps are added up at a time
+constexpr int PT_LEAST = 4;        // fewer steps than this are not worth a CTA of their own
+
+// Steps of tile `tile` of a sequence: up to the last slot that its last row sees. A tile that
+// sees nothing has one step too (in which everything is masked): it writes its zeros.
+__device__ __forceinline__ int pt_tile_steps(const PagedSeq& seq, int group, int tile) {
+  const int last = min((tile + 1) * PT_ROWS, seq.n * group) - 1;
+  return max(1, (seq.limit(last / group) + PT_KEYS - 1) / PT_KEYS);
+}
+__device__ __forceinline__ int pt_tiles(const PagedSeq& seq, int group) {
+  return (seq.n * group + PT_ROWS - 1) / PT_ROWS;
+}
+
+// A CTA's walk over its share: segments of tiles.
+struct PtWalk {
+  PagedSeq seq;
+  int b, head, tile;
+  int j0, j1, steps;  // the segment: steps j0 .. j1 - 1 of the tile's `steps`
+  int64_t left;       // steps of the share from j0 on
+
+  __device__ __forceinline__ void segment(int group) {
+    steps = pt_tile_steps(seq, group, tile);
+    j1 = (int)min((int64_t)steps, j0 + left);
+  }
+  // The next segment; false when the share is done.
+  __device__ __forceinline__ bool next(const PagedKV& kv, int group) {
+    left -= j1 - j0;
+    if (left <= 0) return false;
+    j0 = 0;
+    if (++tile >= pt_tiles(seq, group)) {
+      tile = 0;
+      if (++head >= kv.kv_heads) {
+        head = 0;
+        do {
+          if (++b >= kv.batch) return false;
+          seq = paged_seq(kv, b);
+        } while (seq.n == 0);
+      }
+    }
+    segment(group);
+    return true;
+  }
+  __device__ __forceinline__ bool whole() const { return j0 == 0 && j1 == steps; }
+};
+
+struct PtShare {  // in shared memory
+  int64_t seq_steps[PT_CHUNK];
+  int64_t total;  // steps of all tiles and key heads
+  int64_t lo, hi;
+  int ctas;       // CTAs that have a share
+  int b, head, tile, j0;
+  PtWalk walk[PT_THREADS / 32];  // every warp's walk (registers are for the scores)
+};
+
+// First step of share c of `ctas` over `total` steps, and the share that a step lies in.
+__device__ __forceinline__ int64_t pt_share_begin(int64_t total, int ctas, int c) {
+  return total * c / ctas;
+}
+__device__ __forceinline__ int pt_share_of(int64_t total, int ctas, int64_t step) {
+  return (int)(((step + 1) * ctas - 1) / total);
+}
+
+// The whole block: adds up the steps of every sequence and finds where this CTA's share
+// begins. A warp per sequence when they are few, else a thread.
+__device__ __forceinline__ void pt_find_share(const PagedKV& kv, int group, PtShare& sh) {
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  auto sum_chunk = [&](int base, int count) {
+    if (count <= 96) {
+      for (int i = warp; i < count; i += PT_THREADS / 32) {
+        const PagedSeq s = paged_seq(kv, base + i);
+        const int tiles = pt_tiles(s, group);
+        int64_t n = 0;
+        for (int t = lane; t < tiles; t += 32) n += pt_tile_steps(s, group, t);
+#pragma unroll
+        for (int off = 16; off > 0; off >>= 1) n += __shfl_xor_sync(0xffffffffu, n, off);
+        if (lane == 0) sh.seq_steps[i] = n;
+      }
+    } else {
+      for (int i = threadIdx.x; i < count; i += PT_THREADS) {
+        const PagedSeq s = paged_seq(kv, base + i);
+        const int tiles = pt_tiles(s, group);
+        int64_t n = 0;
+        for (int t = 0; t < tiles; ++t) n += pt_tile_steps(s, group, t);
+        sh.seq_steps[i] = n;
+      }
+    }
+    __syncthreads();
+  };
+  // one warp: the sum of the chunk, or the sequence in it that holds step `want`
+  auto scan_chunk = [&](int count, int64_t before, int64_t want, int64_t& inside) -> int {
+    for (int i = 0; i < count; i += 32) {
+      const int64_t n = i + lane < count ? sh.seq_steps[i + lane] : 0;
+      int64_t incl = n;
+#pragma unroll
+      for (int off = 1; off < 32; off <<= 1) {
+        const int64_t up = __shfl_up_sync(0xffffffffu, incl, off);
+        if (lane >= off) incl += up;
+      }
+      const unsigned past = __ballot_sync(0xffffffffu, before + incl > want);
+      if (past) {
+        const int src = __ffs(past) - 1;
+        inside = want - before - __shfl_sync(0xffffffffu, incl - n, src);
+        return i + src;
+      }
+      before += __shfl_sync(0xffffffffu, incl, 31);
+    }
+    inside = before;  // not here: the steps so far
+    return -1;
+  };
+  int64_t total = 0;
+  for (int base = 0; base < kv.batch; base += PT_CHUNK) {
+    const int count = min(PT_CHUNK, kv.batch - base);
+    __syncthreads();
+    sum_chunk(base, count);
+    int64_t inside;
+    scan_chunk(count, total, INT64_MAX, inside);  // every warp, the same sum
+    total = inside;
+  }
+  const int64_t all = total * kv.kv_heads;
+  const int ctas = (int)max((int64_t)1, min((int64_t)gridDim.x, all / PT_LEAST));
+  const int c = blockIdx.x;
+  const int64_t lo = c < ctas ? pt_share_begin(all, ctas, c) : all;
+  const int64_t hi = c < ctas ? pt_share_begin(all, ctas, c + 1) : all;
+  if (lo < hi) {
+    // heads of one sequence lie side by side: step lo lies in the sequence that holds step
+    // lo / kv_heads of one head
+    const int64_t want = lo / kv.kv_heads;
+    int64_t before = 0;
+    for (int base = 0; base < kv.batch; base += PT_CHUNK) {
+      const int count = min(PT_CHUNK, kv.batch - base);
+      if (kv.batch > PT_CHUNK) {
+        __syncthreads();
+        sum_chunk(base, count);
+      }
+      int64_t inside;
+      const int i = scan_chunk(count, before, want, inside);
+      if (i >= 0) {
+        if (warp == 0) {
+          const int64_t one = sh.seq_steps[i];
+          int64_t r = lo - (want - inside) * kv.kv_heads;  // within the sequence
+          const int head = (int)(r / one);
+          r -= head * one;
+          const PagedSeq s = paged_seq(kv, base + i);
+          const int tiles = pt_tiles(s, group);
+          int64_t run = 0;
+          for (int t0 = 0; t0 < tiles; t0 += 32) {
+            const int n = t0 + lane < tiles ? pt_tile_steps(s, group, t0 + lane) : 0;
+            int64_t incl = n;
+#pragma unroll
+            for (int off = 1; off < 32; off <<= 1) {
+              const int64_t up = __shfl_up_sync(0xffffffffu, incl, off);
+              if (lane >= off) incl += up;
+            }
+            const unsigned past = __ballot_sync(0xffffffffu, run + incl > r);
+            if (past) {
+              if (lane == __ffs(past) - 1) {
+                sh.b = base + i;
+                sh.head = head;
+                sh.tile = t0 + lane;
+                sh.j0 = (int)(r - run - (incl - n));
+              }
+              break;
+            }
+            run += __shfl_sync(0xffffffffu, incl, 31);
+          }
+        }
+        break;
+      }
+      before = inside;
+    }
+  }
+  if (threadIdx.x == 0) {
+    sh.total = all;
+    sh.lo = lo;
+    sh.hi = hi;
+    sh.ctas = ctas;
+  }
+  __syncthreads();
+}
+
+// The parts of cut tiles, and what is to be joined. Part 2 c is CTA c's first segment, part
+// 2 c + 1 its last one.
+struct PtJoin {  // one per CTA: the tile that begins in its share and goes on behind it
+  int count;  // parts, 0 = no such tile
+  int first;  // part of this CTA; the others are 2 (c + 1), 2 (c + 2), ...
+  int row0, head, f0, rows;
+};
+struct PtParts {
+  float* o;    // [2 gridDim][128][256 rows] normalised within the part
+  float* lse;  // [2 gridDim][256]
+  PtJoin* join;
+};
 
 template <typename T>
 __global__ void __launch_bounds__(PT_THREADS, 1)
@@ -88,46 +350,28 @@ __global__ void __launch_bounds__(PT_THREADS, 1)
                       const __grid_constant__ CUtensorMap tmV, const PagedKV kv,
                       const T* __restrict__ q, int64_t q_stride, int heads, float scale_log2,
                       T* __restrict__ out, int64_t out_stride, float* __restrict__ lse,
-                      const PagedParts parts, int box_rows) {
+                      const PtParts parts, int box_rows) {
   using H = Half16<T>;
   extern __shared__ uint8_t pt_smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>(
       (reinterpret_cast<uintptr_t>(pt_smem_raw) + 1023) & ~uintptr_t(1023));
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + PT_BAR_OFF);
-  uint64_t* q_full = bars;
-  uint64_t* k_full = bars + 1;   // [2]
-  uint64_t* k_empty = bars + 3;  // [2]
-  uint64_t* v_full = bars + 5;   // [2]
-  uint64_t* v_empty = bars + 7;  // [2]
-  uint64_t* s_full = bars + 9;   // [2] tile A, tile B
-  uint64_t* p_full = bars + 11;  // [2]
-  uint64_t* o_full = bars + 13;  // [2]
-  uint64_t* drain = bars + 15;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 16);
-  int* failed = reinterpret_cast<int*>(bars + 17);
+  PtShare& sh = *reinterpret_cast<PtShare*>(smem + PT_SHARE_OFF);
+  uint64_t* k_full = bars;        // [2]
+  uint64_t* k_empty = bars + 2;   // [2]
+  uint64_t* v_full = bars + 4;    // [2]
+  uint64_t* v_empty = bars + 6;   // [2]
+  uint64_t* s_full = bars + 8;    // [tile]
+  uint64_t* p_full = bars + 10;   // [tile][first, last 64 keys]
+  uint64_t* o_full = bars + 14;   // [tile]
+  uint64_t* q_full = bars + 16;
+  uint64_t* drain = bars + 17;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 18);
+  int* failed = reinterpret_cast<int*>(bars + 19);
+  uint32_t* absent_of = reinterpret_cast<uint32_t*>(bars + 20);  // [4] absent pages of a step
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int group = heads / kv.kv_heads;
-  const int split = blockIdx.x % parts.splits;
-  const int rest = blockIdx.x / parts.splits;
-  const int head = rest % kv.kv_heads;
-  const PagedTile t = paged_find_tile<PT_ROWS>(kv, group, rest / kv.kv_heads);
-  if (t.b < 0) return;
-  const PagedSeq seq = t.seq;
-  const int f0 = t.tile * PT_ROWS;
-  const int rows = min(PT_ROWS, seq.n * group - f0);
-  const int k0 = split * parts.keys;
-  // steps of each tile: up to the last slot that its last row sees
-  int n_sub[2];
-#pragma unroll
-  for (int s = 0; s < 2; ++s) {
-    const int last = min(rows, (s + 1) * PT_SUB) - 1;
-    const int end = last < s * PT_SUB ? 0 : seq.limit((f0 + last) / group);
-    n_sub[s] = (max(0, min(end - k0, parts.keys)) + PT_KEYS - 1) / PT_KEYS;
-  }
-  const int n = max(n_sub[0], n_sub[1]);
-  if (split > 0 && n == 0) return;  // a part that the join does not ask for
-
   if (threadIdx.x == 0) {
     mbar_init(q_full, 8);
     mbar_init(drain, 1);
@@ -137,7 +381,8 @@ __global__ void __launch_bounds__(PT_THREADS, 1)
       mbar_init(&v_full[i], 1);
       mbar_init(&v_empty[i], 1);
       mbar_init(&s_full[i], 1);
-      mbar_init(&p_full[i], 4);
+      mbar_init(&p_full[2 * i], 4);
+      mbar_init(&p_full[2 * i + 1], 4);
       mbar_init(&o_full[i], 1);
     }
     *failed = 0;
@@ -145,6 +390,9 @@ __global__ void __launch_bounds__(PT_THREADS, 1)
     tma_prefetch_desc(&tmK);
     tma_prefetch_desc(&tmV);
   }
+  pt_find_share(kv, group, sh);
+  if (threadIdx.x == 0) parts.join[blockIdx.x].count = 0;  // (set below where a tile goes on)
+  if (sh.lo >= sh.hi) return;
   if (warp == 1) {
     tmem_alloc(tmem_slot, PT_TMEM_COLS);
     tmem_relinquish();
@@ -154,262 +402,412 @@ __global__ void __launch_bounds__(PT_THREADS, 1)
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
 
-  if (warp == 0) {
-    // ---------------- producer
-    const int end = min(seq.end, k0 + n * PT_KEYS);
-    int id = pt_step_id(kv, t.b, k0, end, box_rows, lane);
-    for (int j = 0; j < n; ++j) {
-      const int key0 = k0 + j * PT_KEYS, buf = j & 1;
-      const uint32_t free_parity = ((j >> 1) & 1) ^ 1u;
-      const int next = j + 1 < n ? pt_step_id(kv, t.b, key0 + PT_KEYS, end, box_rows, lane) : -1;
-      if (!mbar_wait(&k_empty[buf], free_parity, failed)) break;
-      pt_load_step(&tmK, smem + PT_K_OFF + buf * 32768, &k_full[buf], kv, head, key0, id, box_rows,
-                   lane);
-      if (!mbar_wait(&v_empty[buf], free_parity, failed)) break;
-      pt_load_step(&tmV, smem + PT_V_OFF + buf * 32768, &v_full[buf], kv, head, key0, id, box_rows,
-                   lane);
-      id = next;
-    }
-  } else if (warp == 1) {
-    if (lane == 0 && n > 0) {
+  PtWalk& w = sh.walk[warp];
+  if (lane == 0) {
+    w.b = sh.b;
+    w.head = sh.head;
+    w.tile = sh.tile;
+    w.j0 = sh.j0;
+    w.left = sh.hi - sh.lo;
+    w.seq = paged_seq(kv, w.b);
+    w.segment(group);
+  }
+  __syncwarp();
+  auto next_segment = [&]() -> bool {  // the whole warp
+    __syncwarp();
+    bool more = false;
+    if (lane == 0) more = w.next(kv, group);
+    return __any_sync(0xffffffffu, more);
+  };
+  // steps of the segment's two tiles, from j0 on
+  auto sub_steps = [&](int s) {
+    const int f = w.tile * PT_ROWS + s * PT_SUB, rows = w.seq.n * group;
+    if (f >= rows) return 0;
+    const int end = w.seq.limit((min(f + PT_SUB, rows) - 1) / group);
+    // the tile whose rows see nothing keeps the one step it has
+    const int n = max(w.steps == 1 ? 1 : 0, (end + PT_KEYS - 1) / PT_KEYS);
+    return max(0, min(n, w.j1) - w.j0);
+  };
+
+  // 128 x 72 + 256 x 216 registers of the 384 x 168 that the block was launched with
+  if (warp < 4) {
+    regs_dec<72>();
+    if (warp == 0) {
+      // ---------------- producer
+      uint32_t g = 0;  // steps loaded
+      bool ok = true;
+      do {
+        const int n = w.j1 - w.j0;
+        const int b = w.b, head = w.head, end = w.seq.end, first = w.j0 * PT_KEYS;
+        int id = pt_step_id<PT_KEYS>(kv, b, first, end, box_rows, lane);
+        for (int j = 0; ok && j < n; ++j, ++g) {
+          const int key0 = first + j * PT_KEYS, buf = g % PT_BUFS;
+          const uint32_t free_parity = ((g / PT_BUFS) & 1) ^ 1u;
+          const int next =
+              j + 1 < n ? pt_step_id<PT_KEYS>(kv, b, key0 + PT_KEYS, end, box_rows, lane) : -1;
+          // absent pages, a bit per 16 keys. (Four steps' words are kept: a step's is written
+          // when S of two steps before is done, which the softmax of the one four before
+          // precedes.)
+          const int part = lane >> 1;
+          const bool gone = (lane & 1) == 0 && part * box_rows < PT_KEYS &&
+                            key0 + part * box_rows < end && id < 0;
+          uint32_t absent = 0;
+          for (uint32_t parts_gone = __ballot_sync(0xffffffffu, gone); parts_gone;
+               parts_gone &= parts_gone - 1)
+            absent |= ((1u << (box_rows / 16)) - 1) << ((__ffs(parts_gone) - 1) / 2 * (box_rows / 16));
+          if (!(ok = mbar_wait(&k_empty[buf], free_parity, failed))) break;
+          if (lane == 0) absent_of[g & 3] = absent;
+          pt_load_step<PT_KEYS>(&tmK, smem + PT_K_OFF + buf * PT_STEP_BYTES, &k_full[buf], kv, head,
+                                key0, id, box_rows, lane);
+          if (!(ok = mbar_wait(&v_empty[buf], free_parity, failed))) break;
+          pt_load_step<PT_KEYS>(&tmV, smem + PT_V_OFF + buf * PT_STEP_BYTES, &v_full[buf], kv, head,
+                                key0, id, box_rows, lane);
+          id = next;
+        }
+      } while (__all_sync(0xffffffffu, ok) && next_segment());
+    } else if (warp == 1) {
       // ---------------- matrix instructions
-      constexpr uint32_t idesc_s = pt_idesc<T>(false), idesc_pv = pt_idesc<T>(true);
-      const uint32_t q_addr = smem_u32(smem + PT_Q_OFF);
-      const uint32_t k_addr = smem_u32(smem + PT_K_OFF);
-      const uint32_t v_addr = smem_u32(smem + PT_V_OFF);
-      auto issue_s = [&](int s, int j) {
+      constexpr uint32_t idesc_s = pt_idesc<T>(PT_KEYS, false), idesc_pv = pt_idesc<T>(128, true);
+      const uint32_t leader = pt_elect();
+      const uint32_t t0 = __shfl_sync(0xffffffffu, tmem, 0);
+      auto wait = [&](uint64_t* bar, uint32_t parity) -> bool {
+        const bool there = __all_sync(0xffffffffu, mbar_wait(bar, parity, failed));
+        tc_fence_after();
+        return there;
+      };
+      const uint32_t q_desc = pt_desc_k(smem_u32(smem + PT_Q_OFF));
+      const uint32_t k_desc = pt_desc_k(smem_u32(smem + PT_K_OFF));
+      const uint32_t v_desc = pt_desc_mn(smem_u32(smem + PT_V_OFF), PT_KEYS * 128);
+      auto issue_s = [&](int s, uint32_t g) {
+        const uint32_t a = q_desc + s * (32768 >> 4);
+        const uint32_t b = k_desc + (g % PT_BUFS) * (PT_STEP_BYTES >> 4);
 #pragma unroll
         for (int k = 0; k < 8; ++k) {  // head dim in steps of 16
-          const uint32_t off = (uint32_t)((k >> 2) * 16384 + (k & 3) * 32);
-          umma_f16_ss(tmem + s * 128, sw128_kmajor_desc(q_addr + s * 32768 + off),
-                      sw128_kmajor_desc(k_addr + (j & 1) * 32768 + off), idesc_s, k != 0);
+          const uint32_t off = (k >> 2) * (16384 >> 4) + (k & 3) * 2;
+          pt_mma_ss(leader, t0 + s * 128, a + off, b + off, idesc_s, k != 0);
         }
-        umma_commit(&s_full[s]);
+        pt_commit(leader, &s_full[s]);
       };
-      auto issue_pv = [&](int s, int j) {
+      auto issue_pv = [&](int s, uint32_t& gp, uint32_t g, bool first) -> bool {
+        const uint32_t b = v_desc + (g % PT_BUFS) * (PT_STEP_BYTES >> 4);
 #pragma unroll
-        for (int k = 0; k < 8; ++k)  // keys in steps of 16 (8 packed columns of P)
-          umma_f16_ts(tmem + 256 + s * 128, tmem + s * 128 + k * 8,
-                      sw128_mnmajor_desc(v_addr + (j & 1) * 32768 + k * 2048, 16384), idesc_pv,
-                      (j | k) != 0);
-      };
-      bool ok = mbar_wait(q_full, 0, failed) && mbar_wait(&k_full[0], 0, failed);
-      tc_fence_after();
-      if (ok) {
-        for (int s = 0; s < 2; ++s)
-          if (n_sub[s] > 0) issue_s(s, 0);
-        umma_commit(&k_empty[0]);
-      }
-      for (int j = 0; ok && j < n; ++j) {
-        const int buf = j & 1;
-        bool k_ready = false;
-        ok = mbar_wait(&v_full[buf], (j >> 1) & 1, failed);
-        for (int s = 0; ok && s < 2; ++s) {
-          if (j >= n_sub[s]) continue;
-          if (!(ok = mbar_wait(&p_full[s], j & 1, failed))) break;
-          tc_fence_after();
-          issue_pv(s, j);
-          if (s == 1 || j >= n_sub[1]) umma_commit(&v_empty[buf]);
-          if (j + 1 < n_sub[s]) {
-            if (!k_ready && !(ok = mbar_wait(&k_full[buf ^ 1], ((j + 1) >> 1) & 1, failed))) break;
-            k_ready = true;
-            tc_fence_after();
-            issue_s(s, j + 1);
-          } else {
-            umma_commit(&o_full[s]);
-          }
+        for (int half = 0; half < 2; ++half) {
+          if (!wait(&p_full[s * 2 + half], gp & 1)) return false;
+#pragma unroll
+          for (int k = half * 4; k < half * 4 + 4; ++k)  // keys in steps of 16 (8 columns of P)
+            pt_mma_ts(leader, t0 + 256 + s * 128, t0 + s * 128 + k * 8, b + k * (2048 >> 4),
+                      idesc_pv, !first || k != 0);
         }
-        if (ok && j + 1 < n) umma_commit(&k_empty[buf ^ 1]);
-      }
-      umma_commit(drain);  // nothing is in flight when TMEM is given back
+        ++gp;
+        return true;
+      };
+      uint32_t g = 0, seg = 0, gpA = 0, gpB = 0;  // steps, segments, P of tiles A and B
+      bool ok = true;
+      do {
+        const int n = __shfl_sync(0xffffffffu, w.j1 - w.j0, 0);
+        const int nA = __shfl_sync(0xffffffffu, sub_steps(0), 0);
+        const int nB = __shfl_sync(0xffffffffu, sub_steps(1), 0);
+        if (!(ok = wait(q_full, seg & 1))) break;
+        if (!(ok = wait(&k_full[g % PT_BUFS], (g / PT_BUFS) & 1))) break;
+        if (nA > 0) issue_s(0, g);
+        if (nB > 0) issue_s(1, g);
+        pt_commit(leader, &k_empty[g % PT_BUFS]);
+        for (int j = 0; ok && j < n; ++j) {
+          const uint32_t h = g + j;
+          if (!(ok = wait(&v_full[h % PT_BUFS], (h / PT_BUFS) & 1))) break;
+          if (j < nA) {
+            if (!(ok = issue_pv(0, gpA, h, j == 0))) break;
+            if (j >= nB) pt_commit(leader, &v_empty[h % PT_BUFS]);
+            if (j + 1 < nA) {
+              if (!(ok = wait(&k_full[(h + 1) % PT_BUFS], ((h + 1) / PT_BUFS) & 1))) break;
+              issue_s(0, h + 1);
+            } else {
+              pt_commit(leader, &o_full[0]);
+            }
+          }
+          if (j < nB) {
+            if (!(ok = issue_pv(1, gpB, h, j == 0))) break;
+            pt_commit(leader, &v_empty[h % PT_BUFS]);
+            if (j + 1 < nB) {
+              if (!(ok = wait(&k_full[(h + 1) % PT_BUFS], ((h + 1) / PT_BUFS) & 1))) break;
+              issue_s(1, h + 1);
+            } else {
+              pt_commit(leader, &o_full[1]);
+            }
+          }
+          if (j + 1 < n) pt_commit(leader, &k_empty[(h + 1) % PT_BUFS]);
+        }
+        // also for a tile without steps in this segment: no tile's warps run ahead of the
+        // others by a segment
+        if (ok && nA == 0) pt_commit(leader, &o_full[0]);
+        if (ok && nB == 0) pt_commit(leader, &o_full[1]);
+        g += n;
+        ++seg;
+      } while (ok && next_segment());
+      pt_commit(leader, drain);  // nothing is in flight when TMEM is given back
       mbar_wait(drain, 0, failed);
     }
-  } else if (warp >= 4) {
+  } else {
+    regs_inc<216>();
     // ---------------- softmax: thread = query row r of tile s
     const int s = (warp - 4) >> 2, quad = warp & 3;
     const int r = quad * 32 + lane;
-    const int f = f0 + s * PT_SUB + r;
     uint8_t* q_tile = smem + PT_Q_OFF + s * 32768;
-    pt_load_q(q_tile, q, q_stride, seq, head, group, f, r);
-    fence_proxy_async_smem();
-    __syncwarp();
-    if (lane == 0) mbar_arrive(q_full);
-
-    const int i = f / group;
-    const bool valid = i < seq.n;
-    const int lim = valid ? seq.limit(i) : 0;
-    // every row of the tile sees the slots below this
-    const int lim_all = s * PT_SUB + PT_SUB <= rows ? seq.limit((f0 + s * PT_SUB) / group) : 0;
-    const int n_s = s == 0 ? n_sub[0] : n_sub[1];
     const uint32_t lane_off = (uint32_t)(quad * 32) << 16;
     const uint32_t t_s = tmem + s * 128 + lane_off, t_o = tmem + 256 + s * 128 + lane_off;
-    float m = -CUDART_INF_F, l = 0.f;
+    uint32_t g0 = 0;       // steps of the segments before
+    uint32_t gs = 0;       // S taken of this tile
+    uint32_t seg = 0;      // segments before this one
     bool ok = true;
-    for (int j = 0; j < n_s; ++j) {
-      const int key0 = k0 + j * PT_KEYS;
-      // absent pages of this step, a bit per 16 keys
-      bool gone = false;
-      if (lane < PT_KEYS / 16 && key0 + lane * 16 < seq.end)
-        gone = kv.page_id(t.b, key0 + lane * 16) < 0;
-      const uint32_t absent = __ballot_sync(0xffffffffu, gone);
-      if (!mbar_wait(&s_full[s], j & 1, failed)) { ok = false; break; }
-      tc_fence_after();
-      uint32_t u[4][32];
-#pragma unroll
-      for (int c = 0; c < 4; ++c) tmem_ld_32x32b_x32(t_s + c * 32, u[c]);
-#pragma unroll
-      for (int c = 0; c < 4; ++c) tmem_ld_wait_regs(u[c]);
-      if (absent || key0 + PT_KEYS > lim_all) {
-#pragma unroll
-        for (int c = 0; c < 4; ++c)
-#pragma unroll
-          for (int e = 0; e < 32; ++e)
-            if (key0 + c * 32 + e >= lim || (absent >> (c * 2 + e / 16) & 1u))
-              u[c][e] = 0xff800000u;  // -inf
-      }
-      float mx[4];
-#pragma unroll
-      for (int c = 0; c < 4; ++c) {
-        mx[c] = __uint_as_float(u[c][0]);
-#pragma unroll
-        for (int e = 1; e < 31; e += 2)
-          mx[c] = fmax3(mx[c], __uint_as_float(u[c][e]), __uint_as_float(u[c][e + 1]));
-        mx[c] = fmaxf(mx[c], __uint_as_float(u[c][31]));
-      }
-      const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * scale_log2;
-      float corr = 1.0f;
-      bool need = false;
-      if (j == 0) {
-        m = top;
-      } else if (top > m + PT_RESCALE) {  // also when nothing was seen so far (m = -inf)
-        corr = exp2_mufu(m - top);
-        m = top;
-        l *= corr;
-        need = true;
-      }
-      if (__any_sync(0xffffffffu, need)) {
-#pragma unroll 1
-        for (int c = 0; c < 8; ++c) {
-          uint32_t o[16];
-          tmem_ld_32x32b_x16(t_o + c * 16, o);
-          tmem_ld_wait_regs16(o);
-#pragma unroll
-          for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * corr);
-          tmem_st_32x32b_x16(t_o + c * 16, o);
-        }
-      }
-      const float base = m == -CUDART_INF_F ? 0.f : m;
-      const float2 sc2 = make_float2(scale_log2, scale_log2), nb2 = make_float2(-base, -base);
-      float2 sum[4];
-#pragma unroll
-      for (int c = 0; c < 4; ++c) {
-        sum[c] = make_float2(0.f, 0.f);
-        uint32_t p[16];
-#pragma unroll
-        for (int e = 0; e < 16; ++e) {
-          float2 x = ffma2(make_float2(__uint_as_float(u[c][2 * e]), __uint_as_float(u[c][2 * e + 1])),
-                           sc2, nb2);
-          x.x = exp2_mufu(x.x);
-          x.y = exp2_mufu(x.y);
-          sum[c] = fadd2(sum[c], x);
-          // P rounds to the cache's type: at most half a step of each weight, the size of the
-          // output's own rounding
-          p[e] = H::pack(x.x, x.y);
-        }
-        tmem_st_32x32b_x16(t_s + c * 16, p);
-      }
-      sum[0] = fadd2(fadd2(sum[0], sum[1]), fadd2(sum[2], sum[3]));
-      l += sum[0].x + sum[0].y;
-      if (key0 + PT_KEYS > seq.end) {
-        // slots behind the sequence may hold anything, and 0 x NaN is not 0: zero their V
-        const int row0 = seq.end - key0;  // 1 .. 127
-        if (!mbar_wait(&v_full[j & 1], (j >> 1) & 1, failed)) { ok = false; break; }
-        uint8_t* v = smem + PT_V_OFF + (j & 1) * 32768;
-        if (r >= row0) {
-#pragma unroll
-          for (int c = 0; c < 16; ++c)
-            *reinterpret_cast<uint4*>(v + (c >> 3) * 16384 + r * 128 + (c & 7) * 16) =
-                make_uint4(0, 0, 0, 0);
-        }
-        fence_proxy_async_smem();
-      }
-      tmem_st_wait();
-      tc_fence_before();
+    int64_t at = sh.lo;    // the segment's first step among all
+    do {
+      const PagedSeq seq = w.seq;
+      const int key_first = w.j0 * PT_KEYS;
+      const int f_sub = w.tile * PT_ROWS + s * PT_SUB, f = f_sub + r;
+      pt_load_q(q_tile, q, q_stride, seq, w.head, group, f_sub, quad * 32, lane);
+      fence_proxy_async_smem();
       __syncwarp();
-      if (lane == 0) mbar_arrive(&p_full[s]);
-    }
-    // ---------------- the tile's output
-    const int h = head * group + f - i * group;
-    const int64_t row = (int64_t)seq.row0 + i;
-    const float inv = l == 0.f ? 0.f : 1.0f / l;
-    const float row_lse = l == 0.f ? -CUDART_INF_F : m + log2f(l);
-    if (ok && n_s > 0) ok = mbar_wait(&o_full[s], 0, failed);
-    tc_fence_after();
-    if (ok) {
-      if (parts.splits > 1) {
-        const int64_t part = (row * heads + h) * parts.splits + split;
-        if (valid) parts.lse[part] = row_lse;
+      if (lane == 0) mbar_arrive(q_full);
+
+      const int i = f / group;
+      const bool valid = i < seq.n;
+      const int lim = valid ? seq.limit(i) : 0;
+      // every row of the tile sees the slots below this
+      const int lim_all = f_sub + PT_SUB <= seq.n * group ? seq.limit(f_sub / group) : 0;
+      const int n_s = sub_steps(s);
+      float m = -CUDART_INF_F, l = 0.f;
+      for (int j = 0; j < n_s; ++j, ++gs) {
+        const int key0 = key_first + j * PT_KEYS;
+        ok = mbar_wait(&s_full[s], gs & 1, failed);
+        __syncwarp();
+        if (!__all_sync(0xffffffffu, ok)) break;
+        tc_fence_after();
+        uint32_t u[4][32];
+#pragma unroll
+        for (int c = 0; c < 4; ++c) tmem_ld_32x32b_x32(t_s + c * 32, u[c]);
+        const uint32_t absent = absent_of[(g0 + j) & 3];
+#pragma unroll
+        for (int c = 0; c < 4; ++c) tmem_ld_wait_regs(u[c]);
+        if (absent || key0 + PT_KEYS > lim_all) {
+#pragma unroll
+          for (int c = 0; c < 4; ++c)
+#pragma unroll
+            for (int e = 0; e < 32; ++e)
+              if (key0 + c * 32 + e >= lim || (absent >> (c * 2 + e / 16) & 1u))
+                u[c][e] = 0xff800000u;  // -inf
+        }
+        float mx[4];
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          mx[c] = __uint_as_float(u[c][0]);
+#pragma unroll
+          for (int e = 1; e < 31; e += 2)
+            mx[c] = fmax3(mx[c], __uint_as_float(u[c][e]), __uint_as_float(u[c][e + 1]));
+          mx[c] = fmaxf(mx[c], __uint_as_float(u[c][31]));
+        }
+        const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * scale_log2;
+        float corr = 1.0f;
+        bool need = false;
+        if (j == 0) {
+          m = top;
+        } else if (top > m + PT_RESCALE) {  // also when nothing was seen so far (m = -inf)
+          corr = exp2_mufu(m - top);
+          m = top;
+          l *= corr;
+          need = true;
+        }
+        if (__any_sync(0xffffffffu, need)) {
+#pragma unroll 1
+          for (int c = 0; c < 8; ++c) {
+            uint32_t o[16];
+            tmem_ld_32x32b_x16(t_o + c * 16, o);
+            tmem_ld_wait_regs16(o);
+#pragma unroll
+            for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * corr);
+            tmem_st_32x32b_x16(t_o + c * 16, o);
+          }
+        }
+        if (key0 + PT_KEYS > seq.end) {
+          // slots behind the sequence may hold anything, and 0 x NaN is not 0: zero their V
+          const uint32_t g = g0 + j;
+          ok = mbar_wait(&v_full[g % PT_BUFS], (g / PT_BUFS) & 1, failed);
+          uint8_t* v = smem + PT_V_OFF + (g % PT_BUFS) * PT_STEP_BYTES;
+          if (r >= seq.end - key0) {
+#pragma unroll
+            for (int c = 0; c < 16; ++c)
+              *reinterpret_cast<uint4*>(v + (c >> 3) * 16384 + r * 128 + (c & 7) * 16) =
+                  make_uint4(0, 0, 0, 0);
+          }
+          fence_proxy_async_smem();
+          __syncwarp();
+        }
+        const float base = m == -CUDART_INF_F ? 0.f : m;
+        const float2 sc2 = make_float2(scale_log2, scale_log2), nb2 = make_float2(-base, -base);
+        float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          uint32_t p[16];
+#pragma unroll
+          for (int e = 0; e < 16; ++e) {
+            float2 x = ffma2(make_float2(__uint_as_float(u[c][2 * e]), __uint_as_float(u[c][2 * e + 1])),
+                             sc2, nb2);
+            x.x = exp2_mufu(x.x);
+            x.y = exp2_mufu(x.y);
+            sum[e & 1] = fadd2(sum[e & 1], x);
+            // P rounds to the cache's type: at most half a step of each weight, the size of
+            // the output's own rounding
+            p[e] = H::pack(x.x, x.y);
+          }
+          tmem_st_32x32b_x16(t_s + c * 16, p);
+          if (c & 1) {  // 64 keys' P are there
+            tmem_st_wait();
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&p_full[s * 2 + (c >> 1)]);
+          }
+        }
+        sum[0] = fadd2(sum[0], sum[1]);
+        l += sum[0].x + sum[0].y;
+      }
+      // ---------------- the segment's output
+      const int h = w.head * group + f - i * group;
+      const float inv = l == 0.f ? 0.f : 1.0f / l;
+      const float row_lse = l == 0.f ? -CUDART_INF_F : m + log2f(l);
+      const bool some = n_s > 0 && l != 0.f;
+      if (ok) ok = mbar_wait(&o_full[s], seg & 1, failed);
+      __syncwarp();
+      if (!__all_sync(0xffffffffu, ok)) break;
+      tc_fence_after();
+      if (!w.whole()) {
+        const int part = 2 * blockIdx.x + (seg == 0 ? 0 : 1);
+        if (valid) parts.lse[part * PT_ROWS + s * PT_SUB + r] = row_lse;
+        // [128][256 rows]: a warp's store is one line
+        float* po = parts.o + (int64_t)part * PG_HD * PT_ROWS + s * PT_SUB + r;
 #pragma unroll 1
         for (int c = 0; c < 4; ++c) {
           uint32_t o[32];
-          if (n_s > 0) {
-            tmem_ld_32x32b_x32(t_o + c * 32, o);
-            tmem_ld_wait_regs(o);
-          }
-          if (valid) {
+          tmem_ld_32x32b_x32(t_o + c * 32, o);
+          tmem_ld_wait_regs(o);
 #pragma unroll
-            for (int e = 0; e < 8; ++e) {
-              float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
-              if (n_s > 0 && l != 0.f)
-                x = make_float4(__uint_as_float(o[4 * e]) * inv, __uint_as_float(o[4 * e + 1]) * inv,
-                                __uint_as_float(o[4 * e + 2]) * inv,
-                                __uint_as_float(o[4 * e + 3]) * inv);
-              *reinterpret_cast<float4*>(parts.o + part * PG_HD + c * 32 + e * 4) = x;
-            }
-          }
+          for (int e = 0; e < 32; ++e)
+            po[e * PT_ROWS] = some ? __uint_as_float(o[e]) * inv : 0.f;
+          po += 32 * PT_ROWS;
+        }
+        if (w.j0 == 0 && threadIdx.x == 128) {  // begins here, goes on in the next shares
+          const int last = pt_share_of(sh.total, sh.ctas, at + w.steps - 1);
+          PtJoin jn;
+          jn.count = last - blockIdx.x + 1;
+          jn.first = part;
+          jn.row0 = seq.row0;
+          jn.head = w.head;
+          jn.f0 = w.tile * PT_ROWS;
+          jn.rows = min(PT_ROWS, seq.n * group - jn.f0);
+          parts.join[blockIdx.x] = jn;
         }
       } else {
-        if (lse && valid) lse[row * heads + h] = row_lse;
+        if (lse && valid) lse[((int64_t)seq.row0 + i) * heads + h] = row_lse;
         // through the Q tile (no S reads it any more), so that half a warp writes a whole row
 #pragma unroll 1
         for (int c = 0; c < 4; ++c) {
           uint32_t o[32];
-          if (n_s > 0) {
-            tmem_ld_32x32b_x32(t_o + c * 32, o);
-            tmem_ld_wait_regs(o);
-          }
+          tmem_ld_32x32b_x32(t_o + c * 32, o);
+          tmem_ld_wait_regs(o);
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
-            uint4 w = make_uint4(0, 0, 0, 0);
-            if (n_s > 0 && l != 0.f) {
-              w.x = H::pack(__uint_as_float(o[8 * e]) * inv, __uint_as_float(o[8 * e + 1]) * inv);
-              w.y = H::pack(__uint_as_float(o[8 * e + 2]) * inv, __uint_as_float(o[8 * e + 3]) * inv);
-              w.z = H::pack(__uint_as_float(o[8 * e + 4]) * inv, __uint_as_float(o[8 * e + 5]) * inv);
-              w.w = H::pack(__uint_as_float(o[8 * e + 6]) * inv, __uint_as_float(o[8 * e + 7]) * inv);
+            uint4 y = make_uint4(0, 0, 0, 0);
+            if (some) {
+              y.x = H::pack(__uint_as_float(o[8 * e]) * inv, __uint_as_float(o[8 * e + 1]) * inv);
+              y.y = H::pack(__uint_as_float(o[8 * e + 2]) * inv, __uint_as_float(o[8 * e + 3]) * inv);
+              y.z = H::pack(__uint_as_float(o[8 * e + 4]) * inv, __uint_as_float(o[8 * e + 5]) * inv);
+              y.w = H::pack(__uint_as_float(o[8 * e + 6]) * inv, __uint_as_float(o[8 * e + 7]) * inv);
             }
             const int chunk = c * 4 + e;
             *reinterpret_cast<uint4*>(q_tile + (chunk >> 3) * 16384 + r * 128 +
-                                      (((chunk & 7) ^ (r & 7)) << 4)) = w;
+                                      (((chunk & 7) ^ (r & 7)) << 4)) = y;
           }
         }
         __syncwarp();
         const int chunk = lane & 15;
-        for (int rr = quad * 32 + (lane >> 4); rr < quad * 32 + 32; rr += 2) {
-          const int ff = f0 + s * PT_SUB + rr, ii = ff / group;
-          if (ii >= seq.n) break;
-          const uint4 w = *reinterpret_cast<const uint4*>(
-              q_tile + (chunk >> 3) * 16384 + rr * 128 + (((chunk & 7) ^ (rr & 7)) << 4));
-          *reinterpret_cast<uint4*>(out + ((int64_t)seq.row0 + ii) * out_stride +
-                                    (int64_t)(head * group + ff - ii * group) * PG_HD + chunk * 8) = w;
+        int rr = quad * 32 + (lane >> 4);
+        int ii = (f_sub + rr) / group, gg = f_sub + rr - ii * group;
+#pragma unroll 2
+        for (int it = 0; it < 16; ++it) {
+          if (ii < seq.n) {
+            const uint4 y = *reinterpret_cast<const uint4*>(
+                q_tile + (chunk >> 3) * 16384 + rr * 128 + (((chunk & 7) ^ (rr & 7)) << 4));
+            *reinterpret_cast<uint4*>(out + ((int64_t)seq.row0 + ii) * out_stride +
+                                      (int64_t)(w.head * group + gg) * PG_HD + chunk * 8) = y;
+          }
+          rr += 2;
+          gg += 2;
+          while (gg >= group) {
+            gg -= group;
+            ++ii;
+          }
         }
+        __syncwarp();  // the next Q goes over it
       }
-    }
+      tc_fence_before();
+      g0 += w.j1 - w.j0;
+      at += w.j1 - w.j0;
+      ++seg;
+    } while (next_segment());
     tc_fence_before();
   }
   __syncthreads();
   if (warp == 1) {
     tc_fence_after();
     tmem_dealloc(tmem, PT_TMEM_COLS);
+  }
+}
+
+// Joins the parts of the tile that begins in share blockIdx.x and goes on behind it:
+// out = sum_p 2^(lse_p - lse) o_p. A block takes 32 rows; a warp reads the parts of 32 rows
+// at once (whole lines) and the block writes whole rows through shared memory.
+constexpr int PJ_ROWS = 32;
+constexpr int PJ_WARPS = 8;
+template <typename T>
+__global__ void __launch_bounds__(PJ_WARPS * 32)
+    paged_join_kernel(const PtParts parts, int heads, int group, T* __restrict__ out,
+                      int64_t out_stride, float* __restrict__ lse) {
+  using H = Half16<T>;
+  const PtJoin jn = parts.join[blockIdx.x];
+  const int r0 = blockIdx.y * PJ_ROWS;
+  if (jn.count == 0 || r0 >= jn.rows) return;
+  __shared__ float tile[PJ_ROWS][PG_HD + 1];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int r = r0 + lane;
+  auto part_of = [&](int p) { return p == 0 ? jn.first : 2 * ((int)blockIdx.x + p); };
+  float mx = -CUDART_INF_F;
+  for (int p = 0; p < jn.count; ++p) mx = fmaxf(mx, parts.lse[part_of(p) * PT_ROWS + r]);
+  const float base = mx == -CUDART_INF_F ? 0.f : mx;
+  constexpr int PER = PG_HD / PJ_WARPS;
+  float sum = 0.f, acc[PER];
+#pragma unroll
+  for (int e = 0; e < PER; ++e) acc[e] = 0.f;
+  for (int p = 0; p < jn.count; ++p) {
+    const int part = part_of(p);
+    const float c = exp2_mufu(parts.lse[part * PT_ROWS + r] - base);
+    const float* po = parts.o + ((int64_t)part * PG_HD + warp * PER) * PT_ROWS + r;
+    sum += c;
+#pragma unroll
+    for (int e = 0; e < PER; ++e) acc[e] = fmaf(c, po[e * PT_ROWS], acc[e]);
+  }
+  const float inv = sum == 0.f ? 0.f : 1.0f / sum;
+#pragma unroll
+  for (int e = 0; e < PER; ++e) tile[lane][warp * PER + e] = acc[e] * inv;
+  const int f = jn.f0 + r, i = f / group;
+  if (lse && warp == 0 && r < jn.rows)
+    lse[((int64_t)jn.row0 + i) * heads + jn.head * group + f - i * group] =
+        sum == 0.f ? -CUDART_INF_F : mx + log2f(sum);
+  __syncthreads();
+  for (int rr = warp; rr < PJ_ROWS && r0 + rr < jn.rows; rr += PJ_WARPS) {
+    const int ff = jn.f0 + r0 + rr, ii = ff / group;
+    uint2 y;
+    y.x = H::pack(tile[rr][lane * 4], tile[rr][lane * 4 + 1]);
+    y.y = H::pack(tile[rr][lane * 4 + 2], tile[rr][lane * 4 + 3]);
+    *reinterpret_cast<uint2*>(out + ((int64_t)jn.row0 + ii) * out_stride +
+                              (int64_t)(jn.head * group + ff - ii * group) * PG_HD + lane * 4) = y;
   }
 }
 

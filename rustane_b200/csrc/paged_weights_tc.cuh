@@ -108,7 +108,7 @@ __global__ void __launch_bounds__(WT_THREADS, 1)
     __syncwarp();
     for (int s = 0; s < tiles; ++s) {
       const int k = key0 + s * 128;
-      const int id = pt_step_id(kv, b, k, seq.end, box_rows, lane);
+      const int id = pt_step_id<128>(kv, b, k, seq.end, box_rows, lane);
       const int part = lane >> 1, half = lane & 1;
       if (part * box_rows < 128) {
         const int row = id >= 0 ? kv.page_row(id, head, k + part * box_rows) : kv.cache_rows();
@@ -130,7 +130,7 @@ __global__ void __launch_bounds__(WT_THREADS, 1)
   } else if (warp == 1) {
     if (lane == 0) {
       // ---------------- matrix instructions
-      constexpr uint32_t idesc = pt_idesc<T>(false);
+      constexpr uint32_t idesc = pt_idesc<T>(128, false);
       const uint32_t k_addr = smem_u32(smem + WT_K_OFF), q_addr = smem_u32(smem + WT_Q_OFF);
       bool ok = mbar_wait(k_full, 0, failed);
       for (int j = 0; ok && j < steps; ++j) {
