@@ -23,7 +23,8 @@
 //
 // Sequences of a step differ in length and the number of tiles is rarely a multiple of the
 // SMs, so the steps of all tiles (sequence, key head, tile in this order: neighbours share
-// K and V in L2) are laid end to end and every CTA takes an equal share of them. A CTA that
+// K and V in L2), and a unit or two for each tile's own cost, are laid end to end and every
+// CTA takes an equal share of them. A CTA that
 // has all steps of a tile writes its output; of a tile that is cut, each CTA writes its part
 // (at most two per CTA: its first and its last tile) and paged_join_kernel joins them.
 #pragma once
@@ -42,7 +43,7 @@ constexpr int PT_K_OFF = 65536;        // [buffer][half][128 keys][128 B]
 constexpr int PT_V_OFF = PT_K_OFF + PT_BUFS * PT_STEP_BYTES;
 constexpr int PT_BAR_OFF = PT_V_OFF + PT_BUFS * PT_STEP_BYTES;
 constexpr int PT_SHARE_OFF = PT_BAR_OFF + 256;
-constexpr int PT_SMEM = PT_SHARE_OFF + 8192 + 64 + PT_THREADS / 32 * 64 + 1024;
+constexpr int PT_SMEM = PT_SHARE_OFF + 8192 + 64 + PT_THREADS / 32 * 80 + 1024;
 constexpr uint32_t PT_TMEM_COLS = 512;  // S_A, S_B, O_A, O_B: 128 columns each
 constexpr float PT_RESCALE = 8.0f;
 
@@ -151,8 +152,11 @@ __device__ __forceinline__ int pt_step_id(const PagedKV& kv, int b, int key0, in
 }
 
 // ------------------------------------------------------------------- the shares
-constexpr int PT_CHUNK = 1024;     // sequences whose steps are added up at a time
-constexpr int PT_LEAST = 4;        // fewer steps than this are not worth a CTA of their own
+constexpr int PT_CHUNK = 1024;  // sequences whose units are added up at a time
+// A tile counts its steps and this many units for its Q, its pipeline's start and its output
+// (a step takes 1.9 us, a tile 4 to 5 us beside its steps).
+constexpr int PT_TILE_UNITS = 2;
+constexpr int PT_LEAST = 4;     // units of a share; above PT_TILE_UNITS, so each has a step
 
 // Steps of tile `tile` of a sequence: up to the last slot that its last row sees. A tile that
 // sees nothing has one step too (in which everything is masked): it writes its zeros.
@@ -168,52 +172,61 @@ __device__ __forceinline__ int pt_tiles(const PagedSeq& seq, int group) {
 struct PtWalk {
   PagedSeq seq;
   int b, head, tile;
+  int u0;             // the segment's first unit within the tile
   int j0, j1, steps;  // the segment: steps j0 .. j1 - 1 of the tile's `steps`
-  int64_t left;       // steps of the share from j0 on
+  int64_t at, end;    // the segment's first unit among all, and the share's end
 
+  __device__ __forceinline__ int u1() const {
+    return (int)min((int64_t)(steps + PT_TILE_UNITS), u0 + (end - at));
+  }
   __device__ __forceinline__ void segment(int group) {
     steps = pt_tile_steps(seq, group, tile);
-    j1 = (int)min((int64_t)steps, j0 + left);
+    j0 = max(0, u0 - PT_TILE_UNITS);
+    j1 = max(0, u1() - PT_TILE_UNITS);
   }
   // The next segment; false when the share is done.
   __device__ __forceinline__ bool next(const PagedKV& kv, int group) {
-    left -= j1 - j0;
-    if (left <= 0) return false;
-    j0 = 0;
-    if (++tile >= pt_tiles(seq, group)) {
-      tile = 0;
-      if (++head >= kv.kv_heads) {
-        head = 0;
-        do {
-          if (++b >= kv.batch) return false;
-          seq = paged_seq(kv, b);
-        } while (seq.n == 0);
+    do {
+      at += u1() - u0;
+      if (at >= end) return false;
+      u0 = 0;
+      if (++tile >= pt_tiles(seq, group)) {
+        tile = 0;
+        if (++head >= kv.kv_heads) {
+          head = 0;
+          do {
+            if (++b >= kv.batch) return false;
+            seq = paged_seq(kv, b);
+          } while (seq.n == 0);
+        }
       }
-    }
-    segment(group);
+      segment(group);
+    } while (j1 == j0);  // a share may end before a tile's first step
     return true;
   }
   __device__ __forceinline__ bool whole() const { return j0 == 0 && j1 == steps; }
+  // Unit of the tile's last step among all.
+  __device__ __forceinline__ int64_t last_unit() const { return at - u0 + PT_TILE_UNITS + steps - 1; }
 };
 
 struct PtShare {  // in shared memory
-  int64_t seq_steps[PT_CHUNK];
-  int64_t total;  // steps of all tiles and key heads
+  int64_t seq_units[PT_CHUNK];
+  int64_t total;  // units of all tiles and key heads
   int64_t lo, hi;
   int ctas;       // CTAs that have a share
-  int b, head, tile, j0;
+  int b, head, tile, u0;
   PtWalk walk[PT_THREADS / 32];  // every warp's walk (registers are for the scores)
 };
 
-// First step of share c of `ctas` over `total` steps, and the share that a step lies in.
+// First unit of share c of `ctas` over `total` units, and the share that a unit lies in.
 __device__ __forceinline__ int64_t pt_share_begin(int64_t total, int ctas, int c) {
   return total * c / ctas;
 }
-__device__ __forceinline__ int pt_share_of(int64_t total, int ctas, int64_t step) {
-  return (int)(((step + 1) * ctas - 1) / total);
+__device__ __forceinline__ int pt_share_of(int64_t total, int ctas, int64_t unit) {
+  return (int)(((unit + 1) * ctas - 1) / total);
 }
 
-// The whole block: adds up the steps of every sequence and finds where this CTA's share
+// The whole block: adds up the units of every sequence and finds where this CTA's share
 // begins. A warp per sequence when they are few, else a thread.
 __device__ __forceinline__ void pt_find_share(const PagedKV& kv, int group, PtShare& sh) {
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -223,26 +236,26 @@ __device__ __forceinline__ void pt_find_share(const PagedKV& kv, int group, PtSh
         const PagedSeq s = paged_seq(kv, base + i);
         const int tiles = pt_tiles(s, group);
         int64_t n = 0;
-        for (int t = lane; t < tiles; t += 32) n += pt_tile_steps(s, group, t);
+        for (int t = lane; t < tiles; t += 32) n += pt_tile_steps(s, group, t) + PT_TILE_UNITS;
 #pragma unroll
         for (int off = 16; off > 0; off >>= 1) n += __shfl_xor_sync(0xffffffffu, n, off);
-        if (lane == 0) sh.seq_steps[i] = n;
+        if (lane == 0) sh.seq_units[i] = n;
       }
     } else {
       for (int i = threadIdx.x; i < count; i += PT_THREADS) {
         const PagedSeq s = paged_seq(kv, base + i);
         const int tiles = pt_tiles(s, group);
         int64_t n = 0;
-        for (int t = 0; t < tiles; ++t) n += pt_tile_steps(s, group, t);
-        sh.seq_steps[i] = n;
+        for (int t = 0; t < tiles; ++t) n += pt_tile_steps(s, group, t) + PT_TILE_UNITS;
+        sh.seq_units[i] = n;
       }
     }
     __syncthreads();
   };
-  // one warp: the sum of the chunk, or the sequence in it that holds step `want`
+  // one warp: the sum of the chunk, or the sequence in it that holds unit `want`
   auto scan_chunk = [&](int count, int64_t before, int64_t want, int64_t& inside) -> int {
     for (int i = 0; i < count; i += 32) {
-      const int64_t n = i + lane < count ? sh.seq_steps[i + lane] : 0;
+      const int64_t n = i + lane < count ? sh.seq_units[i + lane] : 0;
       int64_t incl = n;
 #pragma unroll
       for (int off = 1; off < 32; off <<= 1) {
@@ -257,7 +270,7 @@ __device__ __forceinline__ void pt_find_share(const PagedKV& kv, int group, PtSh
       }
       before += __shfl_sync(0xffffffffu, incl, 31);
     }
-    inside = before;  // not here: the steps so far
+    inside = before;  // not here: the units so far
     return -1;
   };
   int64_t total = 0;
@@ -275,7 +288,7 @@ __device__ __forceinline__ void pt_find_share(const PagedKV& kv, int group, PtSh
   const int64_t lo = c < ctas ? pt_share_begin(all, ctas, c) : all;
   const int64_t hi = c < ctas ? pt_share_begin(all, ctas, c + 1) : all;
   if (lo < hi) {
-    // heads of one sequence lie side by side: step lo lies in the sequence that holds step
+    // heads of one sequence lie side by side: unit lo lies in the sequence that holds unit
     // lo / kv_heads of one head
     const int64_t want = lo / kv.kv_heads;
     int64_t before = 0;
@@ -289,7 +302,7 @@ __device__ __forceinline__ void pt_find_share(const PagedKV& kv, int group, PtSh
       const int i = scan_chunk(count, before, want, inside);
       if (i >= 0) {
         if (warp == 0) {
-          const int64_t one = sh.seq_steps[i];
+          const int64_t one = sh.seq_units[i];
           int64_t r = lo - (want - inside) * kv.kv_heads;  // within the sequence
           const int head = (int)(r / one);
           r -= head * one;
@@ -297,7 +310,7 @@ __device__ __forceinline__ void pt_find_share(const PagedKV& kv, int group, PtSh
           const int tiles = pt_tiles(s, group);
           int64_t run = 0;
           for (int t0 = 0; t0 < tiles; t0 += 32) {
-            const int n = t0 + lane < tiles ? pt_tile_steps(s, group, t0 + lane) : 0;
+            const int n = t0 + lane < tiles ? pt_tile_steps(s, group, t0 + lane) + PT_TILE_UNITS : 0;
             int64_t incl = n;
 #pragma unroll
             for (int off = 1; off < 32; off <<= 1) {
@@ -310,7 +323,7 @@ __device__ __forceinline__ void pt_find_share(const PagedKV& kv, int group, PtSh
                 sh.b = base + i;
                 sh.head = head;
                 sh.tile = t0 + lane;
-                sh.j0 = (int)(r - run - (incl - n));
+                sh.u0 = (int)(r - run - (incl - n));
               }
               break;
             }
@@ -407,10 +420,12 @@ __global__ void __launch_bounds__(PT_THREADS, 1)
     w.b = sh.b;
     w.head = sh.head;
     w.tile = sh.tile;
-    w.j0 = sh.j0;
-    w.left = sh.hi - sh.lo;
+    w.u0 = sh.u0;
+    w.at = sh.lo;
+    w.end = sh.hi;
     w.seq = paged_seq(kv, w.b);
     w.segment(group);
+    if (w.j1 == w.j0) w.next(kv, group);
   }
   __syncwarp();
   auto next_segment = [&]() -> bool {  // the whole warp
@@ -559,7 +574,6 @@ __global__ void __launch_bounds__(PT_THREADS, 1)
     uint32_t gs = 0;       // S taken of this tile
     uint32_t seg = 0;      // segments before this one
     bool ok = true;
-    int64_t at = sh.lo;    // the segment's first step among all
     do {
       const PagedSeq seq = w.seq;
       const int key_first = w.j0 * PT_KEYS;
@@ -571,9 +585,10 @@ __global__ void __launch_bounds__(PT_THREADS, 1)
 
       const int i = f / group;
       const bool valid = i < seq.n;
-      const int lim = valid ? seq.limit(i) : 0;
+      // (rows behind the sequence's last are zero and need no mask: nobody reads their output)
+      const int lim = valid ? seq.limit(i) : 0x7fffffff;
       // every row of the tile sees the slots below this
-      const int lim_all = f_sub + PT_SUB <= seq.n * group ? seq.limit(f_sub / group) : 0;
+      const int lim_all = seq.limit(f_sub / group);
       const int n_s = sub_steps(s);
       float m = -CUDART_INF_F, l = 0.f;
       for (int j = 0; j < n_s; ++j, ++gs) {
@@ -590,11 +605,17 @@ __global__ void __launch_bounds__(PT_THREADS, 1)
         for (int c = 0; c < 4; ++c) tmem_ld_wait_regs(u[c]);
         if (absent || key0 + PT_KEYS > lim_all) {
 #pragma unroll
-          for (int c = 0; c < 4; ++c)
+          for (int c = 0; c < 4; ++c) {
+            // a bit for each key that this row sees
+            const int seen = min(max(lim - key0 - c * 32, 0), 32);
+            uint32_t bits = seen == 32 ? 0xffffffffu : (1u << seen) - 1;
+            if (absent >> (c * 2) & 1u) bits &= 0xffff0000u;
+            if (absent >> (c * 2 + 1) & 1u) bits &= 0x0000ffffu;
+            if (__all_sync(0xffffffffu, bits == 0xffffffffu)) continue;
 #pragma unroll
             for (int e = 0; e < 32; ++e)
-              if (key0 + c * 32 + e >= lim || (absent >> (c * 2 + e / 16) & 1u))
-                u[c][e] = 0xff800000u;  // -inf
+              if (!(bits >> e & 1u)) u[c][e] = 0xff800000u;  // -inf
+          }
         }
         float mx[4];
 #pragma unroll
@@ -694,7 +715,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1)
           po += 32 * PT_ROWS;
         }
         if (w.j0 == 0 && threadIdx.x == 128) {  // begins here, goes on in the next shares
-          const int last = pt_share_of(sh.total, sh.ctas, at + w.steps - 1);
+          const int last = pt_share_of(sh.total, sh.ctas, w.last_unit());
           PtJoin jn;
           jn.count = last - blockIdx.x + 1;
           jn.first = part;
@@ -749,7 +770,6 @@ __global__ void __launch_bounds__(PT_THREADS, 1)
       }
       tc_fence_before();
       g0 += w.j1 - w.j0;
-      at += w.j1 - w.j0;
       ++seg;
     } while (next_segment());
     tc_fence_before();
