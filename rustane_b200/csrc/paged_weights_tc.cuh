@@ -3,29 +3,37 @@
 //
 // The slots are the rows of the product (S^T = K Q^T): a thread owns one slot, reads the
 // scores of all query rows of a step from its own TMEM lane and adds up, so the sum needs no
-// exchange and its order is fixed. A CTA keeps the K of 256 slots of one key head (two tiles
+// exchange and its order is fixed. A CTA keeps the K of 512 slots of one key head (four tiles
 // of 128, one warpgroup each) and walks the query rows in steps of whole tokens, at most 128
-// rows: every Q step that is loaded serves both tiles. 384 threads:
-//   warp 0       TMA producer: K once, then the Q steps (three buffers)
-//   warp 1       TMEM owner; lane 0 issues S^T (128 x 128 x 128) into two buffers per tile
-//   warp 2       copies the steps' log-sum-exps and limits to shared memory
-//   warps 4-11   the sums
+// rows: every Q step that is loaded serves all tiles, and while one tile's scores are made
+// the other warpgroups add up theirs. 640 threads:
+//   warp 0       TMA producer: K once, then the Q steps (two buffers)
+//   warp 1       TMEM owner; issues S^T (128 x 128 x 128), one buffer per tile
+//   warps 2, 3   copy the steps' log-sum-exps and limits to shared memory
+//   warps 4-19   the sums
+// The exponentials are the bound (half of the flops of an attention, as many exponentials):
+// 16 a clock and SM, 4096 cycles per 512 slots and 128 rows against the products' 2048, so a
+// quarter of them goes to the FMA pipes. (Two tiles a CTA with two buffers each left two warps
+// per scheduler and took 1.4 times as long; steps of 64 rows with two CTAs an SM likewise: a
+// step costs a warp some 60 instructions whatever its rows.)
 #pragma once
 #include "paged_attention_tc.cuh"
 
 namespace cb {
 
-constexpr int WT_KEYS = 256;        // slots of a CTA
+constexpr int WT_TILES = 4;
+constexpr int WT_KEYS = WT_TILES * 128;  // slots of a CTA
 constexpr int WT_ROWS = 128;        // query rows of a step, at most
-constexpr int WT_THREADS = 384;
-constexpr int WT_Q_BUFS = 3;
+constexpr int WT_THREADS = 640;
+constexpr int WT_Q_BUFS = 2;
+constexpr int WT_Q_BYTES = WT_ROWS * PG_HD * 2;
 constexpr int WT_L_BUFS = 4;
 constexpr int WT_K_OFF = 0;         // [tile][half of the head][128 slots][128 B]
-constexpr int WT_Q_OFF = 65536;     // [buffer][half][128 rows][128 B]
-constexpr int WT_L_OFF = WT_Q_OFF + WT_Q_BUFS * 32768;  // [buffer]: -lse [128], limit [128]
-constexpr int WT_BAR_OFF = WT_L_OFF + WT_L_BUFS * 1024;
+constexpr int WT_Q_OFF = WT_TILES * 32768;  // [buffer][half][128 rows][128 B]
+constexpr int WT_L_OFF = WT_Q_OFF + WT_Q_BUFS * WT_Q_BYTES;  // [buffer]: -lse [128], limit [128]
+constexpr int WT_BAR_OFF = WT_L_OFF + WT_L_BUFS * WT_ROWS * 8;
 constexpr int WT_SMEM = WT_BAR_OFF + 256 + 1024;
-constexpr uint32_t WT_TMEM_COLS = 512;  // tile A: two buffers of 128 columns, tile B: two
+constexpr uint32_t WT_TMEM_COLS = 512;  // 128 columns per tile
 
 // 3-D tiled TMA load without a cache hint.
 __device__ __forceinline__ void tma_load_3d_plain(void* smem_dst, const CUtensorMap* map,
@@ -52,13 +60,13 @@ __global__ void __launch_bounds__(WT_THREADS, 1)
       (reinterpret_cast<uintptr_t>(wt_smem_raw) + 1023) & ~uintptr_t(1023));
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + WT_BAR_OFF);
   uint64_t* k_full = bars;
-  uint64_t* q_full = bars + 1;    // [3]
-  uint64_t* q_empty = bars + 4;   // [3]
-  uint64_t* l_full = bars + 7;    // [4]
-  uint64_t* l_empty = bars + 11;  // [4]
-  uint64_t* s_full = bars + 15;   // [tile][2]
-  uint64_t* s_empty = bars + 19;  // [tile][2]
-  uint64_t* drain = bars + 23;
+  uint64_t* q_full = bars + 1;    // [2]
+  uint64_t* q_empty = bars + 3;   // [2]
+  uint64_t* l_full = bars + 5;    // [4]
+  uint64_t* l_empty = bars + 9;   // [4]
+  uint64_t* s_full = bars + 13;   // [tile]
+  uint64_t* s_empty = bars + 17;  // [tile]
+  uint64_t* drain = bars + 21;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 24);
   int* failed = reinterpret_cast<int*>(bars + 25);
 
@@ -70,7 +78,7 @@ __global__ void __launch_bounds__(WT_THREADS, 1)
   const int key0 = (rest % blocks) * WT_KEYS;
   const PagedSeq seq = paged_seq(kv, b);
   if (seq.n == 0 || key0 >= seq.limit(seq.n - 1)) return;  // no query sees these slots
-  const int tiles = key0 + 128 < seq.limit(seq.n - 1) ? 2 : 1;
+  const int tiles = min(WT_TILES, (seq.limit(seq.n - 1) - key0 + 127) / 128);
   const int i0 = max(0, key0 - seq.past);  // the first token that sees one of them
   const int steps = (seq.n - i0 + step_tokens - 1) / step_tokens;
   const int step_rows = step_tokens * group;
@@ -120,58 +128,80 @@ __global__ void __launch_bounds__(WT_THREADS, 1)
       for (int j = 0; j < steps; ++j) {
         const int buf = j % WT_Q_BUFS;
         if (!mbar_wait(&q_empty[buf], ((j / WT_Q_BUFS) & 1) ^ 1u, failed)) break;
-        uint8_t* dst = smem + WT_Q_OFF + buf * 32768;
+        uint8_t* dst = smem + WT_Q_OFF + buf * WT_Q_BYTES;
         const int row = seq.row0 + i0 + j * step_tokens;
         mbar_arrive_expect_tx(&q_full[buf], step_rows * 256);
         tma_load_3d_plain(dst, &tmQ, &q_full[buf], 0, head * group, row);
-        tma_load_3d_plain(dst + 16384, &tmQ, &q_full[buf], 64, head * group, row);
+        tma_load_3d_plain(dst + WT_Q_BYTES / 2, &tmQ, &q_full[buf], 64, head * group, row);
       }
     }
   } else if (warp == 1) {
-    if (lane == 0) {
-      // ---------------- matrix instructions
-      constexpr uint32_t idesc = pt_idesc<T>(128, false);
-      const uint32_t k_addr = smem_u32(smem + WT_K_OFF), q_addr = smem_u32(smem + WT_Q_OFF);
-      bool ok = mbar_wait(k_full, 0, failed);
-      for (int j = 0; ok && j < steps; ++j) {
-        const int buf = j % WT_Q_BUFS;
-        if (!(ok = mbar_wait(&q_full[buf], (j / WT_Q_BUFS) & 1, failed))) break;
-        for (int s = 0; ok && s < tiles; ++s) {
-          if (!(ok = mbar_wait(&s_empty[s * 2 + (j & 1)], ((j >> 1) & 1) ^ 1u, failed))) break;
-          tc_fence_after();
+    // ---------------- matrix instructions
+    constexpr uint32_t idesc = pt_idesc<T>(WT_ROWS, false);
+    const uint32_t leader = pt_elect();
+    const uint32_t t0 = __shfl_sync(0xffffffffu, tmem, 0);
+    auto wait = [&](uint64_t* bar, uint32_t parity) -> bool {
+      const bool there = __all_sync(0xffffffffu, mbar_wait(bar, parity, failed));
+      tc_fence_after();
+      return there;
+    };
+    const uint32_t k_desc = pt_desc_k(smem_u32(smem + WT_K_OFF));
+    const uint32_t q_desc = pt_desc_k(smem_u32(smem + WT_Q_OFF));
+    bool ok = wait(k_full, 0);
+    for (int j = 0; ok && j < steps; ++j) {
+      const int buf = j % WT_Q_BUFS;
+      if (!(ok = wait(&q_full[buf], (j / WT_Q_BUFS) & 1))) break;
+      for (int s = 0; ok && s < tiles; ++s) {
+        if (!(ok = wait(&s_empty[s], (j & 1) ^ 1u))) break;
 #pragma unroll
-          for (int k = 0; k < 8; ++k) {
-            const uint32_t off = (uint32_t)((k >> 2) * 16384 + (k & 3) * 32);
-            umma_f16_ss(tmem + s * 256 + (j & 1) * 128, sw128_kmajor_desc(k_addr + s * 32768 + off),
-                        sw128_kmajor_desc(q_addr + buf * 32768 + off), idesc, k != 0);
-          }
-          umma_commit(&s_full[s * 2 + (j & 1)]);
+        for (int k = 0; k < 8; ++k) {
+          const uint32_t k_off = s * (32768 >> 4) + (k >> 2) * (16384 >> 4) + (k & 3) * 2;
+          const uint32_t q_off = buf * (WT_Q_BYTES >> 4) + (k >> 2) * (WT_Q_BYTES >> 5) + (k & 3) * 2;
+          pt_mma_ss(leader, t0 + s * 128, k_desc + k_off, q_desc + q_off, idesc,
+                    k != 0);
         }
-        umma_commit(&q_empty[buf]);
+        pt_commit(leader, &s_full[s]);
       }
-      umma_commit(drain);
-      mbar_wait(drain, 0, failed);
+      pt_commit(leader, &q_empty[buf]);
     }
-  } else if (warp == 2) {
-    // ---------------- log-sum-exps and limits of the steps' rows
-    for (int j = 0; j < steps; ++j) {
-      const int buf = j % WT_L_BUFS;
-      float x[4];
-      int lim[4];
+    pt_commit(leader, drain);
+    mbar_wait(drain, 0, failed);
+  } else if (warp < 4) {
+    // ---------------- log-sum-exps and limits of the steps' rows: a warp takes every other
+    // step and loads its next one before it waits for the buffer (one step after another,
+    // the loads' latency was the kernel's pace: 2.1 us a step)
+    float x[4];
+    int lim[4];
+    auto load = [&](int j) {
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         const int c = lane + 32 * e;
-        const int i = i0 + j * step_tokens + c / group;
+        const int tok = c / group, i = i0 + j * step_tokens + tok;
         const bool valid = c < step_rows && i < seq.n;
-        x[e] = valid ? -__ldg(lse + (int64_t)(seq.row0 + i) * heads + head * group + c % group) : 0.f;
+        x[e] = valid ? -__ldg(lse + (int64_t)(seq.row0 + i) * heads + head * group + c - tok * group)
+                     : 0.f;
         lim[e] = valid ? seq.limit(i) : 0;
       }
-      if (!mbar_wait(&l_empty[buf], ((j / WT_L_BUFS) & 1) ^ 1u, failed)) break;
-      float* dst = reinterpret_cast<float*>(smem + WT_L_OFF + buf * 1024);
+    };
+    if (warp - 2 < steps) load(warp - 2);
+    for (int j = warp - 2; j < steps; j += 2) {
+      const int buf = j % WT_L_BUFS;
+      float y[4];
+      int lm[4];
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        dst[lane + 32 * e] = x[e];
-        reinterpret_cast<int*>(dst)[128 + lane + 32 * e] = lim[e];
+        y[e] = x[e];
+        lm[e] = lim[e];
+      }
+      if (j + 2 < steps) load(j + 2);
+      const bool ok = mbar_wait(&l_empty[buf], ((j / WT_L_BUFS) & 1) ^ 1u, failed);
+      __syncwarp();
+      if (!__all_sync(0xffffffffu, ok)) break;
+      float* dst = reinterpret_cast<float*>(smem + WT_L_OFF + buf * WT_ROWS * 8);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        dst[lane + 32 * e] = y[e];
+        reinterpret_cast<int*>(dst)[WT_ROWS + lane + 32 * e] = lm[e];
       }
       __syncwarp();
       if (lane == 0) mbar_arrive(&l_full[buf]);
@@ -180,7 +210,7 @@ __global__ void __launch_bounds__(WT_THREADS, 1)
     // ---------------- sums: thread = slot
     const int s = (warp - 4) >> 2, quad = warp & 3;
     const int key = key0 + s * 128 + quad * 32 + lane;
-    const uint32_t t_s = tmem + s * 256 + ((uint32_t)(quad * 32) << 16);
+    const uint32_t t_s = tmem + s * 128 + ((uint32_t)(quad * 32) << 16);
     const float2 sc2 = make_float2(scale_log2, scale_log2);
     float2 acc[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
     bool ok = true;
@@ -190,25 +220,24 @@ __global__ void __launch_bounds__(WT_THREADS, 1)
       // whole steps whose rows all see the tile's slots need no masks
       const bool whole = step_rows == WT_ROWS && first + step_tokens <= seq.n &&
                          key0 + s * 128 + 128 <= seq.limit(first);
-      const float4* nl = reinterpret_cast<const float4*>(smem + WT_L_OFF + buf * 1024);
-      const int4* lim = reinterpret_cast<const int4*>(nl + 32);
+      const float4* nl = reinterpret_cast<const float4*>(smem + WT_L_OFF + buf * WT_ROWS * 8);
+      const int4* lim = reinterpret_cast<const int4*>(nl + WT_ROWS / 4);
       if (!mbar_wait(&l_full[buf], (j / WT_L_BUFS) & 1, failed) ||
-          !mbar_wait(&s_full[s * 2 + (j & 1)], (j >> 1) & 1, failed)) { ok = false; break; }
+          !mbar_wait(&s_full[s], j & 1, failed)) { ok = false; break; }
       tc_fence_after();
-      // 32 query rows at a time, the next ones on their way
-      uint32_t u[2][32];
-      tmem_ld_32x32b_x32(t_s + (j & 1) * 128, u[0]);
+      uint32_t u[2][32];  // 32 query rows at a time, the next ones on their way
+      tmem_ld_32x32b_x32(t_s, u[0]);
 #pragma unroll
       for (int c = 0; c < 4; ++c) {
+        const uint32_t(&w)[32] = u[c & 1];
         tmem_ld_wait_regs(u[c & 1]);
         if (c < 3) {
-          tmem_ld_32x32b_x32(t_s + (j & 1) * 128 + (c + 1) * 32, u[(c + 1) & 1]);
+          tmem_ld_32x32b_x32(t_s + (c + 1) * 32, u[(c + 1) & 1]);
         } else {
           tc_fence_before();
           __syncwarp();
-          if (lane == 0) mbar_arrive(&s_empty[s * 2 + (j & 1)]);
+          if (lane == 0) mbar_arrive(&s_empty[s]);
         }
-        const uint32_t(&w)[32] = u[c & 1];
         if (whole) {
 #pragma unroll
           for (int e = 0; e < 32; e += 4) {
@@ -219,8 +248,12 @@ __global__ void __launch_bounds__(WT_THREADS, 1)
                              make_float2(y.z, y.w));
             a.x = exp2_mufu(a.x);
             a.y = exp2_mufu(a.y);
-            d.x = exp2_mufu(d.x);
-            d.y = exp2_mufu(d.y);
+            if (e % 8 == 0) {  // a quarter of the exponentials on the FMA pipes
+              d = exp2_poly2<5>(d);
+            } else {
+              d.x = exp2_mufu(d.x);
+              d.y = exp2_mufu(d.y);
+            }
             acc[0] = fadd2(acc[0], a);
             acc[1] = fadd2(acc[1], d);
           }
