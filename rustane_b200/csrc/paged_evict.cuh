@@ -5,10 +5,11 @@
 // weight's bits made monotone (NaN lowest). Which slots go:
 //   - up to EV_FEW of them (a decode step drops one): the smallest key, of equals the highest
 //     slot, is looked for that many times;
-//   - more: the budget-th largest key is found two bits a pass by counting (at most 16
-//     passes over keys that stay in registers, fewer once a pass hits the budget exactly).
-//     Keys above it stay, of those equal to it the lowest slots. Counting needs no atomics on
-//     a histogram, which would pile up on the few exponents that weights have.
+//   - more: the budget-th largest key is found eleven bits a pass by a histogram in shared
+//     memory (at most 3 passes over keys that stay in registers, fewer once a bin's border
+//     hits the budget exactly). Keys above it stay, of those equal to it the lowest slots.
+//     (Counting against three thresholds a pass needs no atomics but up to 16 passes, each
+//     with a barrier of the cluster: 22 us for 32768 slots on eight CTAs.)
 // Either way the result does not depend on any order of execution. Then the i-th slot below
 // the budget that is not kept (a hole) takes the i-th kept slot behind the budget (a mover).
 // Holes and movers are disjoint ranges of slots, so all rows move at once and in place.
@@ -39,6 +40,7 @@ __device__ __forceinline__ uint32_t evict_key(float w) {
 }
 
 constexpr int EV_FEW = 8;
+constexpr int EV_BINS = 2048;
 
 template <int THREADS, int PER>
 struct EvictShared {
@@ -47,6 +49,9 @@ struct EvictShared {
   uint32_t least[2][2];    // this CTA's smallest key and its highest slot, two buffers
   uint32_t warp_key[WARPS], warp_slot[WARPS];
   int few[EV_FEW];         // the slots that go, when they are few
+  uint32_t hist[2][EV_BINS];         // two passes' histograms in turn
+  uint32_t coarse[2][EV_BINS / 32];  // and their sums over 32 bins
+  uint32_t total[EV_BINS / 32], fine[32];  // sums over the cluster
   uint32_t scan[PER * WARPS];
   uint32_t scan2[PER * WARPS];
   uint32_t warp_sum[32], warp_sum2[32];
@@ -69,11 +74,16 @@ __device__ __forceinline__ void block_scan(uint32_t* v, int n, uint32_t* warp_su
     }
     if (lane == 31) warp_sum[warp] = incl;
     __syncthreads();
-    uint32_t before = run;
-    for (int w = 0; w < THREADS / 32; ++w) {
-      if (w < warp) before += warp_sum[w];
-      run += warp_sum[w];
+    // every warp scans the warps' sums
+    const uint32_t own = lane < THREADS / 32 ? warp_sum[lane] : 0;
+    uint32_t sums = own;
+#pragma unroll
+    for (int off = 1; off < 32; off <<= 1) {
+      const uint32_t up = __shfl_up_sync(0xffffffffu, sums, off);
+      if (lane >= off) sums += up;
     }
+    const uint32_t before = run + __shfl_sync(0xffffffffu, sums - own, warp);
+    run += __shfl_sync(0xffffffffu, sums, 31);
     if (i < n) v[i] = before + incl - x;
     __syncthreads();
   }
@@ -263,37 +273,82 @@ __global__ void __launch_bounds__(THREADS)
   if (t < 3) sm.count[0][t] = 0;
   __syncthreads();
 
-  // ---- the budget-th largest key: the largest T with at least `budget` keys >= T
-  uint32_t T = 0, dummy[3];
-  bool exact = false;  // just `budget` keys >= T
-  const uint32_t want = (uint32_t)a.budget;
-  for (int shift = 30; shift >= 0 && !exact; shift -= 2) {
-    uint32_t c[3] = {0, 0, 0};
-    const uint32_t t1 = T | (1u << shift), t2 = T | (2u << shift), t3 = T | (3u << shift);
+  // ---- the budget-th largest key T: the histogram of the keys within [T, T + 2^(shift + 11))
+  // (all of them at first), the bin that holds it, and on within that bin. Of the other CTAs'
+  // histograms only the sums over 32 bins and then the 32 bins in question are read (all of
+  // them would be 64 KB a CTA and pass: 3 to 20 us over the SMs' network).
+  uint32_t T = 0;
+  uint32_t want = (uint32_t)a.budget;  // that many of the range's largest keys stay
+  bool exact = false;                  // all keys >= T stay
+  // Two entries per lane, from the top down: the one with which their sum reaches `want`.
+  auto reach = [&](uint32_t hi, uint32_t lo, uint32_t& above, uint32_t& inside) -> int {
+    uint32_t incl = hi + lo;
+#pragma unroll
+    for (int off = 1; off < 32; off <<= 1) {
+      const uint32_t up = __shfl_up_sync(0xffffffffu, incl, off);
+      if (lane >= off) incl += up;
+    }
+    const int src = __ffs(__ballot_sync(0xffffffffu, incl >= want)) - 1;
+    const uint32_t before = incl - hi - lo;
+    const bool second = before + hi < want;
+    above = __shfl_sync(0xffffffffu, second ? before + hi : before, src);
+    inside = __shfl_sync(0xffffffffu, second ? lo : hi, src);
+    return 2 * src + (int)__shfl_sync(0xffffffffu, (uint32_t)second, src);
+  };
+  // Sums over the cluster of `count` words at the same place in every CTA, to `out`.
+  auto gather = [&](const uint32_t* words, int count, uint32_t* out) {
+    for (int i = t; i < count * 8; i += THREADS) {
+      const int r = i & 7;
+      uint32_t v = 0;
+      if (ctas == 1)
+        v = r == 0 ? words[i >> 3] : 0u;
+      else if (r < ctas)
+        v = ld_cluster_u32(mapa_shared(smem_u32(words + (i >> 3)), r));
+#pragma unroll
+      for (int off = 1; off < 8; off <<= 1) v += __shfl_xor_sync(0xffffffffu, v, off);
+      if (r == 0) out[i >> 3] = v;
+    }
+    __syncthreads();
+  };
+  int pass = 0;
+  for (int shift = 21;; shift = shift == 21 ? 10 : 0, ++pass) {
+    uint32_t* hist = sm.hist[pass & 1];
+    uint32_t* coarse = sm.coarse[pass & 1];
+    // (a buffer was last read two passes ago, two barriers of the cluster back)
+    for (int i = t; i < EV_BINS; i += THREADS) hist[i] = 0;
+    __syncthreads();
 #pragma unroll
     for (int e = 0; e < PER; ++e) {
-      c[0] += key[e] >= t1;
-      c[1] += key[e] >= t2;
-      c[2] += key[e] >= t3;
+      const uint32_t bin = (key[e] - T) >> shift;
+      // (the last pass's range is 2^10: its bins are the lower half)
+      if (base + e * THREADS + t < n && key[e] >= T && bin < (shift == 0 ? 1024u : EV_BINS))
+        atomicAdd(&hist[bin], 1u);
     }
-    cluster_counts(c, dummy);
-    if (c[2] >= want) {
-      T = t3;
-      exact = c[2] == want;
-    } else if (c[1] >= want) {
-      T = t2;
-      exact = c[1] == want;
-    } else if (c[0] >= want) {
-      T = t1;
-      exact = c[0] == want;
+    __syncthreads();
+    for (int i = warp; i < EV_BINS / 32; i += WARPS) {
+      const uint32_t sum = __reduce_add_sync(0xffffffffu, hist[i * 32 + lane]);
+      if (lane == 0) coarse[i] = sum;
     }
+    cluster_barrier();
+    uint32_t above, inside;
+    gather(coarse, EV_BINS / 32, sm.total);
+    const int big = EV_BINS / 32 - 1 - reach(sm.total[EV_BINS / 32 - 1 - 2 * lane],
+                                             sm.total[EV_BINS / 32 - 2 - 2 * lane], above, inside);
+    want -= above;
+    gather(hist + big * 32, 32, sm.fine);
+    const int bin = big * 32 + 31 - reach(lane < 16 ? sm.fine[31 - 2 * lane] : 0u,
+                                          lane < 16 ? sm.fine[30 - 2 * lane] : 0u, above, inside);
+    want -= above;
+    T += (uint32_t)bin << shift;
+    exact = inside == want;
+    if (exact || shift == 0) break;
   }
 
   uint32_t keep = 0;  // bit e: this thread's element e stays
   if (exact) {
 #pragma unroll
     for (int e = 0; e < PER; ++e)
-      if (key[e] >= T) keep |= 1u << e;
+      if (base + e * THREADS + t < n && key[e] >= T) keep |= 1u << e;
   } else {
     // of the keys equal to T only some stay, the lowest slots: number them
     uint32_t above[3] = {0, 0, 0}, above_before[3];
@@ -306,7 +361,7 @@ __global__ void __launch_bounds__(THREADS)
       if (lane == 0) sm.scan[e * WARPS + warp] = __popc(eq);
     }
     cluster_counts(above, above_before);
-    const uint32_t equals_kept = want - above[0];
+    const uint32_t equals_kept = (uint32_t)a.budget - above[0];
     block_scan<THREADS>(sm.scan, PER * WARPS, sm.warp_sum);
 #pragma unroll
     for (int e = 0; e < PER; ++e) {
