@@ -166,43 +166,46 @@ int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
 // ------------------------------------------------------------------- attention plan
 struct AttentionPlan {
-  bool tc;        // the tcgen05 kernel, else the 16-row one
-  int64_t tiles;  // an upper bound: the device knows how many there are
-  int splits;     // 16-row kernel: parts of a tile, and their keys
-  int keys;
-  size_t parts;   // partial results: rows of 128 (and a log-sum-exp)
-  int ctas;       // tcgen05 kernel
+  bool tc;          // the tcgen05 kernel, else the 16-row one
+  int ctas;         // one per SM, or as many as there can be shares of work
+  size_t workers;   // with a share each
+  size_t rows;      // query rows of a tile: of a part
   size_t bytes() const {
-    if (tc) return parts * (PG_HD + 1) * sizeof(float) + ctas * sizeof(PtJoin);
-    return splits > 1 ? parts * (PG_HD + 1) * sizeof(float) : 0;
+    return workers * (2 * rows * (PG_HD + 1) * sizeof(float) + sizeof(ShareJoin));
   }
 };
 
-// Tiles of m query rows: no more than the rows need with one ragged tile per sequence, and
-// no more than batch x the tiles of the longest.
-int64_t tile_bound(const cb_paged_kv* kv, int group, int m) {
-  return std::min<int64_t>(kv->batch * ceil_div((int64_t)kv->max_new * group, m),
-                           ceil_div((int64_t)kv->rows * group, m) + kv->batch);
-}
-
 AttentionPlan plan_attention(const cb_paged_kv* kv, int32_t heads) {
-  AttentionPlan p = {};
+  AttentionPlan p;
   const int group = heads / kv->kv_heads;
   p.tc = (int64_t)kv->max_new * group > PR_ROWS;
-  p.tiles = tile_bound(kv, group, p.tc ? PT_ROWS : PR_ROWS);
-  const int64_t have = std::max<int64_t>(1, p.tiles * kv->kv_heads);
-  if (p.tc) {  // one CTA per SM, or as many as there can be steps
-    p.ctas = (int)std::min<double>(PG_SMS, (double)have * ceil_div(kv->max_len, PT_KEYS));
-    p.parts = (size_t)p.ctas * 2 * PT_ROWS;
-    return p;
-  }
-  // Two CTAs share an SM; four per SM in all leave the last ones little to wait for.
-  const int64_t splits = std::max<int64_t>(
-      1, std::min<int64_t>(ceil_div(4 * PG_SMS, have), ceil_div(kv->max_len, 256)));
-  p.keys = (int)(ceil_div(ceil_div(kv->max_len, splits), PR_BLOCK) * PR_BLOCK);
-  p.splits = (int)ceil_div(kv->max_len, p.keys);
-  p.parts = (size_t)kv->rows * heads * p.splits;
+  p.rows = p.tc ? PT_ROWS : PR_ROWS;
+  // An upper bound of the tiles (the device knows how many there are): no more than the rows
+  // need with one ragged tile per sequence, and no more than batch x the tiles of the longest.
+  const int64_t tiles = std::min<int64_t>(
+      kv->batch * ceil_div((int64_t)kv->max_new * group, p.rows),
+      ceil_div((int64_t)kv->rows * group, p.rows) + kv->batch);
+  const double steps = (double)tiles * kv->kv_heads * ceil_div(kv->max_len, p.tc ? PT_KEYS : PR_BLOCK);
+  p.ctas = (int)std::max(1.0, std::min<double>(PG_SMS, steps));
+  p.workers = (size_t)p.ctas * (p.tc ? 1 : PR_WARPS);
   return p;
+}
+
+// A kernel that may start before the one in front of it on the stream has ended (it waits for
+// that itself).
+template <typename... Params, typename... Args>
+cudaError_t launch_pdl(void (*kernel)(Params...), dim3 grid, int threads, cudaStream_t st,
+                       Args... args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(threads);
+  cfg.stream = st;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, kernel, Params(args)...);
 }
 
 template <typename T>
@@ -211,37 +214,33 @@ cb_status launch_attention(const cb_paged_kv* kv, const T* q, int64_t q_stride, 
                            cudaStream_t st) {
   const AttentionPlan p = plan_attention(kv, heads);
   const int box = p.tc ? std::min(kv->page_size, PT_KEYS) : PR_BLOCK;
+  const int group = heads / kv->kv_heads;
   CUtensorMap tk, tv;
   if (!make_cache_map(&tk, kv->k, kv, box) || !make_cache_map(&tv, kv->v, kv, box))
     return CB_ERR_UNSUPPORTED;
   const PagedKV d = device_kv(kv);
   const float scale_log2 = scale * 1.4426950408889634f;
-  float* part_lse = workspace ? workspace + p.parts * PG_HD : nullptr;
+  float* part_lse = workspace + p.workers * 2 * p.rows * PG_HD;
+  const ShareParts parts{workspace, part_lse,
+                         reinterpret_cast<ShareJoin*>(part_lse + p.workers * 2 * p.rows)};
   cudaError_t e;
   if (p.tc) {
     static std::atomic<uint64_t> done{0};
     if ((e = allow_smem(paged_tile_kernel<T>, PT_SMEM, done)) != cudaSuccess) return status_of(e);
-    const PtParts parts{workspace, part_lse, reinterpret_cast<PtJoin*>(part_lse + p.parts)};
     paged_tile_kernel<T><<<p.ctas, PT_THREADS, PT_SMEM, st>>>(
         tk, tv, d, q, q_stride, heads, scale_log2, out, out_stride, lse, parts, box);
     if ((e = cudaPeekAtLastError()) != cudaSuccess) return status_of(e);
-    paged_join_kernel<T><<<dim3(p.ctas, PT_ROWS / PJ_ROWS), PJ_WARPS * 32, 0, st>>>(
-        parts, heads, heads / kv->kv_heads, out, out_stride, lse);
-    return status_of(cudaPeekAtLastError());
-  }
-  const int64_t grid = p.tiles * kv->kv_heads * p.splits;
-  if (grid > INT_LIMIT) return CB_ERR_UNSUPPORTED;
-  static std::atomic<uint64_t> done{0};
-  if ((e = allow_smem(paged_rows_kernel<T>, PR_SMEM, done)) != cudaSuccess) return status_of(e);
-  const PagedParts parts{workspace, part_lse, p.splits, p.keys};
-  paged_rows_kernel<T><<<(unsigned)grid, PR_WARPS * 32, PR_SMEM, st>>>(
-      tk, tv, d, q, q_stride, heads, scale_log2, out, out_stride, lse, parts);
-  e = cudaPeekAtLastError();
-  if (e == cudaSuccess && p.splits > 1) {
-    const int64_t blocks = ceil_div((int64_t)kv->rows * heads, PC_WARPS);
-    paged_combine_kernel<T><<<(unsigned)blocks, PC_WARPS * 32, 0, st>>>(d, heads, parts, out,
-                                                                       out_stride, lse);
-    e = cudaPeekAtLastError();
+    e = launch_pdl(paged_join_kernel<T>, dim3(p.ctas, PT_ROWS / PJ_ROWS), PJ_WARPS * 32, st, parts,
+                   heads, group, out, out_stride, lse);
+  } else {
+    static std::atomic<uint64_t> done{0};
+    if ((e = allow_smem(paged_rows_kernel<T>, PR_SMEM, done)) != cudaSuccess) return status_of(e);
+    paged_rows_kernel<T><<<p.ctas, PR_WARPS * 32, PR_SMEM, st>>>(
+        tk, tv, d, q, q_stride, heads, scale_log2, out, out_stride, lse, parts);
+    if ((e = cudaPeekAtLastError()) != cudaSuccess) return status_of(e);
+    const int tile_rows = (int)std::min<int64_t>(PR_ROWS, (int64_t)kv->max_new * group);
+    e = launch_pdl(paged_rows_join_kernel<T>, dim3(p.ctas, tile_rows), PR_WARPS * 32, st, parts,
+                   heads, group, out, out_stride, lse);
   }
   return status_of(e);
 }
@@ -463,15 +462,15 @@ cb_status cb_paged_attention(const cb_paged_kv* kv, const void* q, int64_t q_str
       !array_ok(out, out_stride, width) || !aligned(lse, 4) || !aligned(workspace, 16))
     return CB_ERR_INVALID_ARG;
   const size_t need = plan_attention(kv, heads).bytes();
-  if (need > 0 && (!workspace || workspace_bytes < need)) return CB_ERR_INVALID_ARG;
+  if (!workspace || workspace_bytes < need) return CB_ERR_INVALID_ARG;
   if (kv->rows == 0 || kv->max_new == 0) return CB_OK;
   if (arrays_overlap(q, q_stride, width, out, out_stride, width, kv->rows))
     return CB_ERR_INVALID_ARG;
   const cb_status s = check_device({kv->k, kv->v, kv->table, kv->len, kv->row_start, q, out, lse,
-                                    need > 0 ? workspace : nullptr});
+                                    workspace});
   if (s != CB_OK) return s;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  float* ws = need > 0 ? static_cast<float*>(workspace) : nullptr;
+  float* ws = static_cast<float*>(workspace);
   if (kv->dtype == CB_DTYPE_F16)
     return launch_attention(kv, static_cast<const __half*>(q), q_stride, heads, scale,
                             static_cast<__half*>(out), out_stride, lse, ws, st);

@@ -8,26 +8,35 @@
 //   o_r = sum_k 2^(s_rk - m) v_k / l
 // with the running maximum and sum (32 bits) of an online softmax. K and V are read once per
 // 16 rows, so for a decode step the kernel is bound by the reads of the cache.
+//
+// A warp is a worker of its own (paged_shares.cuh): it takes an equal share of all tiles'
+// blocks of 16 keys through a ring that TMA fills, running ahead over the borders of tiles, and
+// meets no other warp until the join. (A CTA per tile and part of the keys, whose four warps
+// joined in shared memory, left the SMs idle at every CTA's start and end and in the last
+// wave: 4.4 TB/s on few long sequences, 4.6 on many short ones.)
 #pragma once
-#include "paged_common.cuh"
+#include "paged_shares.cuh"
 
 namespace cb {
 
 constexpr int PR_ROWS = 16;    // query rows of a tile
-constexpr int PR_WARPS = 4;
-constexpr int PR_STAGES = 3;   // blocks of 16 keys in flight per warp
+constexpr int PR_WARPS = 8;    // one CTA per SM
+constexpr int PR_STAGES = 3;   // blocks in flight per warp
 constexpr int PR_BLOCK = 16;   // keys of a block
 constexpr int PR_STAGE_BYTES = 2 * PR_BLOCK * PG_HD * 2;  // K and V
 constexpr int PR_RING = PR_WARPS * PR_STAGES * PR_STAGE_BYTES;
-constexpr int PR_SMEM = PR_RING + 256 + 1024;
+// A tile counts two blocks for its Q and its output.
+using PrShares = PagedShares<PR_ROWS, PR_BLOCK, 2, 6>;
 
-// Where the parts of a split row go: part (row * heads + head) * splits + split.
-struct PagedParts {
-  float* o;    // [rows * heads * splits][128] normalised within the part
-  float* lse;  // [rows * heads * splits] base-2 log-sum-exp of the part
-  int splits;
-  int keys;    // keys of a split, a multiple of 16
+struct PrShared {  // behind the ring
+  uint64_t full[PR_WARPS][PR_STAGES];
+  int absent[PR_WARPS][PR_STAGES];  // the block's page is outside the pool
+  int failed;
+  PrShares::Walk use[PR_WARPS], ahead[PR_WARPS];  // of what is computed, and loaded
+  ShareTable table;
 };
+constexpr int PR_SMEM = PR_RING + (int)sizeof(PrShared) + 1024;
+static_assert(PR_SMEM <= 232448, "shared memory");
 
 // Sum over the four lanes of a quad (the columns of an accumulator row).
 __device__ __forceinline__ float quad_sum(float x) {
@@ -39,296 +48,331 @@ __device__ __forceinline__ float quad_max(float x) {
   return fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 2));
 }
 
-// Grid: ((tile * kv_heads) + key head) * splits + split. Each warp takes every fourth block
-// of 16 keys of the CTA's part through a ring of its own, filled by TMA (128-byte swizzle,
-// so the ldmatrix reads of eight rows meet no bank twice); the warps' results are joined in
-// shared memory. With several splits the parts are joined by paged_combine_kernel.
+// Parts: o [2 workers][16 rows][128], lse [2 workers][16]; worker = warp * gridDim + CTA.
 template <typename T>
-__global__ void __launch_bounds__(PR_WARPS * 32, 2)
+__global__ void __launch_bounds__(PR_WARPS * 32, 1)
     paged_rows_kernel(const __grid_constant__ CUtensorMap tmK,
                       const __grid_constant__ CUtensorMap tmV, const PagedKV kv,
                       const T* __restrict__ q, int64_t q_stride, int heads, float scale_log2,
                       T* __restrict__ out, int64_t out_stride, float* __restrict__ lse,
-                      const PagedParts parts) {
+                      const ShareParts parts) {
   using H = Half16<T>;
   extern __shared__ uint8_t pr_smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>(
       (reinterpret_cast<uintptr_t>(pr_smem_raw) + 1023) & ~uintptr_t(1023));
-  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + PR_RING);
-  __shared__ int failed;
-  __shared__ float sm_m[PR_WARPS][PR_ROWS], sm_l[PR_WARPS][PR_ROWS];
-
+  PrShared& sh = *reinterpret_cast<PrShared*>(smem + PR_RING);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int group = heads / kv.kv_heads;
-  const int split = blockIdx.x % parts.splits;
-  const int rest = blockIdx.x / parts.splits;
-  const int head = rest % kv.kv_heads;
-  const PagedTile t = paged_find_tile<PR_ROWS>(kv, group, rest / kv.kv_heads);
-  if (t.b < 0) return;
-  const PagedSeq seq = t.seq;
-  const int f0 = t.tile * PR_ROWS;
-  const int rows = min(PR_ROWS, seq.n * group - f0);
-  const int tile_end = max(0, seq.limit((f0 + rows - 1) / group));  // slots that any row sees
-  const int k0 = split * parts.keys;
-  const int k1 = min(tile_end, k0 + parts.keys);
-  if (split > 0 && k0 >= k1) return;  // a part that the join does not ask for
-
-  if (threadIdx.x == 0) {
-    failed = 0;
-    for (int i = 0; i < PR_WARPS * PR_STAGES; ++i) mbar_init(&bars[i], 1);
+  const int worker = warp * gridDim.x + blockIdx.x;
+  uint8_t* ring = smem + warp * PR_STAGES * PR_STAGE_BYTES;
+  uint64_t* full = sh.full[warp];
+  PrShares::Walk& w = sh.use[warp];
+  PrShares::Walk& ahead = sh.ahead[warp];
+  if (lane == 0) {
+    for (int i = 0; i < PR_STAGES; ++i) mbar_init(&full[i], 1);
+    sh.failed = 0;
     fence_mbar_init();
   }
-  __syncthreads();
+  pdl_launch_dependents();  // (the join; it waits for this kernel's end)
+  const bool some_work = PrShares::begin(kv, group, sh.table, gridDim.x * PR_WARPS, worker, w);
+  if (lane == 0) parts.join[worker].count = 0;  // (set below where a tile goes on)
+  if (!some_work) return;
 
-  const int blocks = (max(0, k1 - k0) + PR_BLOCK - 1) / PR_BLOCK;
-  const int mine = blocks > warp ? (blocks - warp + PR_WARPS - 1) / PR_WARPS : 0;
-  uint8_t* ring = smem + warp * PR_STAGES * PR_STAGE_BYTES;
-  uint64_t* full = bars + warp * PR_STAGES;
-  auto key_of = [&](int i) { return k0 + (warp + i * PR_WARPS) * PR_BLOCK; };
-  auto id_of = [&](int i) { return i < mine ? kv.page_id(t.b, key_of(i)) : -1; };
-  auto load = [&](int i, int id) {
-    if (lane == 0) {
-      const int stage = i % PR_STAGES;
-      // rows behind the matrix read as zero (a page outside the pool)
-      const int row = id >= 0 ? kv.page_row(id, head, key_of(i)) : kv.cache_rows();
-      uint8_t* dst = ring + stage * PR_STAGE_BYTES;
-      mbar_arrive_expect_tx(&full[stage], PR_STAGE_BYTES);
-      tma_load_2d(dst, &tmK, &full[stage], 0, row);
-      tma_load_2d(dst + 2048, &tmK, &full[stage], 64, row);
-      tma_load_2d(dst + 4096, &tmV, &full[stage], 0, row);
-      tma_load_2d(dst + 6144, &tmV, &full[stage], 64, row);
+  // Lane 0 loads: block next_j of `ahead`, whose page's id was asked for one block before.
+  bool more = false;
+  int next_j = 0, next_id = -1;
+  uint32_t loaded = 0;  // blocks
+  auto issue = [&](int id) {
+    const int stage = loaded % PR_STAGES;
+    // rows behind the matrix read as zero (a page outside the pool)
+    const int row = id >= 0 ? kv.page_row(id, ahead.head, next_j * PR_BLOCK) : kv.cache_rows();
+    uint8_t* dst = ring + stage * PR_STAGE_BYTES;
+    sh.absent[warp][stage] = id < 0;
+    mbar_arrive_expect_tx(&full[stage], PR_STAGE_BYTES);
+    tma_load_2d(dst, &tmK, &full[stage], 0, row);
+    tma_load_2d(dst + 2048, &tmK, &full[stage], 64, row);
+    tma_load_2d(dst + 4096, &tmV, &full[stage], 0, row);
+    tma_load_2d(dst + 6144, &tmV, &full[stage], 64, row);
+    ++loaded;
+    if (++next_j == ahead.j1) {
+      more = ahead.next(kv, group);
+      next_j = ahead.j0;
     }
   };
-  // page ids of the next blocks: ids[0] of the block at hand, the last one is loaded one
-  // step before it is needed
-  int ids[PR_STAGES + 1];
+  auto id_of = [&](const PrShares::Walk& x, int j) {
+    return j * PR_BLOCK < x.seq.end ? kv.page_id(x.b, j * PR_BLOCK) : -1;
+  };
+  {
+    // the ring's first blocks: a lane each asks for their ids (of the first segment) at once
+    const int n = w.j1 - w.j0;
+    const int id = lane < min(n, PR_STAGES) ? id_of(w, w.j0 + lane) : -1;
+    if (lane == 0) {
+      ahead = w;
+      more = true;
+      next_j = ahead.j0;
+    }
 #pragma unroll
-  for (int i = 0; i <= PR_STAGES; ++i) ids[i] = id_of(i);
-#pragma unroll
-  for (int i = 0; i < PR_STAGES; ++i)
-    if (i < mine) load(i, ids[i]);
+    for (int i = 0; i < PR_STAGES; ++i) {
+      const int id_i = __shfl_sync(0xffffffffu, id, i);
+      if (lane == 0 && more) issue(i < n ? id_i : id_of(ahead, next_j));
+    }
+    if (more) next_id = id_of(ahead, next_j);
+  }
+  __syncwarp();
 
-  // Q fragments: rows lane / 4 and lane / 4 + 8, elements 2 (lane % 4) (+ 1, + 8, + 9)
   const int r0 = lane >> 2, c2 = (lane & 3) * 2;
-  uint32_t qf[8][4];
-  int lim[2];
-  const T* qp[2];
+  uint32_t g = 0;  // blocks used
+  bool first_segment = true, ok = true, go_on;
+  do {
+    const PagedSeq seq = w.seq;
+    const int head = w.head, f0 = w.tile * PR_ROWS, rows = w.rows(group);
+    const int j0 = w.j0, j1 = w.j1;
+    // Q fragments: rows lane / 4 and lane / 4 + 8, elements 2 (lane % 4) (+ 1, + 8, + 9)
+    uint32_t qf[8][4];
+    int lim[2];
+    int64_t row_of[2];
+    int head_of[2];
 #pragma unroll
-  for (int j = 0; j < 2; ++j) {
-    const int r = r0 + 8 * j;
-    const int f = f0 + min(r, rows - 1);
-    const int i = f / group;
-    lim[j] = r < rows ? seq.limit(i) : 0;
-    qp[j] = q + (int64_t)(seq.row0 + i) * q_stride + (int64_t)(head * group + f - i * group) * PG_HD;
-  }
-#pragma unroll
-  for (int k = 0; k < 8; ++k) {
-#pragma unroll
-    for (int a = 0; a < 4; ++a)
-      qf[k][a] = *reinterpret_cast<const uint32_t*>(qp[a & 1] + k * 16 + c2 + (a >> 1) * 8);
-  }
-  const int lim_min = seq.limit(f0 / group);
-
-  float o[16][4];
-#pragma unroll
-  for (int i = 0; i < 16; ++i)
-#pragma unroll
-    for (int j = 0; j < 4; ++j) o[i][j] = 0.f;
-  float m[2] = {-CUDART_INF_F, -CUDART_INF_F}, l[2] = {0.f, 0.f};
-
-  for (int i = 0; i < mine; ++i) {
-    const int stage = i % PR_STAGES;
-    const int key0 = key_of(i);
-    if (!mbar_wait(&full[stage], (i / PR_STAGES) & 1, &failed)) break;
-    const uint32_t kb = smem_u32(ring + stage * PR_STAGE_BYTES), vb = kb + 4096;
-    float s[2][4] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
-    {
-      const int row = (lane & 7) + ((lane >> 4) << 3);
+    for (int j = 0; j < 2; ++j) {
+      const int r = r0 + 8 * j;
+      const int f = f0 + min(r, rows - 1);
+      const int i = f / group;
+      lim[j] = r < rows ? seq.limit(i) : 0;
+      row_of[j] = seq.row0 + i;
+      head_of[j] = head * group + f - i * group;
+      const T* qp = q + row_of[j] * q_stride + (int64_t)head_of[j] * PG_HD + c2;
 #pragma unroll
       for (int k = 0; k < 8; ++k) {
-        const int chunk = (k & 3) * 2 + ((lane >> 3) & 1);
-        uint32_t kf[4];
-        ldmatrix_x4(kf, kb + (k >> 2) * 2048 + row * 128 + ((chunk ^ (row & 7)) << 4));
-        H::mma(s[0], qf[k], kf[0], kf[1]);
-        H::mma(s[1], qf[k], kf[2], kf[3]);
+        qf[k][j] = *reinterpret_cast<const uint32_t*>(qp + k * 16);
+        qf[k][j + 2] = *reinterpret_cast<const uint32_t*>(qp + k * 16 + 8);
       }
     }
-    const bool all_seen = ids[0] >= 0 && key0 + PR_BLOCK <= lim_min;
-    if (!all_seen) {
+    const int lim_min = seq.limit(f0 / group);
+
+    float o[16][4];
+#pragma unroll
+    for (int i = 0; i < 16; ++i)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) o[i][j] = 0.f;
+    float m[2] = {-CUDART_INF_F, -CUDART_INF_F}, l[2] = {0.f, 0.f};
+
+    for (int jb = j0; jb < j1; ++jb, ++g) {
+      const int stage = g % PR_STAGES;
+      const int key0 = jb * PR_BLOCK;
+      if (ok) ok = mbar_wait(&full[stage], (g / PR_STAGES) & 1, &sh.failed);
+      __syncwarp();
+      const uint32_t kb = smem_u32(ring + stage * PR_STAGE_BYTES), vb = kb + 4096;
+      const bool absent = sh.absent[warp][stage] != 0;
+      float s[2][4] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
+      {
+        const int row = (lane & 7) + ((lane >> 4) << 3);
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+          const int chunk = (k & 3) * 2 + ((lane >> 3) & 1);
+          uint32_t kf[4];
+          ldmatrix_x4(kf, kb + (k >> 2) * 2048 + row * 128 + ((chunk ^ (row & 7)) << 4));
+          H::mma(s[0], qf[k], kf[0], kf[1]);
+          H::mma(s[1], qf[k], kf[2], kf[3]);
+        }
+      }
+      if (absent || key0 + PR_BLOCK > lim_min) {
+#pragma unroll
+        for (int n = 0; n < 2; ++n)
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            if (absent || key0 + n * 8 + c2 + (j & 1) >= lim[j >> 1]) s[n][j] = -CUDART_INF_F;
+      }
+      float base[2], corr[2];
+      bool grew = false;
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        const float mx = quad_max(fmaxf(fmaxf(s[0][2 * j], s[0][2 * j + 1]),
+                                        fmaxf(s[1][2 * j], s[1][2 * j + 1]))) * scale_log2;
+        const float mn = fmaxf(m[j], mx);
+        base[j] = mn == -CUDART_INF_F ? 0.f : mn;
+        grew |= mn > m[j];
+        corr[j] = exp2_mufu(m[j] - base[j]);  // 0 for a row that had seen nothing
+        m[j] = mn;
+      }
+      if (__any_sync(0xffffffffu, grew)) {
+#pragma unroll
+        for (int j = 0; j < 2; ++j) l[j] *= corr[j];
+#pragma unroll
+        for (int n = 0; n < 16; ++n) {
+          o[n][0] *= corr[0];
+          o[n][1] *= corr[0];
+          o[n][2] *= corr[1];
+          o[n][3] *= corr[1];
+        }
+      }
 #pragma unroll
       for (int n = 0; n < 2; ++n)
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
-          if (ids[0] < 0 || key0 + n * 8 + c2 + (j & 1) >= lim[j >> 1]) s[n][j] = -CUDART_INF_F;
-    }
-    float base[2], corr[2];
-    bool grew = false;
-#pragma unroll
-    for (int j = 0; j < 2; ++j) {
-      const float mx = quad_max(fmaxf(fmaxf(s[0][2 * j], s[0][2 * j + 1]),
-                                      fmaxf(s[1][2 * j], s[1][2 * j + 1]))) * scale_log2;
-      const float mn = fmaxf(m[j], mx);
-      base[j] = mn == -CUDART_INF_F ? 0.f : mn;
-      grew |= mn > m[j];
-      corr[j] = exp2_mufu(m[j] - base[j]);  // 0 for a row that had seen nothing
-      m[j] = mn;
-    }
-    if (__any_sync(0xffffffffu, grew)) {
-#pragma unroll
-      for (int j = 0; j < 2; ++j) l[j] *= corr[j];
-#pragma unroll
-      for (int n = 0; n < 16; ++n) {
-        o[n][0] *= corr[0];
-        o[n][1] *= corr[0];
-        o[n][2] *= corr[1];
-        o[n][3] *= corr[1];
-      }
-    }
-#pragma unroll
-    for (int n = 0; n < 2; ++n)
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        s[n][j] = exp2_mufu(fmaf(s[n][j], scale_log2, -base[j >> 1]));
-        l[j >> 1] += s[n][j];
-      }
-    // P rounds to the cache's type (the matrix instruction takes one type for both sides):
-    // at most half a step of each weight, the size of the output's own rounding.
-    const uint32_t pf[4] = {H::pack(s[0][0], s[0][1]), H::pack(s[0][2], s[0][3]),
-                            H::pack(s[1][0], s[1][1]), H::pack(s[1][2], s[1][3])};
-    // slots behind the sequence may hold anything, and 0 x NaN is not 0: their V reads as 0
-    uint32_t v_mask[2] = {0xffffffffu, 0xffffffffu};
-    const bool v_whole = key0 + PR_BLOCK <= seq.end;
-    if (!v_whole) {
-#pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        const int key = key0 + c2 + 8 * j;
-        v_mask[j] = (key < seq.end ? 0xffffu : 0u) | (key + 1 < seq.end ? 0xffff0000u : 0u);
-      }
-    }
-#pragma unroll
-    for (int n = 0; n < 8; ++n) {
-      const int row = lane & 15, chunk = (n & 3) * 2 + (lane >> 4);
-      uint32_t vf[4];
-      ldmatrix_x4_trans(vf, vb + (n >> 2) * 2048 + row * 128 + ((chunk ^ (row & 7)) << 4));
+        for (int j = 0; j < 4; ++j) {
+          s[n][j] = exp2_mufu(fmaf(s[n][j], scale_log2, -base[j >> 1]));
+          l[j >> 1] += s[n][j];
+        }
+      // P rounds to the cache's type (the matrix instruction takes one type for both sides):
+      // at most half a step of each weight, the size of the output's own rounding.
+      const uint32_t pf[4] = {H::pack(s[0][0], s[0][1]), H::pack(s[0][2], s[0][3]),
+                              H::pack(s[1][0], s[1][1]), H::pack(s[1][2], s[1][3])};
+      // slots behind the sequence may hold anything, and 0 x NaN is not 0: their V reads as 0
+      uint32_t v_mask[2] = {0xffffffffu, 0xffffffffu};
+      const bool v_whole = key0 + PR_BLOCK <= seq.end;
       if (!v_whole) {
 #pragma unroll
-        for (int j = 0; j < 4; ++j) vf[j] &= v_mask[j & 1];
+        for (int j = 0; j < 2; ++j) {
+          const int key = key0 + c2 + 8 * j;
+          v_mask[j] = (key < seq.end ? 0xffffu : 0u) | (key + 1 < seq.end ? 0xffff0000u : 0u);
+        }
       }
-      H::mma(o[2 * n], pf, vf[0], vf[1]);
-      H::mma(o[2 * n + 1], pf, vf[2], vf[3]);
+#pragma unroll
+      for (int n = 0; n < 8; ++n) {
+        const int row = lane & 15, chunk = (n & 3) * 2 + (lane >> 4);
+        uint32_t vf[4];
+        ldmatrix_x4_trans(vf, vb + (n >> 2) * 2048 + row * 128 + ((chunk ^ (row & 7)) << 4));
+        if (!v_whole) {
+#pragma unroll
+          for (int j = 0; j < 4; ++j) vf[j] &= v_mask[j & 1];
+        }
+        H::mma(o[2 * n], pf, vf[0], vf[1]);
+        H::mma(o[2 * n + 1], pf, vf[2], vf[3]);
+      }
+      __syncwarp();  // every lane has read the stage
+      if (lane == 0 && more) {
+        issue(next_id);
+        if (more) next_id = id_of(ahead, next_j);
+      }
     }
-    __syncwarp();  // every lane has read the stage
-    if (i + PR_STAGES < mine) load(i + PR_STAGES, ids[PR_STAGES]);
+    // ---- the segment's output
+    const bool whole = w.whole();
+    const int part = 2 * worker + (first_segment ? 0 : 1);
+    if (lane == 0 && !whole && j0 == 0)  // begins here, goes on in the next shares
+      parts.join[worker] = w.join(sh.table, worker, part, group);
 #pragma unroll
-    for (int j = 0; j < PR_STAGES; ++j) ids[j] = ids[j + 1];
-    ids[PR_STAGES] = id_of(i + PR_STAGES + 1);
-  }
+    for (int j = 0; j < 2; ++j) {
+      l[j] = quad_sum(l[j]);
+      const int r = r0 + 8 * j;
+      const float inv = l[j] == 0.f ? 0.f : 1.0f / l[j];  // a row that sees nothing: 0
+      const float row_lse = l[j] == 0.f ? -CUDART_INF_F : m[j] + log2f(l[j]);
+      if (r < rows && ok) {
+        if (whole) {
+          T* po = out + row_of[j] * out_stride + (int64_t)head_of[j] * PG_HD + c2;
 #pragma unroll
-  for (int j = 0; j < 2; ++j) l[j] = quad_sum(l[j]);
-
-  // ---- join the warps: [warp][row][128] over the ring (whose last load has arrived)
-  __syncthreads();
-  float* sm_o = reinterpret_cast<float*>(smem);
+          for (int n = 0; n < 16; ++n)
+            *reinterpret_cast<uint32_t*>(po + n * 8) =
+                H::pack(o[n][2 * j] * inv, o[n][2 * j + 1] * inv);
+          if (lse && c2 == 0) lse[row_of[j] * heads + head_of[j]] = row_lse;
+        } else {
+          float* po = parts.o + ((int64_t)part * PR_ROWS + r) * PG_HD + c2;
 #pragma unroll
-  for (int j = 0; j < 2; ++j) {
-    const int r = r0 + 8 * j;
-    if ((lane & 3) == 0) {
-      sm_m[warp][r] = m[j];
-      sm_l[warp][r] = l[j];
+          for (int n = 0; n < 16; ++n)
+            *reinterpret_cast<float2*>(po + n * 8) =
+                make_float2(o[n][2 * j] * inv, o[n][2 * j + 1] * inv);
+          if (c2 == 0) parts.lse[part * PR_ROWS + r] = row_lse;
+        }
+      }
     }
-#pragma unroll
-    for (int n = 0; n < 16; ++n)
-      *reinterpret_cast<float2*>(sm_o + (warp * PR_ROWS + r) * PG_HD + n * 8 + c2) =
-          make_float2(o[n][2 * j], o[n][2 * j + 1]);
-  }
-  __syncthreads();
-  const int d = threadIdx.x;  // one thread per element
-  for (int r = 0; r < rows; ++r) {
-    float mx = sm_m[0][r];
-#pragma unroll
-    for (int w = 1; w < PR_WARPS; ++w) mx = fmaxf(mx, sm_m[w][r]);
-    const float base = mx == -CUDART_INF_F ? 0.f : mx;
-    float sum = 0.f, acc = 0.f;
-#pragma unroll
-    for (int w = 0; w < PR_WARPS; ++w) {
-      const float c = exp2_mufu(sm_m[w][r] - base);
-      sum = fmaf(c, sm_l[w][r], sum);
-      acc = fmaf(c, sm_o[(w * PR_ROWS + r) * PG_HD + d], acc);
-    }
-    const float res = sum == 0.f ? 0.f : acc / sum;  // a row that sees nothing: 0
-    const float row_lse = sum == 0.f ? -CUDART_INF_F : mx + log2f(sum);
-    const int f = f0 + r, i = f / group;
-    const int64_t at = (int64_t)(seq.row0 + i);
-    const int h = head * group + f - i * group;
-    if (parts.splits == 1) {
-      out[at * out_stride + (int64_t)h * PG_HD + d] = H::from(res);
-      if (lse && d == 0) lse[at * heads + h] = row_lse;
-    } else {
-      const int64_t p = (at * heads + h) * parts.splits + split;
-      parts.o[p * PG_HD + d] = res;
-      if (d == 0) parts.lse[p] = row_lse;
-    }
-  }
+    first_segment = false;
+    __syncwarp();
+    go_on = false;
+    if (lane == 0) go_on = w.next(kv, group);
+    go_on = __any_sync(0xffffffffu, go_on);
+  } while (go_on);
 }
 
-// Joins the parts of every row: out = sum_s 2^(lse_s - lse) o_s, lse = log2 sum_s 2^lse_s.
-// One warp per (row, head). A tile has as many parts as its last row's slots need.
-constexpr int PC_WARPS = 4;
+// Joins the parts of the tiles that begin in a worker's share and go on behind it:
+// out = sum_p 2^(lse_p - lse) o_p, lse = log2 sum_p 2^lse_p. Block (x, y) looks after workers
+// k * gridDim.x + x, k < 8, and the rows y, y + gridDim.y, ...: warp k after worker k's tile
+// where the parts are few, all warps after one where they are many.
 template <typename T>
-__global__ void __launch_bounds__(PC_WARPS * 32)
-    paged_combine_kernel(const PagedKV kv, int heads, const PagedParts parts,
-                         T* __restrict__ out, int64_t out_stride, float* __restrict__ lse) {
+__global__ void __launch_bounds__(PR_WARPS * 32)
+    paged_rows_join_kernel(const ShareParts parts, int heads, int group, T* __restrict__ out,
+                           int64_t out_stride, float* __restrict__ lse) {
   using H = Half16<T>;
-  const int lane = threadIdx.x & 31;
-  const int64_t w = (int64_t)blockIdx.x * PC_WARPS + (threadIdx.x >> 5);
-  if (w >= (int64_t)kv.rows * heads) return;
-  const int r = (int)(w / heads), h = (int)(w - (int64_t)r * heads);
-  int started = 0;
-  for (int base = 0; base <= kv.batch; base += 32) {
-    const bool before = base + lane <= kv.batch && __ldg(kv.row_start + base + lane) <= r;
-    started += __popc(__ballot_sync(0xffffffffu, before));
-  }
-  const int b = started - 1;
-  if (b < 0 || b >= kv.batch) return;  // padding
-  const PagedSeq seq = paged_seq(kv, b);
-  const int i = r - seq.row0;
-  if (i < 0 || i >= seq.n) return;
-  const int group = heads / kv.kv_heads;
-  const int f = i * group + h % group;
-  const int last = min((f / PR_ROWS + 1) * PR_ROWS, seq.n * group) - 1;
-  const int tile_end = max(0, seq.limit(last / group));
-  const int n = min(parts.splits, max(1, (tile_end + parts.keys - 1) / parts.keys));
-
-  const float* pl = parts.lse + w * parts.splits;
-  const float* po = parts.o + w * parts.splits * PG_HD + lane * 4;
-  float mx = -CUDART_INF_F;
-  for (int s = lane; s < n; s += 32) mx = fmaxf(mx, pl[s]);
+  constexpr int FEW = 8;
+  __shared__ float sm_m[PR_WARPS], sm_l[PR_WARPS];
+  __shared__ float4 sm_o[PR_WARPS][32];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  pdl_wait();
+  // parts p0, p0 + step, ... of a row
+  auto merge = [&](const ShareJoin& jn, int worker, int r, int p0, int step, float& m, float& l,
+                   float4& o) {
+    m = -CUDART_INF_F;
+    for (int p = p0 + lane * step; p < jn.count; p += 32 * step)
+      m = fmaxf(m, parts.lse[share_part(jn, worker, p) * PR_ROWS + r]);
 #pragma unroll
-  for (int off = 16; off > 0; off >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, off));
-  const float base = mx == -CUDART_INF_F ? 0.f : mx;
-  float sum = 0.f;
-  float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-  for (int s0 = 0; s0 < n; s0 += 32) {
-    // max and sum both skip NaN of a maximum; a NaN part makes its weight and the row NaN
-    const float mine = s0 + lane < n ? exp2_mufu(pl[s0 + lane] - base) : 0.f;
-    const int m = min(32, n - s0);
-#pragma unroll 4
-    for (int s = 0; s < m; ++s) {
-      const float c = __shfl_sync(0xffffffffu, mine, s);
-      const float4 x = *reinterpret_cast<const float4*>(po + (int64_t)(s0 + s) * PG_HD);
-      sum += c;
-      acc.x = fmaf(c, x.x, acc.x);
-      acc.y = fmaf(c, x.y, acc.y);
-      acc.z = fmaf(c, x.z, acc.z);
-      acc.w = fmaf(c, x.w, acc.w);
+    for (int off = 16; off > 0; off >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, off));
+    const float base = m == -CUDART_INF_F ? 0.f : m;
+    l = 0.f;
+    o = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 8
+    for (int p = p0; p < jn.count; p += step) {
+      const int64_t at = (int64_t)share_part(jn, worker, p) * PR_ROWS + r;
+      const float c = exp2_mufu(parts.lse[at] - base);
+      const float4 x = *reinterpret_cast<const float4*>(parts.o + at * PG_HD + lane * 4);
+      l += c;
+      o.x = fmaf(c, x.x, o.x);
+      o.y = fmaf(c, x.y, o.y);
+      o.z = fmaf(c, x.z, o.z);
+      o.w = fmaf(c, x.w, o.w);
+    }
+  };
+  auto write = [&](const ShareJoin& jn, int r, float m, float l, const float4& o) {
+    const float inv = l == 0.f ? 0.f : 1.0f / l;
+    const int f = jn.f0 + r, i = f / group, h = jn.head * group + f - i * group;
+    const int64_t row = (int64_t)jn.row0 + i;
+    uint2 y;
+    y.x = H::pack(o.x * inv, o.y * inv);
+    y.y = H::pack(o.z * inv, o.w * inv);
+    *reinterpret_cast<uint2*>(out + row * out_stride + (int64_t)h * PG_HD + lane * 4) = y;
+    if (lse && lane == 0) lse[row * heads + h] = l == 0.f ? -CUDART_INF_F : m + log2f(l);
+  };
+  float m, l;
+  float4 o;
+  const int counts = lane < PR_WARPS ? parts.join[lane * gridDim.x + blockIdx.x].count : 0;
+  const int mine = __shfl_sync(0xffffffffu, counts, warp);
+  if (mine > 0 && mine <= FEW) {
+    const int worker = warp * gridDim.x + blockIdx.x;
+    const ShareJoin jn = parts.join[worker];
+    for (int r = blockIdx.y; r < jn.rows; r += gridDim.y) {
+      merge(jn, worker, r, 0, 1, m, l, o);
+      write(jn, r, m, l, o);
     }
   }
-  const float inv = sum == 0.f ? 0.f : 1.0f / sum;
-  uint2 w2;
-  w2.x = H::pack(acc.x * inv, acc.y * inv);
-  w2.y = H::pack(acc.z * inv, acc.w * inv);
-  *reinterpret_cast<uint2*>(out + (int64_t)r * out_stride + (int64_t)h * PG_HD + lane * 4) = w2;
-  if (lse && lane == 0) lse[w] = sum == 0.f ? -CUDART_INF_F : mx + log2f(sum);
+  for (unsigned many = __ballot_sync(0xffffffffu, counts > FEW); many; many &= many - 1) {
+    const int worker = (__ffs(many) - 1) * gridDim.x + blockIdx.x;
+    const ShareJoin jn = parts.join[worker];
+    for (int r = blockIdx.y; r < jn.rows; r += gridDim.y) {
+      merge(jn, worker, r, warp, PR_WARPS, m, l, o);
+      if (lane == 0) {
+        sm_m[warp] = m;
+        sm_l[warp] = l;
+      }
+      sm_o[warp][lane] = o;
+      __syncthreads();
+      if (warp == 0) {
+        m = sm_m[0];
+#pragma unroll
+        for (int k = 1; k < PR_WARPS; ++k) m = fmaxf(m, sm_m[k]);
+        const float base = m == -CUDART_INF_F ? 0.f : m;
+        l = 0.f;
+        o = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+        for (int k = 0; k < PR_WARPS; ++k) {
+          const float c = exp2_mufu(sm_m[k] - base);
+          const float4 x = sm_o[k][lane];
+          l = fmaf(c, sm_l[k], l);
+          o.x = fmaf(c, x.x, o.x);
+          o.y = fmaf(c, x.y, o.y);
+          o.z = fmaf(c, x.z, o.z);
+          o.w = fmaf(c, x.w, o.w);
+        }
+        write(jn, r, m, l, o);
+      }
+      __syncthreads();
+    }
+  }
 }
 
 // ------------------------------------------------------------------ attention weights

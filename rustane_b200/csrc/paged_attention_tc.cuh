@@ -21,14 +21,10 @@
 // two threads per row, hide the products' latency as well, but a step costs a warp about 60
 // instructions whatever its keys: both took 2.3 us for 128 keys.
 //
-// Sequences of a step differ in length and the number of tiles is rarely a multiple of the
-// SMs, so the steps of all tiles (sequence, key head, tile in this order: neighbours share
-// K and V in L2), and a unit or two for each tile's own cost, are laid end to end and every
-// CTA takes an equal share of them. A CTA that
-// has all steps of a tile writes its output; of a tile that is cut, each CTA writes its part
-// (at most two per CTA: its first and its last tile) and paged_join_kernel joins them.
+// The work is handed out in equal shares (paged_shares.cuh), a share to a CTA; paged_join_kernel
+// joins the tiles that are cut.
 #pragma once
-#include "paged_attention.cuh"
+#include "paged_shares.cuh"
 
 namespace cb {
 
@@ -43,7 +39,7 @@ constexpr int PT_K_OFF = 65536;        // [buffer][half][128 keys][128 B]
 constexpr int PT_V_OFF = PT_K_OFF + PT_BUFS * PT_STEP_BYTES;
 constexpr int PT_BAR_OFF = PT_V_OFF + PT_BUFS * PT_STEP_BYTES;
 constexpr int PT_SHARE_OFF = PT_BAR_OFF + 256;
-constexpr int PT_SMEM = PT_SHARE_OFF + 8192 + 64 + PT_THREADS / 32 * 80 + 1024;
+constexpr int PT_SMEM = PT_SHARE_OFF + SHARE_CHUNK * 8 + 64 + PT_THREADS / 32 * 80 + 1024;
 constexpr uint32_t PT_TMEM_COLS = 512;  // S_A, S_B, O_A, O_B: 128 columns each
 constexpr float PT_RESCALE = 8.0f;
 
@@ -151,225 +147,30 @@ __device__ __forceinline__ int pt_step_id(const PagedKV& kv, int b, int key0, in
   return (lane >> 1) * box_rows < KEYS && key < end ? kv.page_id(b, key) : -1;
 }
 
-// ------------------------------------------------------------------- the shares
-constexpr int PT_CHUNK = 1024;  // sequences whose units are added up at a time
-// A tile counts its steps and this many units for its Q, its pipeline's start and its output
-// (a step takes 1.9 us, a tile 4 to 5 us beside its steps).
-constexpr int PT_TILE_UNITS = 2;
-constexpr int PT_LEAST = 4;     // units of a share; above PT_TILE_UNITS, so each has a step
+// A tile counts two steps for its Q, its pipeline's start and its output (a step takes
+// 1.9 us, a tile 4 to 5 us beside its steps).
+using PtShares = PagedShares<PT_ROWS, PT_KEYS, 2, 4>;
 
-// Steps of tile `tile` of a sequence: up to the last slot that its last row sees. A tile that
-// sees nothing has one step too (in which everything is masked): it writes its zeros.
-__device__ __forceinline__ int pt_tile_steps(const PagedSeq& seq, int group, int tile) {
-  const int last = min((tile + 1) * PT_ROWS, seq.n * group) - 1;
-  return max(1, (seq.limit(last / group) + PT_KEYS - 1) / PT_KEYS);
-}
-__device__ __forceinline__ int pt_tiles(const PagedSeq& seq, int group) {
-  return (seq.n * group + PT_ROWS - 1) / PT_ROWS;
-}
-
-// A CTA's walk over its share: segments of tiles.
-struct PtWalk {
-  PagedSeq seq;
-  int b, head, tile;
-  int u0;             // the segment's first unit within the tile
-  int j0, j1, steps;  // the segment: steps j0 .. j1 - 1 of the tile's `steps`
-  int64_t at, end;    // the segment's first unit among all, and the share's end
-
-  __device__ __forceinline__ int u1() const {
-    return (int)min((int64_t)(steps + PT_TILE_UNITS), u0 + (end - at));
-  }
-  __device__ __forceinline__ void segment(int group) {
-    steps = pt_tile_steps(seq, group, tile);
-    j0 = max(0, u0 - PT_TILE_UNITS);
-    j1 = max(0, u1() - PT_TILE_UNITS);
-  }
-  // The next segment; false when the share is done.
-  __device__ __forceinline__ bool next(const PagedKV& kv, int group) {
-    do {
-      at += u1() - u0;
-      if (at >= end) return false;
-      u0 = 0;
-      if (++tile >= pt_tiles(seq, group)) {
-        tile = 0;
-        if (++head >= kv.kv_heads) {
-          head = 0;
-          do {
-            if (++b >= kv.batch) return false;
-            seq = paged_seq(kv, b);
-          } while (seq.n == 0);
-        }
-      }
-      segment(group);
-    } while (j1 == j0);  // a share may end before a tile's first step
-    return true;
-  }
-  __device__ __forceinline__ bool whole() const { return j0 == 0 && j1 == steps; }
-  // Unit of the tile's last step among all.
-  __device__ __forceinline__ int64_t last_unit() const { return at - u0 + PT_TILE_UNITS + steps - 1; }
+struct PtShared {  // at PT_SHARE_OFF
+  PtShares::Walk walk[PT_THREADS / 32];  // every warp's (registers are for the scores)
+  ShareTable table;
 };
+static_assert(sizeof(PtShared) <= PT_SMEM - 1024 - PT_SHARE_OFF, "shared memory");
 
-struct PtShare {  // in shared memory
-  int64_t seq_units[PT_CHUNK];
-  int64_t total;  // units of all tiles and key heads
-  int64_t lo, hi;
-  int ctas;       // CTAs that have a share
-  int b, head, tile, u0;
-  PtWalk walk[PT_THREADS / 32];  // every warp's walk (registers are for the scores)
-};
-
-// First unit of share c of `ctas` over `total` units, and the share that a unit lies in.
-__device__ __forceinline__ int64_t pt_share_begin(int64_t total, int ctas, int c) {
-  return total * c / ctas;
-}
-__device__ __forceinline__ int pt_share_of(int64_t total, int ctas, int64_t unit) {
-  return (int)(((unit + 1) * ctas - 1) / total);
-}
-
-// The whole block: adds up the units of every sequence and finds where this CTA's share
-// begins. A warp per sequence when they are few, else a thread.
-__device__ __forceinline__ void pt_find_share(const PagedKV& kv, int group, PtShare& sh) {
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  auto sum_chunk = [&](int base, int count) {
-    if (count <= 96) {
-      for (int i = warp; i < count; i += PT_THREADS / 32) {
-        const PagedSeq s = paged_seq(kv, base + i);
-        const int tiles = pt_tiles(s, group);
-        int64_t n = 0;
-        for (int t = lane; t < tiles; t += 32) n += pt_tile_steps(s, group, t) + PT_TILE_UNITS;
-#pragma unroll
-        for (int off = 16; off > 0; off >>= 1) n += __shfl_xor_sync(0xffffffffu, n, off);
-        if (lane == 0) sh.seq_units[i] = n;
-      }
-    } else {
-      for (int i = threadIdx.x; i < count; i += PT_THREADS) {
-        const PagedSeq s = paged_seq(kv, base + i);
-        const int tiles = pt_tiles(s, group);
-        int64_t n = 0;
-        for (int t = 0; t < tiles; ++t) n += pt_tile_steps(s, group, t) + PT_TILE_UNITS;
-        sh.seq_units[i] = n;
-      }
-    }
-    __syncthreads();
-  };
-  // one warp: the sum of the chunk, or the sequence in it that holds unit `want`
-  auto scan_chunk = [&](int count, int64_t before, int64_t want, int64_t& inside) -> int {
-    for (int i = 0; i < count; i += 32) {
-      const int64_t n = i + lane < count ? sh.seq_units[i + lane] : 0;
-      int64_t incl = n;
-#pragma unroll
-      for (int off = 1; off < 32; off <<= 1) {
-        const int64_t up = __shfl_up_sync(0xffffffffu, incl, off);
-        if (lane >= off) incl += up;
-      }
-      const unsigned past = __ballot_sync(0xffffffffu, before + incl > want);
-      if (past) {
-        const int src = __ffs(past) - 1;
-        inside = want - before - __shfl_sync(0xffffffffu, incl - n, src);
-        return i + src;
-      }
-      before += __shfl_sync(0xffffffffu, incl, 31);
-    }
-    inside = before;  // not here: the units so far
-    return -1;
-  };
-  int64_t total = 0;
-  for (int base = 0; base < kv.batch; base += PT_CHUNK) {
-    const int count = min(PT_CHUNK, kv.batch - base);
-    __syncthreads();
-    sum_chunk(base, count);
-    int64_t inside;
-    scan_chunk(count, total, INT64_MAX, inside);  // every warp, the same sum
-    total = inside;
-  }
-  const int64_t all = total * kv.kv_heads;
-  const int ctas = (int)max((int64_t)1, min((int64_t)gridDim.x, all / PT_LEAST));
-  const int c = blockIdx.x;
-  const int64_t lo = c < ctas ? pt_share_begin(all, ctas, c) : all;
-  const int64_t hi = c < ctas ? pt_share_begin(all, ctas, c + 1) : all;
-  if (lo < hi) {
-    // heads of one sequence lie side by side: unit lo lies in the sequence that holds unit
-    // lo / kv_heads of one head
-    const int64_t want = lo / kv.kv_heads;
-    int64_t before = 0;
-    for (int base = 0; base < kv.batch; base += PT_CHUNK) {
-      const int count = min(PT_CHUNK, kv.batch - base);
-      if (kv.batch > PT_CHUNK) {
-        __syncthreads();
-        sum_chunk(base, count);
-      }
-      int64_t inside;
-      const int i = scan_chunk(count, before, want, inside);
-      if (i >= 0) {
-        if (warp == 0) {
-          const int64_t one = sh.seq_units[i];
-          int64_t r = lo - (want - inside) * kv.kv_heads;  // within the sequence
-          const int head = (int)(r / one);
-          r -= head * one;
-          const PagedSeq s = paged_seq(kv, base + i);
-          const int tiles = pt_tiles(s, group);
-          int64_t run = 0;
-          for (int t0 = 0; t0 < tiles; t0 += 32) {
-            const int n = t0 + lane < tiles ? pt_tile_steps(s, group, t0 + lane) + PT_TILE_UNITS : 0;
-            int64_t incl = n;
-#pragma unroll
-            for (int off = 1; off < 32; off <<= 1) {
-              const int64_t up = __shfl_up_sync(0xffffffffu, incl, off);
-              if (lane >= off) incl += up;
-            }
-            const unsigned past = __ballot_sync(0xffffffffu, run + incl > r);
-            if (past) {
-              if (lane == __ffs(past) - 1) {
-                sh.b = base + i;
-                sh.head = head;
-                sh.tile = t0 + lane;
-                sh.u0 = (int)(r - run - (incl - n));
-              }
-              break;
-            }
-            run += __shfl_sync(0xffffffffu, incl, 31);
-          }
-        }
-        break;
-      }
-      before = inside;
-    }
-  }
-  if (threadIdx.x == 0) {
-    sh.total = all;
-    sh.lo = lo;
-    sh.hi = hi;
-    sh.ctas = ctas;
-  }
-  __syncthreads();
-}
-
-// The parts of cut tiles, and what is to be joined. Part 2 c is CTA c's first segment, part
-// 2 c + 1 its last one.
-struct PtJoin {  // one per CTA: the tile that begins in its share and goes on behind it
-  int count;  // parts, 0 = no such tile
-  int first;  // part of this CTA; the others are 2 (c + 1), 2 (c + 2), ...
-  int row0, head, f0, rows;
-};
-struct PtParts {
-  float* o;    // [2 gridDim][128][256 rows] normalised within the part
-  float* lse;  // [2 gridDim][256]
-  PtJoin* join;
-};
-
+// Parts: o [2 gridDim][128][256 rows], lse [2 gridDim][256].
 template <typename T>
 __global__ void __launch_bounds__(PT_THREADS, 1)
     paged_tile_kernel(const __grid_constant__ CUtensorMap tmK,
                       const __grid_constant__ CUtensorMap tmV, const PagedKV kv,
                       const T* __restrict__ q, int64_t q_stride, int heads, float scale_log2,
                       T* __restrict__ out, int64_t out_stride, float* __restrict__ lse,
-                      const PtParts parts, int box_rows) {
+                      const ShareParts parts, int box_rows) {
   using H = Half16<T>;
   extern __shared__ uint8_t pt_smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>(
       (reinterpret_cast<uintptr_t>(pt_smem_raw) + 1023) & ~uintptr_t(1023));
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + PT_BAR_OFF);
-  PtShare& sh = *reinterpret_cast<PtShare*>(smem + PT_SHARE_OFF);
+  PtShared& sh = *reinterpret_cast<PtShared*>(smem + PT_SHARE_OFF);
   uint64_t* k_full = bars;        // [2]
   uint64_t* k_empty = bars + 2;   // [2]
   uint64_t* v_full = bars + 4;    // [2]
@@ -403,9 +204,11 @@ __global__ void __launch_bounds__(PT_THREADS, 1)
     tma_prefetch_desc(&tmK);
     tma_prefetch_desc(&tmV);
   }
-  pt_find_share(kv, group, sh);
+  PtShares::Walk& w = sh.walk[warp];
+  pdl_launch_dependents();  // (the join; it waits for this kernel's end)
+  const bool some_work = PtShares::begin(kv, group, sh.table, gridDim.x, blockIdx.x, w);
   if (threadIdx.x == 0) parts.join[blockIdx.x].count = 0;  // (set below where a tile goes on)
-  if (sh.lo >= sh.hi) return;
+  if (!some_work) return;
   if (warp == 1) {
     tmem_alloc(tmem_slot, PT_TMEM_COLS);
     tmem_relinquish();
@@ -415,19 +218,6 @@ __global__ void __launch_bounds__(PT_THREADS, 1)
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
 
-  PtWalk& w = sh.walk[warp];
-  if (lane == 0) {
-    w.b = sh.b;
-    w.head = sh.head;
-    w.tile = sh.tile;
-    w.u0 = sh.u0;
-    w.at = sh.lo;
-    w.end = sh.hi;
-    w.seq = paged_seq(kv, w.b);
-    w.segment(group);
-    if (w.j1 == w.j0) w.next(kv, group);
-  }
-  __syncwarp();
   auto next_segment = [&]() -> bool {  // the whole warp
     __syncwarp();
     bool more = false;
@@ -714,17 +504,8 @@ __global__ void __launch_bounds__(PT_THREADS, 1)
             po[e * PT_ROWS] = some ? __uint_as_float(o[e]) * inv : 0.f;
           po += 32 * PT_ROWS;
         }
-        if (w.j0 == 0 && threadIdx.x == 128) {  // begins here, goes on in the next shares
-          const int last = pt_share_of(sh.total, sh.ctas, w.last_unit());
-          PtJoin jn;
-          jn.count = last - blockIdx.x + 1;
-          jn.first = part;
-          jn.row0 = seq.row0;
-          jn.head = w.head;
-          jn.f0 = w.tile * PT_ROWS;
-          jn.rows = min(PT_ROWS, seq.n * group - jn.f0);
-          parts.join[blockIdx.x] = jn;
-        }
+        if (w.j0 == 0 && threadIdx.x == 128)  // begins here, goes on in the next shares
+          parts.join[blockIdx.x] = w.join(sh.table, blockIdx.x, part, group);
       } else {
         if (lse && valid) lse[((int64_t)seq.row0 + i) * heads + h] = row_lse;
         // through the Q tile (no S reads it any more), so that half a warp writes a whole row
@@ -788,16 +569,17 @@ constexpr int PJ_ROWS = 32;
 constexpr int PJ_WARPS = 8;
 template <typename T>
 __global__ void __launch_bounds__(PJ_WARPS * 32)
-    paged_join_kernel(const PtParts parts, int heads, int group, T* __restrict__ out,
+    paged_join_kernel(const ShareParts parts, int heads, int group, T* __restrict__ out,
                       int64_t out_stride, float* __restrict__ lse) {
   using H = Half16<T>;
-  const PtJoin jn = parts.join[blockIdx.x];
+  pdl_wait();
+  const ShareJoin jn = parts.join[blockIdx.x];
   const int r0 = blockIdx.y * PJ_ROWS;
   if (jn.count == 0 || r0 >= jn.rows) return;
   __shared__ float tile[PJ_ROWS][PG_HD + 1];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int r = r0 + lane;
-  auto part_of = [&](int p) { return p == 0 ? jn.first : 2 * ((int)blockIdx.x + p); };
+  auto part_of = [&](int p) { return share_part(jn, blockIdx.x, p); };
   float mx = -CUDART_INF_F;
   for (int p = 0; p < jn.count; ++p) mx = fmaxf(mx, parts.lse[part_of(p) * PT_ROWS + r]);
   const float base = mx == -CUDART_INF_F ? 0.f : mx;

@@ -90,6 +90,15 @@ __device__ __forceinline__ PagedTile paged_find_tile(const PagedKV& kv, int grou
   return PagedTile{-1, 0, PagedSeq{0, 0, 0, 0}};
 }
 
+// Programmatic dependent launch, in its two halves: a kernel lets the next one on the stream
+// start (it then waits in pdl_wait for this one's end and memory).
+__device__ __forceinline__ void pdl_launch_dependents() {
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+}
+__device__ __forceinline__ void pdl_wait() {
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+}
+
 // 2^x of two numbers on the FMA pipes, for kernels whose exponentials keep the MUFU busy
 // (16 results a clock and SM). x = n + f with n the nearest whole number: 2^f on [-1/2, 1/2] by
 // the polynomial of degree DEG with the least largest relative error (Remez's exchange; degree

@@ -1,0 +1,235 @@
+// Equal shares of a step's attention work.
+//
+// The query rows of each key head in each sequence are cut into tiles of ROWS, a tile's keys
+// into steps of KEYS. Sequences differ in length, so the steps of all tiles (sequence, key
+// head, tile in this order: neighbours share K and V in L2), and UNITS more per tile for its
+// own cost, are laid end to end, and every worker takes an equal share of these units. A
+// worker that has all steps of a tile writes its output; of a tile that is cut, each worker
+// writes its part (at most two: its first and its last tile), and a second kernel joins them.
+#pragma once
+#include "paged_common.cuh"
+
+namespace cb {
+
+constexpr int SHARE_CHUNK = 1024;  // sequences whose units are added up at a time
+
+// What is to be joined: one record per worker, the tile that begins in its share and goes on
+// behind it. Part 2 w is worker w's first segment, 2 w + 1 its last one.
+struct ShareJoin {
+  int count;  // parts, 0 = no such tile
+  int first;  // part of this worker; the others are 2 (w + 1), 2 (w + 2), ...
+  int row0, head, f0, rows;
+};
+struct ShareParts {
+  float* o;    // the parts' outputs, normalised within the part
+  float* lse;  // and base-2 log-sum-exps
+  ShareJoin* join;
+};
+__device__ __forceinline__ int share_part(const ShareJoin& jn, int worker, int p) {
+  return p == 0 ? jn.first : 2 * (worker + p);
+}
+
+struct ShareTable {  // in shared memory
+  int64_t seq_units[SHARE_CHUNK];
+  int64_t total;  // units of all tiles and key heads
+  int workers;    // that have a share
+};
+
+// LEAST: units of a share at least; above UNITS, so that every share has a step.
+template <int ROWS, int KEYS, int UNITS, int LEAST>
+struct PagedShares {
+  static_assert(LEAST > UNITS, "a share without a step");
+
+  // Steps of a tile: up to the last slot that its last row sees. A tile that sees nothing has
+  // one step too (in which everything is masked): it writes its zeros.
+  static __device__ __forceinline__ int tile_steps(const PagedSeq& seq, int group, int tile) {
+    const int last = min((tile + 1) * ROWS, seq.n * group) - 1;
+    return max(1, (seq.limit(last / group) + KEYS - 1) / KEYS);
+  }
+  static __device__ __forceinline__ int tiles(const PagedSeq& seq, int group) {
+    return (seq.n * group + ROWS - 1) / ROWS;
+  }
+
+  // A worker's walk over its share: segments of tiles.
+  struct Walk {
+    PagedSeq seq;
+    int b, head, tile;
+    int u0;             // the segment's first unit within the tile
+    int j0, j1, steps;  // the segment: steps j0 .. j1 - 1 of the tile's `steps`
+    int64_t at, end;    // the segment's first unit among all, and the share's end
+
+    __device__ __forceinline__ int u1() const {
+      return (int)min((int64_t)(steps + UNITS), u0 + (end - at));
+    }
+    __device__ __forceinline__ void segment(int group) {
+      steps = tile_steps(seq, group, tile);
+      j0 = max(0, u0 - UNITS);
+      j1 = max(0, u1() - UNITS);
+    }
+    // The next segment; false when the share is done.
+    __device__ __forceinline__ bool next(const PagedKV& kv, int group) {
+      do {
+        at += u1() - u0;
+        if (at >= end) return false;
+        u0 = 0;
+        if (++tile >= tiles(seq, group)) {
+          tile = 0;
+          if (++head >= kv.kv_heads) {
+            head = 0;
+            do {
+              if (++b >= kv.batch) return false;
+              seq = paged_seq(kv, b);
+            } while (seq.n == 0);
+          }
+        }
+        segment(group);
+      } while (j1 == j0);  // a share may end before a tile's first step
+      return true;
+    }
+    __device__ __forceinline__ bool whole() const { return j0 == 0 && j1 == steps; }
+    __device__ __forceinline__ int rows(int group) const {
+      return min(ROWS, seq.n * group - tile * ROWS);
+    }
+    // The join record of a segment that begins its tile and does not end it.
+    __device__ __forceinline__ ShareJoin join(const ShareTable& table, int worker, int part,
+                                              int group) const {
+      const int64_t last_unit = at - u0 + UNITS + steps - 1;
+      ShareJoin jn;
+      jn.count = (int)(((last_unit + 1) * table.workers - 1) / table.total) - worker + 1;
+      jn.first = part;
+      jn.row0 = seq.row0;
+      jn.head = head;
+      jn.f0 = tile * ROWS;
+      jn.rows = rows(group);
+      return jn;
+    }
+  };
+
+  // The whole block: adds up the units of all sequences and puts every warp's walk at the
+  // beginning of its share (workers 0 .. most - 1; warps may be of one worker or of several).
+  // False in the warps whose worker has none.
+  static __device__ __forceinline__ bool begin(const PagedKV& kv, int group, ShareTable& table,
+                                               int most, int worker, Walk& walk) {
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int warps = blockDim.x >> 5;
+    // A warp per sequence where sequences are few and have many tiles, else a thread (their
+    // loads are one after another).
+    const bool by_warp = kv.max_new * group > 8 * ROWS && kv.batch <= 8 * warps;
+    auto add_up = [&](int base, int count) {
+      if (by_warp) {
+        for (int i = warp; i < count; i += warps) {
+          const PagedSeq s = paged_seq(kv, base + i);
+          const int n_tiles = tiles(s, group);
+          int64_t n = 0;
+          for (int t = lane; t < n_tiles; t += 32) n += tile_steps(s, group, t) + UNITS;
+#pragma unroll
+          for (int off = 16; off > 0; off >>= 1) n += __shfl_xor_sync(0xffffffffu, n, off);
+          if (lane == 0) table.seq_units[i] = n;
+        }
+      } else {
+        for (int i = threadIdx.x; i < count; i += blockDim.x) {
+          const PagedSeq s = paged_seq(kv, base + i);
+          const int n_tiles = tiles(s, group);
+          int64_t n = 0;
+          for (int t = 0; t < n_tiles; ++t) n += tile_steps(s, group, t) + UNITS;
+          table.seq_units[i] = n;
+        }
+      }
+      __syncthreads();
+    };
+    // The sequence of a chunk that holds unit `want` and the units of it before that, or -1
+    // and the units so far.
+    auto scan = [&](int count, int64_t before, int64_t want, int64_t& inside) -> int {
+      for (int i = 0; i < count; i += 32) {
+        const int64_t n = i + lane < count ? table.seq_units[i + lane] : 0;
+        int64_t incl = n;
+#pragma unroll
+        for (int off = 1; off < 32; off <<= 1) {
+          const int64_t up = __shfl_up_sync(0xffffffffu, incl, off);
+          if (lane >= off) incl += up;
+        }
+        const unsigned past = __ballot_sync(0xffffffffu, before + incl > want);
+        if (past) {
+          const int src = __ffs(past) - 1;
+          inside = want - before - __shfl_sync(0xffffffffu, incl - n, src);
+          return i + src;
+        }
+        before += __shfl_sync(0xffffffffu, incl, 31);
+      }
+      inside = before;
+      return -1;
+    };
+    int64_t total = 0;
+    for (int base = 0; base < kv.batch; base += SHARE_CHUNK) {
+      const int count = min(SHARE_CHUNK, kv.batch - base);
+      __syncthreads();
+      add_up(base, count);
+      int64_t inside;
+      scan(count, total, INT64_MAX, inside);
+      total = inside;
+    }
+    const int64_t all = total * kv.kv_heads;
+    const int workers = (int)max((int64_t)1, min((int64_t)most, all / LEAST));
+    const int64_t lo = worker < workers ? all * worker / workers : all;
+    const int64_t hi = worker < workers ? all * (worker + 1) / workers : all;
+    if (threadIdx.x == 0) {
+      table.total = all;
+      table.workers = workers;
+    }
+    // heads of one sequence lie side by side: unit lo lies in the sequence that holds unit
+    // lo / kv_heads of one head
+    const int64_t want = lo / kv.kv_heads;
+    int64_t before = 0;
+    bool found = lo >= hi;
+    for (int base = 0; base < kv.batch; base += SHARE_CHUNK) {
+      const int count = min(SHARE_CHUNK, kv.batch - base);
+      if (kv.batch > SHARE_CHUNK) {
+        __syncthreads();
+        add_up(base, count);
+      }
+      int64_t inside;
+      const int i = found ? -1 : scan(count, before, want, inside);
+      if (i >= 0) {
+        found = true;
+        const int64_t one = table.seq_units[i];
+        int64_t r = lo - (want - inside) * kv.kv_heads;  // within the sequence
+        const int head = (int)(r / one);
+        r -= head * one;
+        const PagedSeq s = paged_seq(kv, base + i);
+        const int n_tiles = tiles(s, group);
+        int64_t run = 0;
+        for (int t0 = 0; t0 < n_tiles; t0 += 32) {
+          const int n = t0 + lane < n_tiles ? tile_steps(s, group, t0 + lane) + UNITS : 0;
+          int64_t incl = n;
+#pragma unroll
+          for (int off = 1; off < 32; off <<= 1) {
+            const int64_t up = __shfl_up_sync(0xffffffffu, incl, off);
+            if (lane >= off) incl += up;
+          }
+          const unsigned past = __ballot_sync(0xffffffffu, run + incl > r);
+          if (past) {
+            if (lane == __ffs(past) - 1) {
+              walk.seq = s;
+              walk.b = base + i;
+              walk.head = head;
+              walk.tile = t0 + lane;
+              walk.u0 = (int)(r - run - (incl - n));
+              walk.at = lo;
+              walk.end = hi;
+              walk.segment(group);
+              if (walk.j1 == walk.j0) walk.next(kv, group);
+            }
+            break;
+          }
+          run += __shfl_sync(0xffffffffu, incl, 31);
+        }
+      } else if (!found) {
+        before = inside;
+      }
+    }
+    __syncthreads();
+    return lo < hi;
+  }
+};
+
+}  // namespace cb
