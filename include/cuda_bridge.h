@@ -551,7 +551,7 @@ cb_status cb_paged_attention_workspace(const cb_paged_kv* kv, int32_t heads, siz
 /* Attention of a step's new tokens over the cache: query row r (token i of n of sequence b)
  * sees the slots 0 .. len[b] - n + i (the new tokens' own K and V must be in the cache:
  * cb_paged_append). out[r][h] = softmax(scale * q[r][h] . K) V with key head
- * h / (heads / kv_heads). heads is a multiple of kv_heads. q and out: [rows][heads][128];
+ * h / (heads / kv_heads). heads is a multiple of kv_heads, at most 128 times it. q and out: [rows][heads][128];
  * out must not overlap q. lse (nullable, [rows][heads]): the base-2 log-sum-exp of the
  * scaled scores, as cb_attention_fwd_lse_f16. A row that sees no slot gets out = 0 and
  * lse = -inf. workspace: 16-byte aligned; its contents do not matter and none are kept, but

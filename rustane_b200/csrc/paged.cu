@@ -53,7 +53,8 @@ bool kv_pointers_ok(const cb_paged_kv* kv, bool rows_needed) {
 }
 
 bool heads_ok(const cb_paged_kv* kv, int32_t heads) {
-  return heads > 0 && heads % kv->kv_heads == 0 && (int64_t)kv->rows * heads <= INT_LIMIT &&
+  return heads > 0 && heads % kv->kv_heads == 0 && heads / kv->kv_heads <= 128 &&
+         (int64_t)kv->rows * heads <= INT_LIMIT &&
          (int64_t)kv->max_new * heads <= INT_LIMIT;
 }
 
@@ -266,16 +267,17 @@ cb_status launch_weights(const cb_paged_kv* kv, const T* q, int64_t q_stride, in
   const int group = heads / kv->kv_heads;
   const PagedKV d = device_kv(kv);
   const float scale_log2 = scale * 1.4426950408889634f;
-  // the tcgen05 kernel needs a token's whole group in a step
-  const bool tc = (int64_t)kv->max_new * group > PR_ROWS && group <= WT_ROWS;
-  const int blocks = (int)ceil_div(kv->max_len, tc ? WT_KEYS : PW_KEYS);
-  const int64_t grid = (int64_t)kv->batch * blocks * kv->kv_heads;
-  if (grid > INT_LIMIT) return CB_ERR_UNSUPPORTED;
-  if (!tc) {
-    paged_weights_kernel<T><<<(unsigned)grid, PW_WARPS * 32, 0, st>>>(
-        d, q, q_stride, heads, scale_log2, lse, weights, blocks);
+  if ((int64_t)kv->max_new * group <= PR_ROWS) {
+    // two CTAs per SM; no more than there are blocks of slots
+    const double blocks = (double)kv->batch * kv->kv_heads * ceil_div(kv->max_len, PR_BLOCK);
+    const int ctas = (int)std::max(1.0, std::min(2.0 * PG_SMS, blocks));
+    paged_weights_kernel<T><<<ctas, PW_WARPS * 32, 0, st>>>(d, q, q_stride, heads, scale_log2, lse,
+                                                           weights);
     return status_of(cudaPeekAtLastError());
   }
+  const int blocks = (int)ceil_div(kv->max_len, WT_KEYS);
+  const int64_t grid = (int64_t)kv->batch * blocks * kv->kv_heads;
+  if (grid > INT_LIMIT) return CB_ERR_UNSUPPORTED;
   const int box = std::min(kv->page_size, 128), tokens = WT_ROWS / group;
   CUtensorMap tk, tq;
   if (!make_cache_map(&tk, kv->k, kv, box) ||

@@ -376,79 +376,131 @@ __global__ void __launch_bounds__(PR_WARPS * 32)
 }
 
 // ------------------------------------------------------------------ attention weights
-// w_k += sum_r 2^(s_rk - lse_r) over the rows that see slot k. The slots are the matrix
-// instruction's rows here (S^T = K Q^T), so a slot's sum stays in the lanes of one quad. A
-// warp keeps 16 slots' K in registers and walks the query rows eight at a time.
+// w_k += sum_r 2^(s_rk - lse_r) over the rows that see slot k, for at most 16 query rows per key
+// head (one tile, so a slot has one worker). The slots are the matrix instruction's rows here
+// (S^T = K Q^T) and the query rows its columns, so a slot's sum stays in the lanes of a quad.
 // The dot product may take the head's elements in any order: lane c of a quad takes the
-// 16-byte pieces c, c + 4, ... of both operands, so a quad reads whole 64-byte runs and no
-// shared memory is needed.
-constexpr int PW_WARPS = 4;
-constexpr int PW_KEYS = PW_WARPS * 16;  // slots of a CTA
+// 16-byte pieces c, c + 4, ... of both operands, so a quad reads whole 64-byte runs and K goes
+// to registers directly. Bound by the reads of K: a warp is a worker as in the attention
+// kernel, with one block of 16 slots on its way while it works on another.
+constexpr int PW_WARPS = 8;  // two CTAs per SM
+struct PwShared {
+  PrShares::Walk walk[PW_WARPS];
+  ShareTable table;
+};
 
-// Grid: ((sequence * blocks of PW_KEYS slots) + block) * kv_heads + key head.
 template <typename T>
-__global__ void __launch_bounds__(PW_WARPS * 32)
+__global__ void __launch_bounds__(PW_WARPS * 32, 2)
     paged_weights_kernel(const PagedKV kv, const T* __restrict__ q, int64_t q_stride, int heads,
                          float scale_log2, const float* __restrict__ lse,
-                         float* __restrict__ weights, int blocks) {
+                         float* __restrict__ weights) {
   using H = Half16<T>;
+  __shared__ PwShared sh;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int group = heads / kv.kv_heads;
-  const int head = blockIdx.x % kv.kv_heads;
-  const int rest = blockIdx.x / kv.kv_heads;
-  const int b = rest / blocks;
-  const PagedSeq seq = paged_seq(kv, b);
-  const int key0 = (rest % blocks) * PW_KEYS + warp * 16;
-  if (seq.n == 0 || key0 >= seq.end || key0 >= seq.limit(seq.n - 1)) return;
-  const int id = kv.page_id(b, key0);  // a page holds whole blocks of 16
-  if (id < 0) return;
-  const int row = kv.page_row(id, head, key0);
+  PrShares::Walk& w = sh.walk[warp];
+  if (!PrShares::begin(kv, group, sh.table, gridDim.x * PW_WARPS, warp * gridDim.x + blockIdx.x, w))
+    return;
+  __syncwarp();
   const int r0 = lane >> 2, c = lane & 3;
-
-  uint4 kf[2][4];
+  const T* k_pool = static_cast<const T*>(kv.k);
+  bool go_on;
+  do {
+    const PagedSeq seq = w.seq;
+    const int b = w.b, head = w.head, rows = w.rows(group), j1 = w.j1;
+    // Q: row lane / 4 of each half of the tile's rows; and of this lane's columns 2 c + e the
+    // log-sum-exp and limit (no slot for the columns behind the last row)
+    uint4 qf[2][4];
+    float x[2][2];
+    int lim[2][2];
 #pragma unroll
-  for (int j = 0; j < 2; ++j)
+    for (int h = 0; h < 2; ++h) {
+      const int f = min(h * 8 + r0, rows - 1), i = f / group;
+      const T* qp = q + (seq.row0 + i) * q_stride + (int64_t)(head * group + f - i * group) * PG_HD;
 #pragma unroll
-    for (int p = 0; p < 4; ++p)
-      kf[j][p] = *reinterpret_cast<const uint4*>(
-          static_cast<const T*>(kv.k) + (int64_t)(row + r0 + 8 * j) * PG_HD + p * 32 + c * 8);
-
-  // the first token that sees key0; the ones before it add nothing
-  const int i0 = max(0, key0 - seq.past);
-  const int f_end = seq.n * group;
-  float sum[2] = {0.f, 0.f};
-  for (int f0 = i0 * group; f0 < f_end; f0 += 8) {
-    const int f = min(f0 + r0, f_end - 1);
-    const int i = f / group;
-    const T* qp = q + (int64_t)(seq.row0 + i) * q_stride + (int64_t)(head * group + f - i * group) * PG_HD;
-    uint4 qf[4];
+      for (int p = 0; p < 4; ++p) qf[h][p] = *reinterpret_cast<const uint4*>(qp + p * 32 + c * 8);
 #pragma unroll
-    for (int p = 0; p < 4; ++p) qf[p] = *reinterpret_cast<const uint4*>(qp + p * 32 + c * 8);
-    float s[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-    for (int p = 0; p < 4; ++p) {
-      const uint32_t a0[4] = {kf[0][p].x, kf[1][p].x, kf[0][p].y, kf[1][p].y};
-      const uint32_t a1[4] = {kf[0][p].z, kf[1][p].z, kf[0][p].w, kf[1][p].w};
-      H::mma(s, a0, qf[p].x, qf[p].y);
-      H::mma(s, a1, qf[p].z, qf[p].w);
-    }
-#pragma unroll
-    for (int j = 0; j < 2; ++j) {  // this lane's two query rows
-      const int fq = f0 + 2 * c + j;
-      if (fq < f_end) {
-        const int iq = fq / group;
-        const float x = __ldg(lse + (int64_t)(seq.row0 + iq) * heads + head * group + fq - iq * group);
-        const int lim = seq.limit(iq);
-        if (key0 + r0 < lim) sum[0] += exp2_mufu(fmaf(s[j], scale_log2, -x));
-        if (key0 + r0 + 8 < lim) sum[1] += exp2_mufu(fmaf(s[2 + j], scale_log2, -x));
+      for (int e = 0; e < 2; ++e) {
+        const int fc = h * 8 + 2 * c + e, ic = min(fc, rows - 1) / group;
+        const int g = min(fc, rows - 1) - ic * group;
+        x[h][e] = -__ldg(lse + (int64_t)(seq.row0 + ic) * heads + head * group + g);
+        lim[h][e] = fc < rows ? seq.limit(ic) : 0;
       }
     }
-  }
+    // rows of the cache of the next 32 blocks, a lane each
+    int first = w.j0, at = -1;
+    auto look_up = [&]() {
+      const int key = (first + lane) * PR_BLOCK;
+      const int id = first + lane < j1 && key < seq.end ? kv.page_id(b, key) : -1;
+      at = id >= 0 ? kv.page_row(id, head, key) : -1;
+    };
+    auto load = [&](int row, uint4 (&k)[2][4]) {
+      if (row < 0) return;  // a page outside the pool
 #pragma unroll
-  for (int j = 0; j < 2; ++j) {
-    sum[j] = quad_sum(sum[j]);
-    if (c == 0 && key0 + r0 + 8 * j < seq.end) atomicAdd(weights + row + r0 + 8 * j, sum[j]);
-  }
+      for (int j = 0; j < 2; ++j)
+#pragma unroll
+        for (int p = 0; p < 4; ++p)
+          k[j][p] = *reinterpret_cast<const uint4*>(k_pool + (int64_t)(row + r0 + 8 * j) * PG_HD +
+                                                    p * 32 + c * 8);
+    };
+    auto use = [&](int jb, int row, const uint4 (&k)[2][4]) {
+      if (row < 0) return;
+      const int key0 = jb * PR_BLOCK;
+      float sum[2] = {0.f, 0.f};
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        if (h * 8 >= rows) break;
+        float s[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int p = 0; p < 4; ++p) {
+          const uint32_t a0[4] = {k[0][p].x, k[1][p].x, k[0][p].y, k[1][p].y};
+          const uint32_t a1[4] = {k[0][p].z, k[1][p].z, k[0][p].w, k[1][p].w};
+          H::mma(s, a0, qf[h][p].x, qf[h][p].y);
+          H::mma(s, a1, qf[h][p].z, qf[h][p].w);
+        }
+#pragma unroll
+        for (int e = 0; e < 2; ++e)
+#pragma unroll
+          for (int j = 0; j < 2; ++j)
+            if (key0 + r0 + 8 * j < lim[h][e])
+              sum[j] += exp2_mufu(fmaf(s[2 * j + e], scale_log2, x[h][e]));
+      }
+      sum[0] = quad_sum(sum[0]);
+      sum[1] = quad_sum(sum[1]);
+      const int mine = r0 + 8 * c;  // lanes c = 0, 1 write a slot each
+      if (c < 2 && key0 + mine < seq.end) atomicAdd(weights + row + mine, c ? sum[1] : sum[0]);
+    };
+    uint4 ka[2][4], kb[2][4];
+    look_up();
+    int row_a = __shfl_sync(0xffffffffu, at, 0), row_b = -1;
+    load(row_a, ka);
+    for (int jb = first; jb < j1; jb += 2) {
+      if (jb + 1 < j1) {
+        if (jb + 1 - first >= 32) {
+          first = jb + 1;
+          look_up();
+        }
+        row_b = __shfl_sync(0xffffffffu, at, jb + 1 - first);
+        load(row_b, kb);
+      }
+      use(jb, row_a, ka);
+      if (jb + 1 < j1) {
+        if (jb + 2 < j1) {
+          if (jb + 2 - first >= 32) {
+            first = jb + 2;
+            look_up();
+          }
+          row_a = __shfl_sync(0xffffffffu, at, jb + 2 - first);
+          load(row_a, ka);
+        }
+        use(jb + 1, row_b, kb);
+      }
+    }
+    __syncwarp();
+    go_on = false;
+    if (lane == 0) go_on = w.next(kv, group);
+    go_on = __any_sync(0xffffffffu, go_on);
+  } while (go_on);
 }
 
 }  // namespace cb

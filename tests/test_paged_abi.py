@@ -137,6 +137,12 @@ def test_evict_refusals(bridge_lib, change):
     assert _evict(bridge_lib, _kv(), **change) == BAD
 
 
+def test_more_than_128_query_heads_to_a_key_head_are_refused(bridge_lib):
+    kv = _kv(kv_heads=1)
+    assert _attention(bridge_lib, kv, heads=129, q_stride=1 << 16, out_stride=1 << 16) == BAD
+    assert _weights(bridge_lib, kv, heads=129, qs=1 << 16) == BAD
+
+
 def test_evict_refuses_sequences_that_no_cluster_holds(bridge_lib):
     kv = _kv(max_len=262145, table_stride=20000, pages=20000)
     assert _evict(bridge_lib, kv) == B.CB_ERR_UNSUPPORTED
