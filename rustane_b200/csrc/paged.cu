@@ -9,7 +9,9 @@
 #include <atomic>
 #include <cmath>
 #include <cstdint>
+#include <initializer_list>
 #include <limits>
+#include <type_traits>
 
 #include "cuda_bridge.h"
 #include "paged_attention.cuh"
@@ -308,6 +310,18 @@ cudaError_t launch_evict(const PagedKV& kv, const EvictArgs& a, int ctas, cudaSt
   return cudaLaunchKernelEx(&cfg, paged_evict_kernel<THREADS, PER>, kv, a, ctas);
 }
 
+// Calls f with a value of the 16-bit type and the piece size as a type.
+template <typename F>
+void with_type(int32_t dtype, int piece, F&& f) {
+  using P4 = std::integral_constant<int, 4>;
+  using P8 = std::integral_constant<int, 8>;
+  if (dtype == CB_DTYPE_F16) {
+    if (piece == 8) f(__half(), P8()); else f(__half(), P4());
+  } else {
+    if (piece == 8) f(__nv_bfloat16(), P8()); else f(__nv_bfloat16(), P4());
+  }
+}
+
 }  // namespace
 
 extern "C" {
@@ -372,24 +386,22 @@ cb_status cb_rope(const cb_rope_config* rope, int32_t dtype, const void* x, int6
     return CB_ERR_INVALID_ARG;
   const cb_status s = check_device({x, y, positions, rope->inv_freq});
   if (s != CB_OK) return s;
-  // Heads of a thread: enough to spread an angle's cost, few enough to fill the GPU.
-  const int64_t units = (int64_t)tokens * heads * (head_dim / 8);
-  const int per_thread = units >= (int64_t)PG_SMS * 2048 * 4 ? 4 : 1;
-  const int64_t threads = (int64_t)tokens * ceil_div(heads, per_thread) * (head_dim / 8);
-  const int64_t blocks = ceil_div(threads, ROPE_THREADS);
+  const int piece = rope->rot_dim % 16 == 0 && head_dim % 16 == 0 ? 8 : 4;
+  // Heads of a thread: as many as leave half of the GPU's threads busy.
+  const int64_t units = (int64_t)tokens * (head_dim / (2 * piece));
+  const int64_t chunks_wanted = std::max<int64_t>(1, ceil_div((int64_t)PG_SMS * 1024, units));
+  const int per_thread = (int)std::max<int64_t>(1, heads / std::min<int64_t>(heads, chunks_wanted));
+  const int64_t blocks = ceil_div(units * ceil_div(heads, per_thread), ROPE_THREADS);
   if (blocks > INT_LIMIT) return CB_ERR_UNSUPPORTED;
-  const bool half = rope->layout == CB_ROPE_HALF;
-  const float amp = rope->amplitude, amp_sin = inverse ? -amp : amp;
-  cudaStream_t st = static_cast<cudaStream_t>(stream);
-  if (dtype == CB_DTYPE_F16)
-    rope_kernel<__half><<<(unsigned)blocks, ROPE_THREADS, 0, st>>>(
-        static_cast<const __half*>(x), x_stride, static_cast<__half*>(y), y_stride, positions,
-        rope->inv_freq, rope->rot_dim, half, amp, amp_sin, tokens, heads, head_dim, per_thread);
-  else
-    rope_kernel<__nv_bfloat16><<<(unsigned)blocks, ROPE_THREADS, 0, st>>>(
-        static_cast<const __nv_bfloat16*>(x), x_stride, static_cast<__nv_bfloat16*>(y), y_stride,
-        positions, rope->inv_freq, rope->rot_dim, half, amp, amp_sin, tokens, heads, head_dim,
-        per_thread);
+  auto launch = [&](auto type, auto piece_of) {
+    using T = decltype(type);
+    rope_kernel<T, decltype(piece_of)::value>
+        <<<(unsigned)blocks, ROPE_THREADS, 0, static_cast<cudaStream_t>(stream)>>>(
+            static_cast<const T*>(x), x_stride, static_cast<T*>(y), y_stride, positions,
+            rope->inv_freq, rope->rot_dim, rope->layout == CB_ROPE_HALF, rope->amplitude,
+            inverse ? -rope->amplitude : rope->amplitude, tokens, heads, head_dim, per_thread);
+  };
+  with_type(dtype, piece, launch);
   return status_of(cudaPeekAtLastError());
 }
 
@@ -421,30 +433,27 @@ cb_status cb_paged_append(const cb_paged_kv* kv, const cb_rope_config* rope, int
                     q, q_out, k, v, positions, weights, slot_positions});
   if (s != CB_OK) return s;
   const int all = heads + 2 * kv->kv_heads;
-  // Heads of a warp: two at a time; more of them where there are warps enough.
-  const int per_warp = rows * all / 8 >= (int64_t)PG_SMS * 64 ? 8 : 2;
-  const int64_t warps = rows * ceil_div(all, per_warp);
-  const int64_t blocks = ceil_div(warps, APPEND_WARPS);
-  if (blocks > INT_LIMIT) return CB_ERR_UNSUPPORTED;
-  const double* freq = rope ? rope->inv_freq : nullptr;
   const int rot = rope ? rope->rot_dim : 0;
-  const bool half = rope && rope->layout == CB_ROPE_HALF;
-  const float amp = rope ? rope->amplitude : 1.0f;
+  const int piece = rot % 16 == 0 ? 8 : 4;
+  const int at_once = 32 / (PG_HD / (2 * piece));
+  // Heads of a warp: as many as leave the GPU's warps three quarters busy (they share their
+  // angles), a whole number of loads.
+  const int64_t chunks_wanted = std::max<int64_t>(1, ceil_div((int64_t)PG_SMS * 48, rows));
+  const int64_t heads_wanted = all / std::min<int64_t>(all, chunks_wanted);
+  const int per_warp = (int)std::max<int64_t>(1, heads_wanted / at_once) * at_once;
+  const int64_t blocks = ceil_div(rows * ceil_div(all, per_warp), APPEND_WARPS);
+  if (blocks > INT_LIMIT) return CB_ERR_UNSUPPORTED;
   const PagedKV d = device_kv(kv);
-  cudaStream_t st = static_cast<cudaStream_t>(stream);
-  if (kv->dtype == CB_DTYPE_F16) {
-    using T = __half;
-    paged_append_kernel<T><<<(unsigned)blocks, APPEND_WARPS * 32, 0, st>>>(
-        d, static_cast<const T*>(q), q_stride, static_cast<T*>(q_out), q_out_stride, heads,
-        static_cast<const T*>(k), k_stride, static_cast<const T*>(v), v_stride, positions, freq, rot,
-        half, amp, weights, slot_positions, per_warp);
-  } else {
-    using T = __nv_bfloat16;
-    paged_append_kernel<T><<<(unsigned)blocks, APPEND_WARPS * 32, 0, st>>>(
-        d, static_cast<const T*>(q), q_stride, static_cast<T*>(q_out), q_out_stride, heads,
-        static_cast<const T*>(k), k_stride, static_cast<const T*>(v), v_stride, positions, freq, rot,
-        half, amp, weights, slot_positions, per_warp);
-  }
+  auto launch = [&](auto type, auto piece_of) {
+    using T = decltype(type);
+    paged_append_kernel<T, decltype(piece_of)::value>
+        <<<(unsigned)blocks, APPEND_WARPS * 32, 0, static_cast<cudaStream_t>(stream)>>>(
+            d, static_cast<const T*>(q), q_stride, static_cast<T*>(q_out), q_out_stride, heads,
+            static_cast<const T*>(k), k_stride, static_cast<const T*>(v), v_stride, positions,
+            rope ? rope->inv_freq : nullptr, rot, rope && rope->layout == CB_ROPE_HALF,
+            rope ? rope->amplitude : 1.0f, weights, slot_positions, per_warp);
+  };
+  with_type(kv->dtype, piece, launch);
   return status_of(cudaPeekAtLastError());
 }
 

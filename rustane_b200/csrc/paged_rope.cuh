@@ -1,11 +1,12 @@
 // Rotary positions: pair i of a head at position p is turned by the angle a = p f_i,
 //   (x0, x1) -> (x0 cos a - x1 sin a, x1 cos a + x0 sin a),
-// its gradient by -a. Both kernels move 2 + 2 bytes an element and do little else, so they
-// are bound by memory. A thread owns four pairs of a head (eight elements: two 8-byte
-// pieces, adjacent for interleaved pairs and rot_dim / 2 apart for half pairs) at one token
-// and walks heads with them: an angle is formed once for all of a thread's heads, both
-// elements of a pair meet in one thread (so a tensor can be rotated in place), and the lanes
-// of a head read whole 32-byte sectors.
+// its gradient by -a. Both kernels move 2 + 2 bytes an element and are bound by memory as long
+// as an angle (it costs about as much as moving ten elements) serves several heads. A thread
+// owns PIECE pairs of a head at one token (two pieces of PIECE elements, adjacent for
+// interleaved pairs and rot_dim / 2 apart for half pairs) and walks heads with them: an angle is
+// formed once for all of a thread's heads, both elements of a pair meet in one thread (so a
+// tensor can be rotated in place), and the next heads' loads are out while a head is turned.
+// PIECE is 8 (16-byte accesses) where rot_dim and the head's size are multiples of 16, else 4.
 // The angle is formed in 64 bits as a fraction of a turn (at position 10^6 a 32-bit product
 // would be off by 0.06 rad), reduced to [-1/2, 1/2] there, and only then rounded to 32 bits.
 #pragma once
@@ -13,58 +14,84 @@
 
 namespace cb {
 
-// cos and sin of pairs 4u .. 4u + 3 at position p, times amp (sin times amp_sin).
-__device__ __forceinline__ void rope_angles(const double* __restrict__ inv_freq, int u, int p,
-                                            float amp, float amp_sin, float (&c)[4],
-                                            float (&s)[4]) {
+template <int PIECE>
+struct RopeUnit {
+  static constexpr int WORDS = PIECE / 2;  // of a piece
+  float c[PIECE], s[PIECE];                // cos and sin of its pairs
+  int off_a, off_b;                        // of its pieces within the head
+  bool turn;                               // false: these elements pass
+  bool half_layout;
+
+  __device__ __forceinline__ RopeUnit(int u, int rot, bool half) : half_layout(half) {
+    turn = u < rot / (2 * PIECE);
+    const bool apart = half && turn;
+    off_a = apart ? PIECE * u : 2 * PIECE * u;
+    off_b = apart ? rot / 2 + PIECE * u : 2 * PIECE * u + PIECE;
+  }
+  // The angles of unit u at position p; sin times amp_sin.
+  __device__ __forceinline__ void angles(const double* __restrict__ inv_freq, int u, int p,
+                                         float amp, float amp_sin) {
+    if (!turn) return;
 #pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    const double turns = (double)p * __ldg(inv_freq + 4 * u + j) * 0.15915494309189535;
-    float sj, cj;
-    sincospif(2.0f * (float)(turns - rint(turns)), &sj, &cj);
-    c[j] = cj * amp;
-    s[j] = sj * amp_sin;
+    for (int j = 0; j < PIECE; ++j) {
+      const double turns = (double)p * __ldg(inv_freq + PIECE * u + j) * 0.15915494309189535;
+      float sj, cj;
+      sincospif(2.0f * (float)(turns - rint(turns)), &sj, &cj);
+      c[j] = cj * amp;
+      s[j] = sj * amp_sin;
+    }
   }
-}
-
-// The eight elements of unit u: a holds the first four, b the last four.
-template <typename T>
-__device__ __forceinline__ void rope_turn(uint2& a, uint2& b, const float (&c)[4],
-                                          const float (&s)[4], bool half_layout) {
-  using H = Half16<T>;
-  const float2 a0 = H::unpack(a.x), a1 = H::unpack(a.y), b0 = H::unpack(b.x),
-               b1 = H::unpack(b.y);
-  if (half_layout) {
-    a.x = H::pack(a0.x * c[0] - b0.x * s[0], a0.y * c[1] - b0.y * s[1]);
-    a.y = H::pack(a1.x * c[2] - b1.x * s[2], a1.y * c[3] - b1.y * s[3]);
-    b.x = H::pack(b0.x * c[0] + a0.x * s[0], b0.y * c[1] + a0.y * s[1]);
-    b.y = H::pack(b1.x * c[2] + a1.x * s[2], b1.y * c[3] + a1.y * s[3]);
-  } else {
-    a.x = H::pack(a0.x * c[0] - a0.y * s[0], a0.y * c[0] + a0.x * s[0]);
-    a.y = H::pack(a1.x * c[1] - a1.y * s[1], a1.y * c[1] + a1.x * s[1]);
-    b.x = H::pack(b0.x * c[2] - b0.y * s[2], b0.y * c[2] + b0.x * s[2]);
-    b.y = H::pack(b1.x * c[3] - b1.y * s[3], b1.y * c[3] + b1.x * s[3]);
+  template <typename T>
+  static __device__ __forceinline__ void load(const T* head, int off, uint32_t (&w)[WORDS]) {
+    if constexpr (PIECE == 8) {
+      const uint4 x = *reinterpret_cast<const uint4*>(head + off);
+      w[0] = x.x, w[1] = x.y, w[2] = x.z, w[3] = x.w;
+    } else {
+      const uint2 x = *reinterpret_cast<const uint2*>(head + off);
+      w[0] = x.x, w[1] = x.y;
+    }
   }
-}
-
-// Offsets of unit u's two pieces; units from rot / 8 on are not rotated.
-__device__ __forceinline__ void rope_pieces(int u, int rot, bool half_layout, int& off_a,
-                                            int& off_b) {
-  const bool apart = half_layout && u < rot / 8;
-  off_a = apart ? 4 * u : 8 * u;
-  off_b = apart ? rot / 2 + 4 * u : 8 * u + 4;
-}
+  template <typename T>
+  static __device__ __forceinline__ void store(T* head, int off, const uint32_t (&w)[WORDS]) {
+    if constexpr (PIECE == 8)
+      *reinterpret_cast<uint4*>(head + off) = make_uint4(w[0], w[1], w[2], w[3]);
+    else
+      *reinterpret_cast<uint2*>(head + off) = make_uint2(w[0], w[1]);
+  }
+  template <typename T>
+  __device__ __forceinline__ void rotate(uint32_t (&a)[WORDS], uint32_t (&b)[WORDS]) const {
+    using H = Half16<T>;
+    if (half_layout) {  // pair j: element j of both pieces
+#pragma unroll
+      for (int k = 0; k < WORDS; ++k) {
+        const float2 x = H::unpack(a[k]), y = H::unpack(b[k]);
+        a[k] = H::pack(x.x * c[2 * k] - y.x * s[2 * k], x.y * c[2 * k + 1] - y.y * s[2 * k + 1]);
+        b[k] = H::pack(y.x * c[2 * k] + x.x * s[2 * k], y.y * c[2 * k + 1] + x.y * s[2 * k + 1]);
+      }
+    } else {  // pair j: word j of the two pieces one after the other
+#pragma unroll
+      for (int k = 0; k < WORDS; ++k) {
+        const float2 x = H::unpack(a[k]), y = H::unpack(b[k]);
+        const int j = WORDS + k;
+        a[k] = H::pack(x.x * c[k] - x.y * s[k], x.y * c[k] + x.x * s[k]);
+        b[k] = H::pack(y.x * c[j] - y.y * s[j], y.y * c[j] + y.x * s[j]);
+      }
+    }
+  }
+};
 
 constexpr int ROPE_THREADS = 256;
+constexpr int ROPE_BATCH = 2;  // heads whose loads are out together
 
 // Grid: every thread one (token, chunk of per_thread heads, unit), the unit fastest.
-template <typename T>
+template <typename T, int PIECE>
 __global__ void __launch_bounds__(ROPE_THREADS)
     rope_kernel(const T* x, int64_t x_stride, T* y, int64_t y_stride,  // y may be x
                 const int* __restrict__ positions, const double* __restrict__ inv_freq, int rot,
                 bool half_layout, float amp, float amp_sin, int tokens, int heads, int head_dim,
                 int per_thread) {
-  const int units = head_dim / 8;
+  using Unit = RopeUnit<PIECE>;
+  const int units = head_dim / (2 * PIECE);
   const int chunks = (heads + per_thread - 1) / per_thread;
   const int64_t idx = (int64_t)blockIdx.x * ROPE_THREADS + threadIdx.x;
   const int64_t rest = idx / units;
@@ -73,36 +100,43 @@ __global__ void __launch_bounds__(ROPE_THREADS)
   if (t >= tokens) return;
   const int h0 = (int)(rest - t * chunks) * per_thread;
   const int h1 = min(heads, h0 + per_thread);
-  int off_a, off_b;
-  rope_pieces(u, rot, half_layout, off_a, off_b);
-  const bool turn = u < rot / 8;
+  Unit unit(u, rot, half_layout);
   const T* xp = x + t * x_stride;
   T* yp = y + t * y_stride;
-  float c[4], s[4];
-  if (turn) rope_angles(inv_freq, u, __ldg(positions + t), amp, amp_sin, c, s);
-  for (int h = h0; h < h1; h += 4) {
-    uint2 a[4], b[4];
+  uint32_t a[2][ROPE_BATCH][Unit::WORDS], b[2][ROPE_BATCH][Unit::WORDS];
+  auto load = [&](int h, int buf) {
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
+    for (int j = 0; j < ROPE_BATCH; ++j) {
       if (h + j >= h1) break;
-      a[j] = *reinterpret_cast<const uint2*>(xp + (h + j) * head_dim + off_a);
-      b[j] = *reinterpret_cast<const uint2*>(xp + (h + j) * head_dim + off_b);
+      Unit::load(xp + (h + j) * head_dim, unit.off_a, a[buf][j]);
+      Unit::load(xp + (h + j) * head_dim, unit.off_b, b[buf][j]);
     }
+  };
+  auto finish = [&](int h, int buf) {
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
+    for (int j = 0; j < ROPE_BATCH; ++j) {
       if (h + j >= h1) break;
-      if (turn) rope_turn<T>(a[j], b[j], c, s, half_layout);
-      *reinterpret_cast<uint2*>(yp + (h + j) * head_dim + off_a) = a[j];
-      *reinterpret_cast<uint2*>(yp + (h + j) * head_dim + off_b) = b[j];
+      if (unit.turn) unit.template rotate<T>(a[buf][j], b[buf][j]);
+      Unit::store(yp + (h + j) * head_dim, unit.off_a, a[buf][j]);
+      Unit::store(yp + (h + j) * head_dim, unit.off_b, b[buf][j]);
     }
+  };
+  load(h0, 0);
+  unit.angles(inv_freq, u, __ldg(positions + t), amp, amp_sin);
+  for (int h = h0; h < h1; h += 2 * ROPE_BATCH) {
+    load(h + ROPE_BATCH, 1);
+    finish(h, 0);
+    load(h + 2 * ROPE_BATCH, 0);
+    finish(h + ROPE_BATCH, 1);
   }
 }
 
 constexpr int APPEND_WARPS = 8;
 
-// One warp per (row, chunk of per_warp heads): half a warp holds a head's 16 units. The
-// row's heads are counted q first, then k, then v. rot = 0 when nothing is rotated.
-template <typename T>
+// One warp per (row, chunk of per_warp heads): a head's units lie side by side in the warp, so
+// it takes 32 / units heads at once. The row's heads are counted q first, then k, then v.
+// rot = 0 when nothing is rotated.
+template <typename T, int PIECE>
 __global__ void __launch_bounds__(APPEND_WARPS * 32)
     paged_append_kernel(const PagedKV kv, const T* q, int64_t q_stride,
                         T* q_out, int64_t q_out_stride, int heads,  // q_out may be q
@@ -111,6 +145,8 @@ __global__ void __launch_bounds__(APPEND_WARPS * 32)
                         const double* __restrict__ inv_freq, int rot, bool half_layout, float amp,
                         float* __restrict__ weights, int* __restrict__ slot_positions,
                         int per_warp) {
+  using Unit = RopeUnit<PIECE>;
+  constexpr int UNITS = PG_HD / (2 * PIECE), AT_ONCE = 32 / UNITS;
   const int lane = threadIdx.x & 31;
   const int all = heads + 2 * kv.kv_heads;
   const int chunks = (all + per_warp - 1) / per_warp;
@@ -142,43 +178,42 @@ __global__ void __launch_bounds__(APPEND_WARPS * 32)
     }
   }
 
-  const int u = lane & 15;
-  int off_a, off_b;
-  rope_pieces(u, rot, half_layout, off_a, off_b);
-  float c[4], s[4];
-  if (u < rot / 8) rope_angles(inv_freq, u, p, amp, amp, c, s);
+  const int u = lane % UNITS;
+  Unit unit(u, rot, half_layout);
   const int h1 = min(all, (chunk + 1) * per_warp);
-  for (int h0 = chunk * per_warp + (lane >> 4); h0 < h1; h0 += 8) {
-    uint2 a[4], bb[4];
-    const T* src[4];
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const int h = h0 + 2 * j;
-      if (h >= h1) break;
-      src[j] = h < heads ? q + r * q_stride + (int64_t)h * PG_HD
-               : h < heads + kv.kv_heads
-                   ? k + r * k_stride + (int64_t)(h - heads) * PG_HD
-                   : v + r * v_stride + (int64_t)(h - heads - kv.kv_heads) * PG_HD;
-      a[j] = *reinterpret_cast<const uint2*>(src[j] + off_a);
-      bb[j] = *reinterpret_cast<const uint2*>(src[j] + off_b);
+  uint32_t wa[2][Unit::WORDS], wb[2][Unit::WORDS];
+  auto load = [&](int h, int buf) {
+    if (h >= h1) return;
+    const T* src = h < heads ? q + r * q_stride + (int64_t)h * PG_HD
+                   : h < heads + kv.kv_heads
+                       ? k + r * k_stride + (int64_t)(h - heads) * PG_HD
+                       : v + r * v_stride + (int64_t)(h - heads - kv.kv_heads) * PG_HD;
+    Unit::load(src, unit.off_a, wa[buf]);
+    Unit::load(src, unit.off_b, wb[buf]);
+  };
+  auto finish = [&](int h, int buf) {
+    if (h >= h1) return;
+    const bool is_v = h >= heads + kv.kv_heads;
+    if (unit.turn && !is_v) unit.template rotate<T>(wa[buf], wb[buf]);
+    T* dst;
+    if (h < heads) {
+      dst = q_out + r * q_out_stride + (int64_t)h * PG_HD;
+    } else {
+      if (id < 0) return;  // a page outside the pool, or a slot outside the sequence
+      const int hk = is_v ? h - heads - kv.kv_heads : h - heads;
+      dst = static_cast<T*>(is_v ? kv.v : kv.k) + (int64_t)kv.page_row(id, hk, slot) * PG_HD;
     }
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const int h = h0 + 2 * j;
-      if (h >= h1) break;
-      const bool is_v = h >= heads + kv.kv_heads;
-      if (u < rot / 8 && !is_v) rope_turn<T>(a[j], bb[j], c, s, half_layout);
-      T* dst;
-      if (h < heads) {
-        dst = q_out + r * q_out_stride + (int64_t)h * PG_HD;
-      } else {
-        if (id < 0) continue;  // a page outside the pool, or a slot outside the sequence
-        const int hk = is_v ? h - heads - kv.kv_heads : h - heads;
-        dst = static_cast<T*>(is_v ? kv.v : kv.k) + (int64_t)kv.page_row(id, hk, slot) * PG_HD;
-      }
-      *reinterpret_cast<uint2*>(dst + off_a) = a[j];
-      *reinterpret_cast<uint2*>(dst + off_b) = bb[j];
-    }
+    Unit::store(dst, unit.off_a, wa[buf]);
+    Unit::store(dst, unit.off_b, wb[buf]);
+  };
+  const int h0 = chunk * per_warp + lane / UNITS;
+  load(h0, 0);
+  unit.angles(inv_freq, u, p, amp, amp);
+  for (int h = h0; h < h1; h += 2 * AT_ONCE) {
+    load(h + AT_ONCE, 1);
+    finish(h, 0);
+    load(h + 2 * AT_ONCE, 0);
+    finish(h + AT_ONCE, 1);
   }
 }
 
