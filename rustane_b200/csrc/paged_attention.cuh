@@ -14,6 +14,11 @@
 // meets no other warp until the join. (A CTA per tile and part of the keys, whose four warps
 // joined in shared memory, left the SMs idle at every CTA's start and end and in the last
 // wave: 4.4 TB/s on few long sequences, 4.6 on many short ones.)
+//
+// A weight of 0 does not keep an infinity or NaN out of a product. V of slots behind the
+// sequence's end, which may hold anything, reads as 0; and of the slots that only later ones of
+// the step's tokens see, infinities and NaN read as 0 and are added afterwards to the rows that
+// do see them.
 #pragma once
 #include "paged_shares.cuh"
 
@@ -155,6 +160,7 @@ __global__ void __launch_bounds__(PR_WARPS * 32, 1)
 #pragma unroll
       for (int j = 0; j < 4; ++j) o[i][j] = 0.f;
     float m[2] = {-CUDART_INF_F, -CUDART_INF_F}, l[2] = {0.f, 0.f};
+    bool odd_v = false;  // an infinity or NaN was taken out of V
 
     for (int jb = j0; jb < j1; ++jb, ++g) {
       const int stage = g % PR_STAGES;
@@ -216,9 +222,8 @@ __global__ void __launch_bounds__(PR_WARPS * 32, 1)
       // at most half a step of each weight, the size of the output's own rounding.
       const uint32_t pf[4] = {H::pack(s[0][0], s[0][1]), H::pack(s[0][2], s[0][3]),
                               H::pack(s[1][0], s[1][1]), H::pack(s[1][2], s[1][3])};
-      // slots behind the sequence may hold anything, and 0 x NaN is not 0: their V reads as 0
       uint32_t v_mask[2] = {0xffffffffu, 0xffffffffu};
-      const bool v_whole = key0 + PR_BLOCK <= seq.end;
+      const bool v_whole = key0 + PR_BLOCK <= lim_min;  // every row sees every slot
       if (!v_whole) {
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
@@ -233,7 +238,12 @@ __global__ void __launch_bounds__(PR_WARPS * 32, 1)
         ldmatrix_x4_trans(vf, vb + (n >> 2) * 2048 + row * 128 + ((chunk ^ (row & 7)) << 4));
         if (!v_whole) {
 #pragma unroll
-          for (int j = 0; j < 4; ++j) vf[j] &= v_mask[j & 1];
+          for (int j = 0; j < 4; ++j) {
+            vf[j] &= v_mask[j & 1];
+            const uint32_t bad = H::not_finite(vf[j]);
+            odd_v |= bad != 0;
+            vf[j] &= ~bad;
+          }
         }
         H::mma(o[2 * n], pf, vf[0], vf[1]);
         H::mma(o[2 * n + 1], pf, vf[2], vf[3]);
@@ -242,6 +252,25 @@ __global__ void __launch_bounds__(PR_WARPS * 32, 1)
       if (lane == 0 && more) {
         issue(next_id);
         if (more) next_id = id_of(ahead, next_j);
+      }
+    }
+    if (__any_sync(0xffffffffu, odd_v)) {
+      for (int key = max(j0, lim_min / PR_BLOCK) * PR_BLOCK;
+           key < min(j1 * PR_BLOCK, seq.end); ++key) {
+        const int id = kv.page_id(w.b, key);
+        if (id < 0) continue;
+        const T* v = static_cast<const T*>(kv.v) + (int64_t)kv.page_row(id, head, key) * PG_HD + c2;
+#pragma unroll
+        for (int n = 0; n < 16; ++n) {
+          const uint32_t x = *reinterpret_cast<const uint32_t*>(v + n * 8);
+          const float2 odd = H::unpack(x & H::not_finite(x));
+#pragma unroll
+          for (int j = 0; j < 2; ++j)
+            if (key < lim[j]) {
+              o[n][2 * j] += odd.x;
+              o[n][2 * j + 1] += odd.y;
+            }
+        }
       }
     }
     // ---- the segment's output

@@ -21,6 +21,9 @@
 // two threads per row, hide the products' latency as well, but a step costs a warp about 60
 // instructions whatever its keys: both took 2.3 us for 128 keys.
 //
+// Infinities and NaN in V of slots that not every row sees are taken out and added afterwards to
+// the rows that see them (see paged_attention.cuh).
+//
 // The work is handed out in equal shares (paged_shares.cuh), a share to a CTA; paged_join_kernel
 // joins the tiles that are cut.
 #pragma once
@@ -183,6 +186,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1)
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 18);
   int* failed = reinterpret_cast<int*>(bars + 19);
   uint32_t* absent_of = reinterpret_cast<uint32_t*>(bars + 20);  // [4] absent pages of a step
+  volatile uint32_t* odd_v = absent_of + 4;  // infinities or NaN were taken out of V
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int group = heads / kv.kv_heads;
@@ -200,6 +204,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1)
       mbar_init(&o_full[i], 1);
     }
     *failed = 0;
+    *odd_v = 0;
     fence_mbar_init();
     tma_prefetch_desc(&tmK);
     tma_prefetch_desc(&tmV);
@@ -438,16 +443,34 @@ __global__ void __launch_bounds__(PT_THREADS, 1)
             tmem_st_32x32b_x16(t_o + c * 16, o);
           }
         }
-        if (key0 + PT_KEYS > seq.end) {
-          // slots behind the sequence may hold anything, and 0 x NaN is not 0: zero their V
+        if (key0 + PT_KEYS > lim_all) {
+          // not every row sees every slot of this step: V of slots behind the sequence reads as
+          // 0, infinities and NaN of the others too (a thread per slot)
           const uint32_t g = g0 + j;
           ok = mbar_wait(&v_full[g % PT_BUFS], (g / PT_BUFS) & 1, failed);
-          uint8_t* v = smem + PT_V_OFF + (g % PT_BUFS) * PT_STEP_BYTES;
+          uint8_t* v = smem + PT_V_OFF + (g % PT_BUFS) * PT_STEP_BYTES + r * 128;
           if (r >= seq.end - key0) {
-#pragma unroll
+#pragma unroll 4
             for (int c = 0; c < 16; ++c)
-              *reinterpret_cast<uint4*>(v + (c >> 3) * 16384 + r * 128 + (c & 7) * 16) =
+              *reinterpret_cast<uint4*>(v + (c >> 3) * 16384 + ((c & 7) ^ (r & 7)) * 16) =
                   make_uint4(0, 0, 0, 0);
+          } else {
+            uint32_t any = 0;
+#pragma unroll 4
+            for (int c = 0; c < 16; ++c) {
+              const uint4 x = *reinterpret_cast<const uint4*>(  // (eight rows meet no bank twice)
+                  v + (c >> 3) * 16384 + ((c & 7) ^ (r & 7)) * 16);
+              any |= H::not_finite(x.x) | H::not_finite(x.y) | H::not_finite(x.z) | H::not_finite(x.w);
+            }
+            if (any) {
+              *odd_v = 1;  // before the values go: the other tile's warps read the same V
+              __threadfence_block();
+#pragma unroll 1
+              for (int c = 0; c < 64; ++c) {
+                uint32_t* x = reinterpret_cast<uint32_t*>(v + (c >> 5) * 16384) + (c & 31);
+                *x &= ~H::not_finite(*x);
+              }
+            }
           }
           fence_proxy_async_smem();
           __syncwarp();
@@ -489,6 +512,44 @@ __global__ void __launch_bounds__(PT_THREADS, 1)
       __syncwarp();
       if (!__all_sync(0xffffffffu, ok)) break;
       tc_fence_after();
+      if (*odd_v && n_s > 0) {
+        // O += the infinities and NaN that this row sees, of all slots that either tile may
+        // have taken them out of (added twice they are what they were). All of the warp takes
+        // part: the TMEM accesses are its.
+        const int lim_tile = seq.limit(w.tile * PT_ROWS / group);
+        for (int key = max(key_first, lim_tile / PT_KEYS * PT_KEYS);
+             key < min(w.j1 * PT_KEYS, seq.end); ++key) {
+          const int id = kv.page_id(w.b, key);
+          if (id < 0) continue;
+          const uint4* v = reinterpret_cast<const uint4*>(
+              static_cast<const T*>(kv.v) + (int64_t)kv.page_row(id, w.head, key) * PG_HD);
+#pragma unroll 1
+          for (int c = 0; c < 8; ++c) {
+            uint32_t x[8], odd = 0;
+            *reinterpret_cast<uint4*>(x) = v[c * 2];
+            *reinterpret_cast<uint4*>(x + 4) = v[c * 2 + 1];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+              x[e] &= H::not_finite(x[e]);
+              odd |= x[e];
+            }
+            if (!odd) continue;  // the same in all lanes
+            uint32_t o[16];
+            tmem_ld_32x32b_x16(t_o + c * 16, o);
+            tmem_ld_wait_regs16(o);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+              const float2 y = H::unpack(x[e]);
+              if (key < lim) {
+                o[2 * e] = __float_as_uint(__uint_as_float(o[2 * e]) + y.x);
+                o[2 * e + 1] = __float_as_uint(__uint_as_float(o[2 * e + 1]) + y.y);
+              }
+            }
+            tmem_st_32x32b_x16(t_o + c * 16, o);
+            tmem_st_wait();
+          }
+        }
+      }
       if (!w.whole()) {
         const int part = 2 * blockIdx.x + (seg == 0 ? 0 : 1);
         if (valid) parts.lse[part * PT_ROWS + s * PT_SUB + r] = row_lse;

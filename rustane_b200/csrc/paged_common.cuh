@@ -154,6 +154,11 @@ struct Half16<__half> {
   }
   static __device__ __forceinline__ uint32_t pack(float lo, float hi) { return pack_half2(lo, hi); }
   static __device__ __forceinline__ __half from(float x) { return __float2half_rn(x); }
+  // Of two packed values, 0xffff in the halves that are infinite or NaN.
+  static __device__ __forceinline__ uint32_t not_finite(uint32_t w) {
+    const uint32_t all_ones = ((w & 0x7c007c00u) + 0x04000400u) & 0x80008000u;
+    return (all_ones >> 15) * 0xffffu;
+  }
   static __device__ __forceinline__ void mma(float (&d)[4], const uint32_t (&a)[4], uint32_t b0,
                                              uint32_t b1) {
     mma_16816(d, a, b0, b1);
@@ -169,6 +174,10 @@ struct Half16<__nv_bfloat16> {
     return *reinterpret_cast<const uint32_t*>(&h);
   }
   static __device__ __forceinline__ __nv_bfloat16 from(float x) { return __float2bfloat16_rn(x); }
+  static __device__ __forceinline__ uint32_t not_finite(uint32_t w) {
+    const uint32_t all_ones = ((w & 0x7f807f80u) + 0x00800080u) & 0x80008000u;
+    return (all_ones >> 15) * 0xffffu;
+  }
   static __device__ __forceinline__ void mma(float (&d)[4], const uint32_t (&a)[4], uint32_t b0,
                                              uint32_t b1) {
     asm volatile(

@@ -446,3 +446,52 @@ def test_evict_of_a_few_slots(bridge_lib, over, budget, page):
             x[fro[0], h, fro[1]].clone() for x in (k0, w0, p0))
     assert torch.equal(c.k.view(torch.int16), k0.view(torch.int16))
     assert torch.equal(w, w0) and torch.equal(p, p0)
+
+
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("lens,news,heads,kv_heads,page", [
+    ([40], [5], 3, 1, 16),               # the 16-row kernel
+    ([300, 17], [4, 3], 4, 1, 32),
+    ([500, 130], [200, 130], 4, 2, 16),  # the tcgen05 kernel: both tiles of a CTA
+    ([3000], [300], 8, 1, 128),          # parts
+])
+def test_attention_keeps_what_a_row_does_not_see_out_of_it(bridge_lib, lens, news, heads,
+                                                           kv_heads, page, dtype):
+    """Infinities and NaN in K and V of new tokens reach the rows that see those tokens and no
+    other row."""
+    c = Cache(lens, news, heads, kv_heads, page, dtype, seed=11)
+    q = c.tokens(heads * 128, scale=1.5)
+    clean, clean_lse, tol, lse_tol = R.attention_ref(c, q, SCALE)
+    bad = []  # (sequence, slot, element, value)
+    for b in range(c.batch):
+        n, length = news[b], lens[b]
+        for k, (back, d, x) in enumerate([(0, 5, math.nan), (n // 3, 17, math.inf),
+                                          (n // 2, 90, -math.inf), (n // 2, 91, math.nan)]):
+            bad.append((b, length - 1 - back, d, x))
+    for b, slot, d, x in bad:
+        at = c.place(b, torch.tensor([slot], device="cuda"))
+        c.v[at[0], :, at[1], d] = x
+    out = torch.zeros(c.rows, heads * 128, device="cuda", dtype=c.dt)
+    lse = torch.zeros(c.rows, heads, device="cuda")
+    assert R.attention(bridge_lib, c, q, SCALE, out, lse) == 0
+    got = out[:c.starts[-1]].unflatten(1, (heads, 128))
+    want = clean.clone()
+    for b, slot, d, x in bad:
+        first = slot - (lens[b] - news[b])  # the first token that sees it
+        rows = slice(c.starts[b] + first, c.starts[b] + news[b])
+        want[rows, :, d] += x
+    odd = ~torch.isfinite(want)
+    assert bool((torch.isnan(got) == torch.isnan(want)).all())
+    assert bool((got[odd & ~torch.isnan(want)].double() == want[odd & ~torch.isnan(want)]).all())
+    close(torch.where(odd, 0.0, got.double()), torch.where(odd, 0.0, want), tol, "out")
+    close(lse[:c.starts[-1]], clean_lse, lse_tol, "lse")
+    # K of the last token: only its own row sees it
+    c.v[:] = torch.nan_to_num(c.v, 0.0, 0.0, 0.0)
+    for b in range(c.batch):
+        at = c.place(b, torch.tensor([lens[b] - 1], device="cuda"))
+        c.k[at[0], :, at[1]] = math.nan
+    assert R.attention(bridge_lib, c, q, SCALE, out, lse) == 0
+    last = [c.starts[b + 1] - 1 for b in range(c.batch)]
+    others = [r for r in range(c.starts[-1]) if r not in last]
+    assert bool(out[last].isnan().all()) and not bool(out[others].isnan().any())
+    assert not bool(lse[others].isnan().any())
