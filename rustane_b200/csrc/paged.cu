@@ -168,9 +168,22 @@ bool make_cache_map(CUtensorMap* map, const void* ptr, const cb_paged_kv* kv, ui
 int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
 // ------------------------------------------------------------------- attention plan
+// Bounds of a step's work in tiles of `rows` query rows and steps of `keys` slots (the device
+// knows how much there is): no more tiles than the rows need with one ragged tile per sequence,
+// and no more than batch x those of the longest.
+double step_bound(const cb_paged_kv* kv, int group, int rows, int keys) {
+  const int64_t tiles =
+      std::min<int64_t>(kv->batch * ceil_div((int64_t)kv->max_new * group, rows),
+                        ceil_div((int64_t)kv->rows * group, rows) + kv->batch);
+  return (double)tiles * kv->kv_heads * ceil_div(kv->max_len, keys);
+}
+// Shares count units of 32 bits: every step, and up to three for each tile (which has a step).
+bool shares_ok(double steps) { return steps * 4 < (double)INT_LIMIT; }
+
 struct AttentionPlan {
   bool tc;          // the tcgen05 kernel, else the 16-row one
-  int ctas;         // one per SM, or as many as there can be shares of work
+  double steps;     // at most
+  int ctas;         // one per SM, or as many as there can be steps
   size_t workers;   // with a share each
   size_t rows;      // query rows of a tile: of a part
   size_t bytes() const {
@@ -183,13 +196,8 @@ AttentionPlan plan_attention(const cb_paged_kv* kv, int32_t heads) {
   const int group = heads / kv->kv_heads;
   p.tc = (int64_t)kv->max_new * group > PR_ROWS;
   p.rows = p.tc ? PT_ROWS : PR_ROWS;
-  // An upper bound of the tiles (the device knows how many there are): no more than the rows
-  // need with one ragged tile per sequence, and no more than batch x the tiles of the longest.
-  const int64_t tiles = std::min<int64_t>(
-      kv->batch * ceil_div((int64_t)kv->max_new * group, p.rows),
-      ceil_div((int64_t)kv->rows * group, p.rows) + kv->batch);
-  const double steps = (double)tiles * kv->kv_heads * ceil_div(kv->max_len, p.tc ? PT_KEYS : PR_BLOCK);
-  p.ctas = (int)std::max(1.0, std::min<double>(PG_SMS, steps));
+  p.steps = step_bound(kv, group, (int)p.rows, p.tc ? PT_KEYS : PR_BLOCK);
+  p.ctas = (int)std::max(1.0, std::min<double>(PG_SMS, p.steps));
   p.workers = (size_t)p.ctas * (p.tc ? 1 : PR_WARPS);
   return p;
 }
@@ -216,6 +224,7 @@ cb_status launch_attention(const cb_paged_kv* kv, const T* q, int64_t q_stride, 
                            float scale, T* out, int64_t out_stride, float* lse, float* workspace,
                            cudaStream_t st) {
   const AttentionPlan p = plan_attention(kv, heads);
+  if (!shares_ok(p.steps)) return CB_ERR_UNSUPPORTED;
   const int box = p.tc ? std::min(kv->page_size, PT_KEYS) : PR_BLOCK;
   const int group = heads / kv->kv_heads;
   CUtensorMap tk, tv;
@@ -271,7 +280,8 @@ cb_status launch_weights(const cb_paged_kv* kv, const T* q, int64_t q_stride, in
   const float scale_log2 = scale * 1.4426950408889634f;
   if ((int64_t)kv->max_new * group <= PR_ROWS) {
     // two CTAs per SM; no more than there are blocks of slots
-    const double blocks = (double)kv->batch * kv->kv_heads * ceil_div(kv->max_len, PR_BLOCK);
+    const double blocks = step_bound(kv, group, PR_ROWS, PR_BLOCK);
+    if (!shares_ok(blocks)) return CB_ERR_UNSUPPORTED;
     const int ctas = (int)std::max(1.0, std::min(2.0 * PG_SMS, blocks));
     paged_weights_kernel<T><<<ctas, PW_WARPS * 32, 0, st>>>(d, q, q_stride, heads, scale_log2, lse,
                                                            weights);

@@ -150,9 +150,10 @@ __device__ __forceinline__ int pt_step_id(const PagedKV& kv, int b, int key0, in
   return (lane >> 1) * box_rows < KEYS && key < end ? kv.page_id(b, key) : -1;
 }
 
-// A tile counts two steps for its Q, its pipeline's start and its output (a step takes
-// 1.9 us, a tile 4 to 5 us beside its steps).
-using PtShares = PagedShares<PT_ROWS, PT_KEYS, 2, 4>;
+// A tile counts three steps for its Q, its pipeline's start and its output (a step takes 1.9 us,
+// a tile 4 to 6 us beside its steps; ragged prompts: 58.6 us with two, 51.6 with three, 53.8
+// with four).
+using PtShares = PagedShares<PT_ROWS, PT_KEYS, 3, 5>;
 
 struct PtShared {  // at PT_SHARE_OFF
   PtShares::Walk walk[PT_THREADS / 32];  // every warp's (registers are for the scores)
@@ -525,9 +526,8 @@ __global__ void __launch_bounds__(PT_THREADS, 1)
               static_cast<const T*>(kv.v) + (int64_t)kv.page_row(id, w.head, key) * PG_HD);
 #pragma unroll 1
           for (int c = 0; c < 8; ++c) {
-            uint32_t x[8], odd = 0;
-            *reinterpret_cast<uint4*>(x) = v[c * 2];
-            *reinterpret_cast<uint4*>(x + 4) = v[c * 2 + 1];
+            const uint4 x0 = v[c * 2], x1 = v[c * 2 + 1];
+            uint32_t x[8] = {x0.x, x0.y, x0.z, x0.w, x1.x, x1.y, x1.z, x1.w}, odd = 0;
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
               x[e] &= H::not_finite(x[e]);

@@ -6,6 +6,7 @@
 // own cost, are laid end to end, and every worker takes an equal share of these units. A
 // worker that has all steps of a tile writes its output; of a tile that is cut, each worker
 // writes its part (at most two: its first and its last tile), and a second kernel joins them.
+// Units are counted in 32 bits (the host refuses steps that could have 2^31 of them).
 #pragma once
 #include "paged_common.cuh"
 
@@ -30,9 +31,16 @@ __device__ __forceinline__ int share_part(const ShareJoin& jn, int worker, int p
 }
 
 struct ShareTable {  // in shared memory
-  int64_t seq_units[SHARE_CHUNK];
-  int64_t total;  // units of all tiles and key heads
-  int workers;    // that have a share
+  uint32_t seq_units[SHARE_CHUNK];
+  uint32_t base, longer;  // the first `longer` workers have base + 1 units, the others base
+
+  __device__ __forceinline__ uint32_t begin_of(uint32_t worker) const {
+    return base * worker + min(worker, longer);
+  }
+  __device__ __forceinline__ uint32_t worker_of(uint32_t unit) const {
+    const uint32_t border = (base + 1) * longer;
+    return unit < border ? unit / (base + 1) : longer + (unit - border) / base;
+  }
 };
 
 // LEAST: units of a share at least; above UNITS, so that every share has a step.
@@ -56,10 +64,10 @@ struct PagedShares {
     int b, head, tile;
     int u0;             // the segment's first unit within the tile
     int j0, j1, steps;  // the segment: steps j0 .. j1 - 1 of the tile's `steps`
-    int64_t at, end;    // the segment's first unit among all, and the share's end
+    uint32_t at, end;   // the segment's first unit among all, and the share's end
 
     __device__ __forceinline__ int u1() const {
-      return (int)min((int64_t)(steps + UNITS), u0 + (end - at));
+      return min(steps + UNITS, u0 + (int)(end - at));
     }
     __device__ __forceinline__ void segment(int group) {
       steps = tile_steps(seq, group, tile);
@@ -69,7 +77,7 @@ struct PagedShares {
     // The next segment; false when the share is done.
     __device__ __forceinline__ bool next(const PagedKV& kv, int group) {
       do {
-        at += u1() - u0;
+        at += (uint32_t)(u1() - u0);
         if (at >= end) return false;
         u0 = 0;
         if (++tile >= tiles(seq, group)) {
@@ -93,9 +101,8 @@ struct PagedShares {
     // The join record of a segment that begins its tile and does not end it.
     __device__ __forceinline__ ShareJoin join(const ShareTable& table, int worker, int part,
                                               int group) const {
-      const int64_t last_unit = at - u0 + UNITS + steps - 1;
       ShareJoin jn;
-      jn.count = (int)(((last_unit + 1) * table.workers - 1) / table.total) - worker + 1;
+      jn.count = (int)table.worker_of(at - u0 + UNITS + steps - 1) - worker + 1;
       jn.first = part;
       jn.row0 = seq.row0;
       jn.head = head;
@@ -120,66 +127,52 @@ struct PagedShares {
         for (int i = warp; i < count; i += warps) {
           const PagedSeq s = paged_seq(kv, base + i);
           const int n_tiles = tiles(s, group);
-          int64_t n = 0;
+          uint32_t n = 0;
           for (int t = lane; t < n_tiles; t += 32) n += tile_steps(s, group, t) + UNITS;
-#pragma unroll
-          for (int off = 16; off > 0; off >>= 1) n += __shfl_xor_sync(0xffffffffu, n, off);
+          n = __reduce_add_sync(0xffffffffu, n);
           if (lane == 0) table.seq_units[i] = n;
         }
       } else {
         for (int i = threadIdx.x; i < count; i += blockDim.x) {
           const PagedSeq s = paged_seq(kv, base + i);
           const int n_tiles = tiles(s, group);
-          int64_t n = 0;
+          uint32_t n = 0;
           for (int t = 0; t < n_tiles; ++t) n += tile_steps(s, group, t) + UNITS;
           table.seq_units[i] = n;
         }
       }
       __syncthreads();
     };
-    // The sequence of a chunk that holds unit `want` and the units of it before that, or -1
-    // and the units so far.
-    auto scan = [&](int count, int64_t before, int64_t want, int64_t& inside) -> int {
-      for (int i = 0; i < count; i += 32) {
-        const int64_t n = i + lane < count ? table.seq_units[i + lane] : 0;
-        int64_t incl = n;
+    auto inclusive = [&](uint32_t n) {
 #pragma unroll
-        for (int off = 1; off < 32; off <<= 1) {
-          const int64_t up = __shfl_up_sync(0xffffffffu, incl, off);
-          if (lane >= off) incl += up;
-        }
-        const unsigned past = __ballot_sync(0xffffffffu, before + incl > want);
-        if (past) {
-          const int src = __ffs(past) - 1;
-          inside = want - before - __shfl_sync(0xffffffffu, incl - n, src);
-          return i + src;
-        }
-        before += __shfl_sync(0xffffffffu, incl, 31);
+      for (int off = 1; off < 32; off <<= 1) {
+        const uint32_t up = __shfl_up_sync(0xffffffffu, n, off);
+        if (lane >= off) n += up;
       }
-      inside = before;
-      return -1;
+      return n;
     };
-    int64_t total = 0;
+    uint32_t total = 0;  // of one key head
     for (int base = 0; base < kv.batch; base += SHARE_CHUNK) {
       const int count = min(SHARE_CHUNK, kv.batch - base);
       __syncthreads();
       add_up(base, count);
-      int64_t inside;
-      scan(count, total, INT64_MAX, inside);
-      total = inside;
+      uint32_t n = 0;
+      for (int i = lane; i < count; i += 32) n += table.seq_units[i];
+      total += __reduce_add_sync(0xffffffffu, n);
     }
-    const int64_t all = total * kv.kv_heads;
-    const int workers = (int)max((int64_t)1, min((int64_t)most, all / LEAST));
-    const int64_t lo = worker < workers ? all * worker / workers : all;
-    const int64_t hi = worker < workers ? all * (worker + 1) / workers : all;
+    const uint32_t all = total * kv.kv_heads;
+    const uint32_t workers = max(1u, min((uint32_t)most, all / LEAST));
     if (threadIdx.x == 0) {
-      table.total = all;
-      table.workers = workers;
+      table.base = all / workers;
+      table.longer = all - all / workers * workers;
     }
+    __syncthreads();
+    const uint32_t lo = (uint32_t)worker < workers ? table.begin_of(worker) : all;
+    const uint32_t hi = (uint32_t)worker < workers ? table.begin_of(worker + 1) : all;
     // heads of one sequence lie side by side: unit lo lies in the sequence that holds unit
     // lo / kv_heads of one head
-    const int64_t want = lo / kv.kv_heads;
-    int64_t before = 0;
+    const uint32_t want = lo / kv.kv_heads;
+    uint32_t before = 0;  // units of one head of the sequences in front
     bool found = lo >= hi;
     for (int base = 0; base < kv.batch; base += SHARE_CHUNK) {
       const int count = min(SHARE_CHUNK, kv.batch - base);
@@ -187,33 +180,34 @@ struct PagedShares {
         __syncthreads();
         add_up(base, count);
       }
-      int64_t inside;
-      const int i = found ? -1 : scan(count, before, want, inside);
-      if (i >= 0) {
+      for (int i0 = 0; i0 < count && !found; i0 += 32) {
+        const uint32_t n = i0 + lane < count ? table.seq_units[i0 + lane] : 0;
+        const uint32_t incl = inclusive(n);
+        const unsigned past = __ballot_sync(0xffffffffu, before + incl > want);
+        if (!past) {
+          before += __shfl_sync(0xffffffffu, incl, 31);
+          continue;
+        }
         found = true;
-        const int64_t one = table.seq_units[i];
-        int64_t r = lo - (want - inside) * kv.kv_heads;  // within the sequence
-        const int head = (int)(r / one);
+        const int src = __ffs(past) - 1, b = base + i0 + src;
+        const uint32_t one = __shfl_sync(0xffffffffu, n, src);
+        uint32_t r = lo - (before + __shfl_sync(0xffffffffu, incl - n, src)) * kv.kv_heads;
+        const uint32_t head = r / one;
         r -= head * one;
-        const PagedSeq s = paged_seq(kv, base + i);
+        const PagedSeq s = paged_seq(kv, b);
         const int n_tiles = tiles(s, group);
-        int64_t run = 0;
+        uint32_t run = 0;
         for (int t0 = 0; t0 < n_tiles; t0 += 32) {
-          const int n = t0 + lane < n_tiles ? tile_steps(s, group, t0 + lane) + UNITS : 0;
-          int64_t incl = n;
-#pragma unroll
-          for (int off = 1; off < 32; off <<= 1) {
-            const int64_t up = __shfl_up_sync(0xffffffffu, incl, off);
-            if (lane >= off) incl += up;
-          }
-          const unsigned past = __ballot_sync(0xffffffffu, run + incl > r);
-          if (past) {
-            if (lane == __ffs(past) - 1) {
+          const uint32_t m = t0 + lane < n_tiles ? tile_steps(s, group, t0 + lane) + UNITS : 0;
+          const uint32_t sum = inclusive(m);
+          const unsigned in = __ballot_sync(0xffffffffu, run + sum > r);
+          if (in) {
+            if (lane == __ffs(in) - 1) {
               walk.seq = s;
-              walk.b = base + i;
-              walk.head = head;
+              walk.b = b;
+              walk.head = (int)head;
               walk.tile = t0 + lane;
-              walk.u0 = (int)(r - run - (incl - n));
+              walk.u0 = (int)(r - run - (sum - m));
               walk.at = lo;
               walk.end = hi;
               walk.segment(group);
@@ -221,10 +215,8 @@ struct PagedShares {
             }
             break;
           }
-          run += __shfl_sync(0xffffffffu, incl, 31);
+          run += __shfl_sync(0xffffffffu, sum, 31);
         }
-      } else if (!found) {
-        before = inside;
       }
     }
     __syncthreads();
