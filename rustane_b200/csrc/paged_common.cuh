@@ -101,12 +101,17 @@ __device__ __forceinline__ void pdl_wait() {
 
 // 2^x of two numbers on the FMA pipes, for kernels whose exponentials keep the MUFU busy
 // (16 results a clock and SM). x = n + f with n the nearest whole number: 2^f on [-1/2, 1/2] by
-// the polynomial of degree DEG with the least largest relative error (Remez's exchange; degree
-// 4: 2.6e-6, degree 5: 2.6e-7, ex2.approx: 2.4e-7), times 2^n built in the exponent field.
-// Results below 2^-126 are 0, as ex2.approx.ftz's; NaN stays NaN. x <= 127.
+// the polynomial of degree 5 with the least largest relative error (Remez's exchange: 2.6e-7,
+// ex2.approx has 2.4e-7), times 2^n built in the exponent field.
+// Results below 2^-126 are 0, as ex2.approx.ftz's, from 2^128 on infinite; NaN stays NaN.
 __device__ __forceinline__ float max_nan(float a, float b) {
   float r;
   asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ float min_nan(float a, float b) {
+  float r;
+  asm("min.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
   return r;
 }
 __device__ __forceinline__ float2 fmul2(float2 a, float2 b) {
@@ -116,29 +121,20 @@ __device__ __forceinline__ float2 fmul2(float2 a, float2 b) {
       : "l"(*reinterpret_cast<uint64_t*>(&a)), "l"(*reinterpret_cast<uint64_t*>(&b)));
   return *reinterpret_cast<float2*>(&r);
 }
-template <int DEG>
 __device__ __forceinline__ float2 exp2_poly2(float2 x) {
-  static_assert(DEG == 4 || DEG == 5, "degree");
   constexpr float MAGIC = 12582912.0f;  // 1.5 x 2^23: adding it rounds to a whole number
-  x.x = max_nan(x.x, -127.0f);  // n = -127 makes an exponent field of 0: exactly 0
-  x.y = max_nan(x.y, -127.0f);
+  // n = -127 makes an exponent field of 0, exactly 0, and n = 128 one of 255, infinity
+  x.x = min_nan(max_nan(x.x, -127.0f), 128.0f);
+  x.y = min_nan(max_nan(x.y, -127.0f), 128.0f);
   const float2 t = fadd2(x, make_float2(MAGIC, MAGIC));
   const float2 n = fadd2(t, make_float2(-MAGIC, -MAGIC));
   const float2 f = ffma2(n, make_float2(-1.0f, -1.0f), x);
   auto both = [](float c) { return make_float2(c, c); };
-  float2 p;
-  if constexpr (DEG == 5) {
-    p = ffma2(both(1.301088603e-03f), f, both(9.678628296e-03f));
-    p = ffma2(p, f, both(5.551895499e-02f));
-    p = ffma2(p, f, both(2.402208745e-01f));
-    p = ffma2(p, f, both(6.931457520e-01f));
-    p = ffma2(p, f, both(1.0f));
-  } else {
-    p = ffma2(both(9.570102207e-03f), f, both(5.591785908e-02f));
-    p = ffma2(p, f, both(2.402474433e-01f));
-    p = ffma2(p, f, both(6.931217909e-01f));
-    p = ffma2(p, f, both(9.999992847e-01f));
-  }
+  float2 p = ffma2(both(1.301088603e-03f), f, both(9.678628296e-03f));
+  p = ffma2(p, f, both(5.551895499e-02f));
+  p = ffma2(p, f, both(2.402208745e-01f));
+  p = ffma2(p, f, both(6.931457520e-01f));
+  p = ffma2(p, f, both(1.0f));
   const float2 scale = make_float2(__uint_as_float((__float_as_uint(t.x) << 23) + 0x3f800000u),
                                    __uint_as_float((__float_as_uint(t.y) << 23) + 0x3f800000u));
   return fmul2(p, scale);

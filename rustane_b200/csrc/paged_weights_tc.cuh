@@ -249,7 +249,7 @@ __global__ void __launch_bounds__(WT_THREADS, 1)
             a.x = exp2_mufu(a.x);
             a.y = exp2_mufu(a.y);
             if (e % 8 == 0) {  // a quarter of the exponentials on the FMA pipes
-              d = exp2_poly2<5>(d);
+              d = exp2_poly2(d);
             } else {
               d.x = exp2_mufu(d.x);
               d.y = exp2_mufu(d.y);

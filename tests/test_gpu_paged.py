@@ -495,3 +495,307 @@ def test_attention_keeps_what_a_row_does_not_see_out_of_it(bridge_lib, lens, new
     others = [r for r in range(c.starts[-1]) if r not in last]
     assert bool(out[last].isnan().all()) and not bool(out[others].isnan().any())
     assert not bool(lse[others].isnan().any())
+
+
+# ------------------------------------------------------------------ how they are called
+def test_more_sequences_than_are_added_up_at_a_time(bridge_lib):
+    lens = [1 + (i * 37) % 50 for i in range(2500)]
+    for news, heads in (([1] * 2500, 2), ([min(n, 1 + i % 20) for i, n in enumerate(lens)], 2)):
+        c = Cache(lens, news, heads, 1, 16, "f16", seed=heads)
+        q = c.tokens(heads * 128)
+        out = torch.zeros(c.rows, heads * 128, device="cuda", dtype=c.dt)
+        lse = torch.zeros(c.rows, heads, device="cuda")
+        assert R.attention(bridge_lib, c, q, SCALE, out, lse) == 0
+        want, want_lse, tol, lse_tol = R.attention_ref(c, q, SCALE)
+        close(out[:c.starts[-1]].unflatten(1, (heads, 128)), want, tol, "out")
+        w = torch.zeros(c.pages, 1, 16, device="cuda")
+        d = c.desc()
+        assert bridge_lib.cb_paged_attention_weights(C.byref(d), ptr(q), q.stride(0), heads, SCALE,
+                                                     ptr(lse), ptr(w), stream()) == 0
+        want_w, tol_w = R.weights_ref(c, q, SCALE, lse, torch.zeros_like(w))
+        torch.cuda.synchronize()
+        close(w, want_w, tol_w, "weights")
+
+
+@pytest.mark.parametrize("new", [1, 60])
+def test_a_cache_of_more_than_2_to_the_31_elements(bridge_lib, new):
+    """Every page in use lies behind element 2^31 of its array."""
+    page, kv_heads = 64, 2
+    pages = 2 ** 31 // (page * kv_heads * 128) + 100
+    c = Cache([200], [new], 4, kv_heads, page, "f16", seed=3)
+    far = torch.tensor([[pages - 5, pages - 1, pages - 17, pages - 3]], device="cuda", dtype=torch.int32)
+    small_k, small_v = c.k, c.v
+    c.k = torch.zeros(pages, kv_heads, page, 128, device="cuda", dtype=c.dt)
+    c.v = torch.zeros_like(c.k)
+    c.k[far[0].long()], c.v[far[0].long()] = small_k[c.page_lists[0]], small_v[c.page_lists[0]]
+    c.table, c.page_lists, c.pages = far, [far[0].tolist()], pages
+    q = c.tokens(512)
+    out = torch.zeros(c.rows, 512, device="cuda", dtype=c.dt)
+    lse = torch.zeros(c.rows, 4, device="cuda")
+    assert R.attention(bridge_lib, c, q, SCALE, out, lse) == 0
+    want, want_lse, tol, lse_tol = R.attention_ref(c, q, SCALE)
+    close(out[:new].unflatten(1, (4, 128)), want, tol, "out")
+    d = c.desc()
+    w = torch.zeros(pages, kv_heads, page, device="cuda")
+    assert bridge_lib.cb_paged_attention_weights(C.byref(d), ptr(q), q.stride(0), 4, SCALE, ptr(lse),
+                                                 ptr(w), stream()) == 0
+    torch.cuda.synchronize()
+    # every query row and head hands out a weight of one
+    assert abs(float(w.double().sum()) - new * 4) < 1e-3 * new
+    assert float(w[:pages - 20].abs().max()) == 0.0
+    nk, nv = c.tokens(256), c.tokens(256)
+    assert _append(bridge_lib, c, None, None, None, nk, nv, heads=0) == 0
+    p = torch.arange(64, device="cuda", dtype=torch.int32).expand(pages, kv_heads, page).contiguous()
+    lo = torch.zeros_like(c.len)
+    assert _evict(bridge_lib, c, w, w, p, p, c.len, 100, 0, 0, lo) == 0
+    at = c.place(0, torch.arange(200 - new, 200, device="cuda"))
+    kept = at[0] * 0 + torch.arange(200 - new, 200, device="cuda") >= 100  # (others may be holes)
+    assert torch.equal(c.v[at[0][kept], 1, at[1][kept]], nv[:new, 128:][kept])
+
+
+def test_sequences_may_share_pages_for_attention(bridge_lib):
+    """Two sequences with the same first pages; the weights of those collect from both."""
+    c = Cache([70, 90], [1, 9], 4, 2, 16, "f16", seed=8)
+    c.table[1, :3] = c.table[0, :3]
+    c.page_lists[1][:3] = c.page_lists[0][:3]
+    q = c.tokens(512)
+    out = torch.zeros(c.rows, 512, device="cuda", dtype=c.dt)
+    lse = torch.zeros(c.rows, 4, device="cuda")
+    assert R.attention(bridge_lib, c, q, SCALE, out, lse) == 0
+    want, _, tol, _ = R.attention_ref(c, q, SCALE)
+    close(out[:10].unflatten(1, (4, 128)), want, tol)
+    d = c.desc()
+    w = torch.zeros(c.pages, 2, 16, device="cuda")
+    assert bridge_lib.cb_paged_attention_weights(C.byref(d), ptr(q), q.stride(0), 4, SCALE, ptr(lse),
+                                                 ptr(w), stream()) == 0
+    want_w, tol_w = R.weights_ref(c, q, SCALE, lse, torch.zeros_like(w))
+    torch.cuda.synchronize()
+    close(w, want_w, tol_w + 2.0 ** -23 * want_w)
+
+
+@pytest.mark.parametrize("seq,heads", [(512, 12), (320, 3)])
+def test_a_prompt_through_pages_is_the_dense_attention(bridge_lib, seq, heads):
+    """A whole prompt through the pages against the model's own attention kernel."""
+    c = Cache([seq, seq], [seq, seq], heads, heads, 16, "f16", seed=1, pad=0)
+    q = c.tokens(heads * 128)
+    out = torch.zeros(c.rows, heads * 128, device="cuda", dtype=c.dt)
+    assert R.attention(bridge_lib, c, q, SCALE, out) == 0
+    dense = [q.view(2, seq, heads, 128).transpose(1, 2).contiguous()]
+    for pool in (c.k, c.v):
+        dense.append(torch.stack([torch.stack([c.slots(pool, b, h) for h in range(heads)])
+                                  for b in range(2)]).contiguous())
+    want = torch.empty_like(out)
+    assert bridge_lib.cb_attention_f16(*(ptr(x) for x in dense), ptr(want), 2, heads, seq, stream()) == 0
+    torch.cuda.synchronize()
+    # both round their weights and their output to fp16
+    _, _, tol, _ = R.attention_ref(c, q, SCALE)
+    close(out, want, 2 * tol.flatten(1))
+
+
+def test_pointers_that_are_not_device_memory_are_refused(bridge_lib):
+    c = Cache([40], [2], 2, 1, 16, "f16")
+    q = c.tokens(256)
+    out = torch.zeros(c.rows, 256, device="cuda", dtype=c.dt)
+    host = torch.zeros(c.rows, 256, dtype=c.dt)
+    pinned = torch.zeros(c.rows, 256, dtype=c.dt).pin_memory()
+    for bad in (host, pinned):
+        assert R.attention(bridge_lib, c, bad, SCALE, out) == B.CB_ERR_INVALID_ARG
+        assert R.attention(bridge_lib, c, q, SCALE, bad) == B.CB_ERR_INVALID_ARG
+    d = c.desc()
+    table = c.table.cpu()
+    d.table = table.data_ptr()
+    inv, amp = _inv(128)
+    rope = B.cb_rope_config(inv.data_ptr(), 128, B.CB_ROPE_HALF, amp)
+    k = c.tokens(128)
+    assert bridge_lib.cb_paged_append(C.byref(d), C.byref(rope), 2, ptr(q), 256, ptr(out), 256, ptr(k),
+                                      128, ptr(k), 128, None, None, None, stream()) == B.CB_ERR_INVALID_ARG
+    inv_host = inv.cpu()
+    cfg = B.cb_rope_config(inv_host.data_ptr(), 128, B.CB_ROPE_HALF, amp)
+    pos = torch.zeros(c.rows, device="cuda", dtype=torch.int32)
+    assert bridge_lib.cb_rope(C.byref(cfg), B.CB_DTYPE_F16, ptr(q), 256, ptr(out), 256, ptr(pos), 2,
+                              2, 128, 0, stream()) == B.CB_ERR_INVALID_ARG
+
+
+def test_calls_on_two_streams_at_once(bridge_lib):
+    """Two caches, streams and workspaces; the same results as one after the other."""
+    sides = []
+    for seed, (lens, news) in enumerate([([3000, 40], [200, 1]), ([5000, 700], [1, 1])]):
+        c = Cache(lens, news, 8, 2, 32, "bf16", seed=seed)
+        q = c.tokens(1024)
+        alone = torch.zeros(c.rows, 1024, device="cuda", dtype=c.dt)
+        assert R.attention(bridge_lib, c, q, SCALE, alone) == 0
+        size, d = C.c_size_t(), c.desc()
+        assert bridge_lib.cb_paged_attention_workspace(C.byref(d), 8, C.byref(size)) == 0
+        sides.append((c, q, alone, d, torch.empty(size.value, dtype=torch.uint8, device="cuda"),
+                      torch.cuda.Stream(), torch.zeros_like(alone)))
+    torch.cuda.synchronize()
+    for _ in range(20):
+        for c, q, alone, d, ws, st, out in sides:
+            assert bridge_lib.cb_paged_attention(C.byref(d), ptr(q), q.stride(0), 8, SCALE, ptr(out),
+                                                 out.stride(0), None, ptr(ws), ws.numel(),
+                                                 C.c_void_p(st.cuda_stream)) == 0
+    torch.cuda.synchronize()
+    for c, q, alone, d, ws, st, out in sides:
+        assert torch.equal(out, alone)
+
+
+class Serving:
+    """One layer of a decode loop through all of the operators: dense 64-bit bookkeeping beside
+    the calls, so that every step can be checked."""
+
+    def __init__(self, lib, lens, heads, kv_heads, page, budget, dtype, seed):
+        self.lib, self.budget = lib, budget
+        self.sinks, self.recent = 2, budget // 4
+        dev = "cuda"
+        self.c = c = Cache([budget + 8] * len(lens), [1] * len(lens), heads, kv_heads, page, dtype,
+                           seed=seed, pad=2)
+        c.k.zero_(), c.v.zero_()
+        self.real = list(lens)
+        self.next = torch.tensor(lens, dtype=torch.int32, device=dev)  # position of the next token
+        shape = (c.pages, kv_heads, page)
+        self.w = torch.zeros(shape, device=dev)
+        self.pos = torch.zeros(shape, dtype=torch.int32, device=dev)
+        self.inv, self.amp = _inv(128, 3)
+        self.rope = B.cb_rope_config(self.inv.data_ptr(), 128, B.CB_ROPE_INTERLEAVED, self.amp)
+        g = kv_heads * 128
+        self.qkv = c.tokens(heads * 128 + 2 * g)
+        self.q, self.k, self.v = self.qkv.split([heads * 128, g, g], 1)
+        self.row_pos = torch.zeros(c.rows, dtype=torch.int32, device=dev)
+        self.q_out = torch.zeros(c.rows, heads * 128, device=dev, dtype=c.dt)
+        self.out = torch.zeros_like(self.q_out)
+        self.lse = torch.zeros(c.rows, heads, device=dev)
+        self.len_after = torch.zeros_like(c.len)
+        c.len.copy_(torch.tensor(lens, dtype=torch.int32))
+        for b, n in enumerate(lens):  # a cached prefix, its tokens at positions 0 .. n - 1
+            at = c.place(b, torch.arange(n, device=dev))
+            for h in range(kv_heads):
+                c.k[at[0], h, at[1]] = torch.randn(n, 128, device=dev, generator=c.gen).to(c.dt)
+                c.v[at[0], h, at[1]] = torch.randn(n, 128, device=dev, generator=c.gen).to(c.dt)
+                self.w[at[0], h, at[1]] = torch.rand(n, device=dev, generator=c.gen)
+                self.pos[at[0], h, at[1]] = torch.arange(n, device=dev).int()
+        self.d = c.desc()
+        size = C.c_size_t()
+        assert lib.cb_paged_attention_workspace(C.byref(self.d), heads, C.byref(size)) == 0
+        self.ws = torch.empty(size.value, dtype=torch.uint8, device=dev)
+        assert lib.cb_paged_evict_workspace(C.byref(self.d), budget, C.byref(size)) == 0
+        self.evict_ws = torch.empty(size.value, dtype=torch.uint8, device=dev)
+
+    def step(self):
+        """Everything of a step is on the device: it can be captured and replayed."""
+        c, lib, d = self.c, self.lib, C.byref(self.d)
+        st = stream()
+        c.len += 1  # the new token's slot
+        self.row_pos[:c.batch] = self.next
+        assert lib.cb_paged_append(d, C.byref(self.rope), c.heads, ptr(self.q), self.q.stride(0),
+                                   ptr(self.q_out), self.q_out.stride(0), ptr(self.k),
+                                   self.k.stride(0), ptr(self.v), self.v.stride(0),
+                                   ptr(self.row_pos), ptr(self.w), ptr(self.pos), st) == 0
+        assert lib.cb_paged_attention(d, ptr(self.q_out), self.q_out.stride(0), c.heads, SCALE,
+                                      ptr(self.out), self.out.stride(0), ptr(self.lse), ptr(self.ws),
+                                      self.ws.numel(), st) == 0
+        assert lib.cb_paged_attention_weights(d, ptr(self.q_out), self.q_out.stride(0), c.heads,
+                                              SCALE, ptr(self.lse), ptr(self.w), st) == 0
+        self.next += 1
+        assert lib.cb_paged_evict(d, ptr(self.w), ptr(self.w), ptr(self.pos), ptr(self.pos),
+                                  ptr(self.next), self.budget, self.sinks, self.recent,
+                                  ptr(self.len_after), ptr(self.evict_ws), self.evict_ws.numel(),
+                                  st) == 0
+        c.len.copy_(self.len_after)
+
+    def expect(self):
+        """The same step in 64 bits, from the state before it: the attention's output with its
+        bounds, the new weights with theirs, and the lengths."""
+        c = self.c
+        lens = [n + 1 for n in self.real]
+        ref = Cache.__new__(Cache)
+        ref.__dict__.update(c.__dict__, lens=lens, k=c.k.clone(), v=c.v.clone())
+        pos = self.next[:c.batch]
+
+        def turned(x, h):
+            return R.rotate_ref(x[:c.batch].unflatten(1, (h, 128)), pos, self.inv, self.amp,
+                                "interleaved", 128)[0].to(c.dt)
+        q, k = turned(self.q, c.heads), turned(self.k, c.kv_heads)
+        v = self.v[:c.batch].unflatten(1, (c.kv_heads, 128))
+        w = self.w.clone()
+        for b in range(c.batch):
+            at = ref.place(b, torch.tensor([lens[b] - 1], device="cuda"))
+            ref.k[at[0], :, at[1]], ref.v[at[0], :, at[1]] = k[b], v[b]
+            w[at[0], :, at[1]] = 0.0
+        q = torch.cat([q.flatten(1), q.flatten(1)[:1].expand(c.rows - c.batch, -1)])
+        out, lse, tol, lse_tol = R.attention_ref(ref, q, SCALE)
+        weights, w_tol = R.weights_ref(ref, q, SCALE, lse, w)
+        return out, tol, weights, w_tol, lens
+
+
+def _check_serving(s, steps, advance):
+    c = s.c
+    for i in range(steps):
+        s.qkv[:c.batch] = torch.randn(c.batch, s.qkv.shape[1], device="cuda", generator=c.gen).to(c.dt)
+        out, tol, weights, w_tol, lens = s.expect()
+        advance()
+        torch.cuda.synchronize()
+        # q and k rotated to the type by the operator may differ from the 64-bit ones by a step
+        # of the type, which moves a score by that much of the sum of its terms' magnitudes
+        step = torch.finfo(c.dt).eps
+        slack = 2 * step * SCALE * 128 * 3
+        got = s.out[:c.batch].unflatten(1, (c.heads, 128))
+        close(got, out, tol + slack * tol / (step / 2), f"step {i}: out")
+        s.real = [min(n, s.budget) for n in lens]
+        assert c.len.tolist() == s.real
+        for b in range(c.batch):
+            for h in range(c.kv_heads):
+                full = Cache.__new__(Cache)
+                full.__dict__.update(c.__dict__, lens=lens)
+                before = full.slots(weights, b, h)
+                bound = (full.slots(w_tol, b, h) + slack * before.abs()).max()
+                full.lens = s.real
+                after = full.slots(s.w, b, h).double()
+                positions = full.slots(s.pos, b, h)
+                # no position twice, the sinks and the newest are there
+                assert positions.unique().numel() == s.real[b]
+                nxt = int(s.next[b])
+                must = set(range(s.sinks)) | set(range(nxt - s.recent, nxt))
+                assert must <= set(positions.tolist())
+                # what stays has the largest weights: the sorted sums of what is left are the
+                # largest of before, but for the ones that had to stay
+                assert float(after.sum()) <= float(before.sum() + bound * len(before))
+                if lens[b] > s.budget:
+                    gone = float(before.sum() - after.sum())
+                    free = after[(positions >= s.sinks) & (positions < nxt - s.recent)]
+                    assert gone <= float(free.min() + 2 * bound * len(before))
+
+
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("lens,heads,kv_heads,page", [([20, 64, 61], 4, 2, 16), ([100, 127], 6, 6, 32)])
+def test_a_decode_loop_through_all_operators(bridge_lib, lens, heads, kv_heads, page, dtype):
+    s = Serving(bridge_lib, lens, heads, kv_heads, page, 64 if page == 16 else 128, dtype, seed=5)
+    _check_serving(s, 8, s.step)
+
+
+def test_a_captured_decode_loop_serves_every_step(bridge_lib):
+    """One CUDA graph of a step, replayed while lengths and pages' contents move on, with
+    another graph of another cache (and its own workspaces) between its replays."""
+    graphs, loops = [], []
+    for seed in (1, 2):
+        s = Serving(bridge_lib, [20, 64, 61], 4, 2, 16, 64, "f16", seed=seed)
+        keep = {n: x.clone() for n, x in dict(s.__dict__, **s.c.__dict__).items()
+                if isinstance(x, torch.Tensor) and n != "live"}
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            s.step()
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=side):
+            s.step()
+        for n, x in dict(s.__dict__, **s.c.__dict__).items():  # back to the beginning
+            if n in keep:
+                x.copy_(keep[n])
+        graphs.append(graph)
+        loops.append(s)
+    torch.cuda.synchronize()
+
+    def advance():
+        graphs[0].replay()
+        graphs[1].replay()
+    _check_serving(loops[0], 6, advance)
