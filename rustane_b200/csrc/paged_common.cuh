@@ -53,43 +53,6 @@ __device__ __forceinline__ PagedSeq paged_seq(const PagedKV& kv, int b) {
   return PagedSeq{lo, min(hi - lo, kv.max_new), len - (hi - lo), min(len, kv.max_len)};
 }
 
-// The sequence and tile of a flat tile index, when the n * group query rows of each sequence
-// are cut into tiles of M. The whole warp calls it; b = -1 when there are fewer tiles.
-struct PagedTile {
-  int b, tile;
-  PagedSeq seq;
-};
-template <int M>
-__device__ __forceinline__ PagedTile paged_find_tile(const PagedKV& kv, int group, int t) {
-  const int lane = threadIdx.x & 31;
-  int before = 0;
-  for (int base = 0; base < kv.batch; base += 32) {
-    PagedSeq s{0, 0, 0, 0};
-    if (base + lane < kv.batch) s = paged_seq(kv, base + lane);
-    const int tiles = (s.n * group + M - 1) / M;
-    int incl = tiles;
-#pragma unroll
-    for (int off = 1; off < 32; off <<= 1) {
-      const int up = __shfl_up_sync(0xffffffffu, incl, off);
-      if (lane >= off) incl += up;
-    }
-    const unsigned past = __ballot_sync(0xffffffffu, before + incl > t);
-    if (past) {
-      const int src = __ffs(past) - 1;
-      PagedTile r;
-      r.b = base + src;
-      r.tile = t - before - __shfl_sync(0xffffffffu, incl - tiles, src);
-      r.seq.row0 = __shfl_sync(0xffffffffu, s.row0, src);
-      r.seq.n = __shfl_sync(0xffffffffu, s.n, src);
-      r.seq.past = __shfl_sync(0xffffffffu, s.past, src);
-      r.seq.end = __shfl_sync(0xffffffffu, s.end, src);
-      return r;
-    }
-    before += __shfl_sync(0xffffffffu, incl, 31);
-  }
-  return PagedTile{-1, 0, PagedSeq{0, 0, 0, 0}};
-}
-
 // Programmatic dependent launch, in its two halves: a kernel lets the next one on the stream
 // start (it then waits in pdl_wait for this one's end and memory).
 __device__ __forceinline__ void pdl_launch_dependents() {

@@ -33,13 +33,15 @@ __device__ __forceinline__ int share_part(const ShareJoin& jn, int worker, int p
 struct ShareTable {  // in shared memory
   uint32_t seq_units[SHARE_CHUNK];
   uint32_t base, longer;  // the first `longer` workers have base + 1 units, the others base
+  uint32_t workers;       // with a share
 
   __device__ __forceinline__ uint32_t begin_of(uint32_t worker) const {
     return base * worker + min(worker, longer);
   }
   __device__ __forceinline__ uint32_t worker_of(uint32_t unit) const {
     const uint32_t border = (base + 1) * longer;
-    return unit < border ? unit / (base + 1) : longer + (unit - border) / base;
+    const uint32_t worker = unit < border ? unit / (base + 1) : longer + (unit - border) / base;
+    return min(worker, workers - 1);
   }
 };
 
@@ -165,6 +167,7 @@ struct PagedShares {
     if (threadIdx.x == 0) {
       table.base = all / workers;
       table.longer = all - all / workers * workers;
+      table.workers = workers;
     }
     __syncthreads();
     const uint32_t lo = (uint32_t)worker < workers ? table.begin_of(worker) : all;
