@@ -191,6 +191,12 @@ struct AttentionPlan {
   }
 };
 
+// More than 16 query rows per key head go to the tcgen05 kernel. Both sides measured (us; bf16,
+// 8 key heads):  rows per key head     8    16    24    32    64   128
+//   4 x 8192 slots,  16-row kernel  37.3  41.3  52.1  54.0  85.5   150
+//                    tcgen05        46.3  47.7  47.9  47.8  48.9  49.2
+//   32 x 2048 slots, 16-row kernel  59.2  65.8   106   109   194   334
+//                    tcgen05        73.4  76.0  77.5  78.1  79.4  80.9
 AttentionPlan plan_attention(const cb_paged_kv* kv, int32_t heads) {
   AttentionPlan p;
   const int group = heads / kv->kv_heads;
@@ -549,7 +555,9 @@ cb_status cb_paged_evict(const cb_paged_kv* kv, const float* weights, float* wei
   if ((weights != weights_out && ranges_overlap(weights, meta, weights_out, meta)) ||
       (positions != positions_out && ranges_overlap(positions, meta, positions_out, meta)) ||
       ranges_overlap(len_out, kv->batch * 4ll, kv->len, kv->batch * 4ll) ||
-      ranges_overlap(weights_out, meta, positions_out, meta))
+      ranges_overlap(weights_out, meta, positions_out, meta) ||
+      ranges_overlap(weights_out, meta, positions, meta) ||
+      ranges_overlap(weights, meta, positions_out, meta))
     return CB_ERR_INVALID_ARG;
   if (kv->max_len > EV_MAX_LEN) return CB_ERR_UNSUPPORTED;
   const cb_status s = check_device({kv->k, kv->v, kv->table, kv->len, weights, weights_out,

@@ -176,7 +176,7 @@ struct PagedShares {
     // lo / kv_heads of one head
     const uint32_t want = lo / kv.kv_heads;
     uint32_t before = 0;  // units of one head of the sequences in front
-    bool found = lo >= hi;
+    bool found = lo >= hi, placed = false;
     for (int base = 0; base < kv.batch; base += SHARE_CHUNK) {
       const int count = min(SHARE_CHUNK, kv.batch - base);
       if (kv.batch > SHARE_CHUNK) {
@@ -196,6 +196,7 @@ struct PagedShares {
         const uint32_t one = __shfl_sync(0xffffffffu, n, src);
         uint32_t r = lo - (before + __shfl_sync(0xffffffffu, incl - n, src)) * kv.kv_heads;
         const uint32_t head = r / one;
+        if (head >= (uint32_t)kv.kv_heads) break;  // (row starts that do not ascend)
         r -= head * one;
         const PagedSeq s = paged_seq(kv, b);
         const int n_tiles = tiles(s, group);
@@ -205,6 +206,7 @@ struct PagedShares {
           const uint32_t sum = inclusive(m);
           const unsigned in = __ballot_sync(0xffffffffu, run + sum > r);
           if (in) {
+            bool some = true;
             if (lane == __ffs(in) - 1) {
               walk.seq = s;
               walk.b = b;
@@ -214,8 +216,9 @@ struct PagedShares {
               walk.at = lo;
               walk.end = hi;
               walk.segment(group);
-              if (walk.j1 == walk.j0) walk.next(kv, group);
+              if (walk.j1 == walk.j0) some = walk.next(kv, group);
             }
+            placed = __all_sync(0xffffffffu, some);
             break;
           }
           run += __shfl_sync(0xffffffffu, sum, 31);
@@ -223,7 +226,7 @@ struct PagedShares {
       }
     }
     __syncthreads();
-    return lo < hi;
+    return placed;
   }
 };
 

@@ -105,6 +105,14 @@ __global__ void __launch_bounds__(WT_THREADS, 1)
     tmem_alloc(tmem_slot, WT_TMEM_COLS);
     tmem_relinquish();
   }
+  // Rows behind a step's (where 128 is no multiple of the group) are 0 and count with a
+  // log-sum-exp of infinity, weight 0, so that steps need no masks for them.
+  for (int i = threadIdx.x; i < WT_Q_BUFS * 2 * (WT_ROWS - step_rows) * 8; i += WT_THREADS) {
+    const int half = i / ((WT_ROWS - step_rows) * 8), in_half = i - half * (WT_ROWS - step_rows) * 8;
+    *reinterpret_cast<uint4*>(smem + WT_Q_OFF + half * (WT_Q_BYTES / 2) + step_rows * 128 +
+                              in_half * 16) = make_uint4(0, 0, 0, 0);
+  }
+  fence_proxy_async_smem();
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
@@ -179,7 +187,7 @@ __global__ void __launch_bounds__(WT_THREADS, 1)
         const int tok = c / group, i = i0 + j * step_tokens + tok;
         const bool valid = c < step_rows && i < seq.n;
         x[e] = valid ? -__ldg(lse + (int64_t)(seq.row0 + i) * heads + head * group + c - tok * group)
-                     : 0.f;
+                     : -CUDART_INF_F;
         lim[e] = valid ? seq.limit(i) : 0;
       }
     };
@@ -218,8 +226,7 @@ __global__ void __launch_bounds__(WT_THREADS, 1)
       const int buf = j % WT_L_BUFS;
       const int first = i0 + j * step_tokens;
       // whole steps whose rows all see the tile's slots need no masks
-      const bool whole = step_rows == WT_ROWS && first + step_tokens <= seq.n &&
-                         key0 + s * 128 + 128 <= seq.limit(first);
+      const bool whole = first + step_tokens <= seq.n && key0 + s * 128 + 128 <= seq.limit(first);
       const float4* nl = reinterpret_cast<const float4*>(smem + WT_L_OFF + buf * WT_ROWS * 8);
       const int4* lim = reinterpret_cast<const int4*>(nl + WT_ROWS / 4);
       if (!mbar_wait(&l_full[buf], (j / WT_L_BUFS) & 1, failed) ||

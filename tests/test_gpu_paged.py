@@ -335,6 +335,29 @@ def test_weights(bridge_lib, lens, news, heads, kv_heads, page, dtype):
     assert torch.equal(w, w2)  # a fixed order of additions
 
 
+@pytest.mark.parametrize("heads", [3, 5, 7, 100])
+def test_weights_of_a_bad_key_stay_in_its_slot(bridge_lib, heads):
+    """Groups that do not divide 128 leave rows of a step without a query; a key with NaN and
+    infinities reaches its own slot's sum only."""
+    c = Cache([600, 140], [150, 140], heads, 1, 32, "bf16", seed=heads)
+    q = c.tokens(heads * 128, scale=1.5)
+    _, lse64, _, _ = R.attention_ref(c, q, SCALE)
+    lse = torch.zeros(c.rows, heads, device="cuda")
+    lse[:c.starts[-1]] = lse64.float()
+    d = c.desc()
+    w = [torch.zeros(c.pages, 1, 32, device="cuda") for _ in range(2)]
+    page = c.page_lists[0][1]
+    for x in w:
+        assert bridge_lib.cb_paged_attention_weights(C.byref(d), ptr(q), q.stride(0), heads, SCALE,
+                                                     ptr(lse), ptr(x), stream()) == 0
+        torch.cuda.synchronize()
+        c.k[page, 0, 5, :64] = math.nan
+        c.k[page, 0, 5, 64:] = math.inf
+    assert bool(w[1][page, 0, 5].isnan()) and not bool(w[0].isnan().any())
+    w[1][page, 0, 5] = w[0][page, 0, 5]
+    assert torch.equal(w[0], w[1])
+
+
 # ------------------------------------------------------------------------------ evict
 def _evict(lib, c, w, wo, p, po, nxt, budget, sinks, recent, lo, st=None):
     d = c.desc()

@@ -137,6 +137,12 @@ def test_evict_refusals(bridge_lib, change):
     assert _evict(bridge_lib, _kv(), **change) == BAD
 
 
+@pytest.mark.parametrize("change", [
+    dict(wo=9 * A, po=6 * A), dict(wo=7 * A, po=9 * A), dict(wo=7 * A + 4, po=9 * A)], ids=str)
+def test_evict_refuses_an_output_over_the_other_input(bridge_lib, change):
+    assert _evict(bridge_lib, _kv(), **change) == BAD
+
+
 def test_more_than_128_query_heads_to_a_key_head_are_refused(bridge_lib):
     kv = _kv(kv_heads=1)
     assert _attention(bridge_lib, kv, heads=129, q_stride=1 << 16, out_stride=1 << 16) == BAD
