@@ -460,12 +460,14 @@ cb_status cb_lm_head_ce_f16_noalloc(const void* xf, const void* embed, const uin
  * All pointers are device memory of the current device (CB_ERR_INVALID_ARG otherwise),
  * token arrays and caches 16-byte aligned, strides counted in elements and multiples of 8.
  * Work is enqueued on `stream` (NULL = default stream) without allocation or
- * synchronisation. Device-side values are held to the descriptor: a page id outside
- * 0 .. pages - 1 stands for slots that are absent (not written, not seen by any query),
- * slots from max_len on are absent, rows from `rows` on do not exist, and of a sequence
- * with more than max_new new tokens the rows behind max_new are left alone. Rows behind
- * the last sequence (padding) are neither read nor written. A batch whose descriptor allows
- * more work than a launch can count (about 2^29 blocks of 16 slots) is CB_ERR_UNSUPPORTED. */
+ * synchronisation; a call without rows (rows, max_new or tokens 0) does nothing, and with
+ * rows or tokens 0 its token arrays may be NULL. Device-side values are held to the
+ * descriptor: a page id outside 0 .. pages - 1 stands for slots that are absent (not
+ * written, not seen by any query), slots from max_len on are absent, rows from `rows` on
+ * do not exist, and of a sequence with more than max_new new tokens the rows behind
+ * max_new are left alone. Rows behind the last sequence (padding) are neither read nor
+ * written. A batch whose descriptor allows more work than a launch can count (about 2^29
+ * blocks of 16 slots) is CB_ERR_UNSUPPORTED. */
 
 #define CB_DTYPE_F16 1
 #define CB_DTYPE_BF16 2
@@ -551,12 +553,13 @@ cb_status cb_paged_attention_workspace(const cb_paged_kv* kv, int32_t heads, siz
 
 /* Attention of a step's new tokens over the cache: query row r (token i of n of sequence b)
  * sees the slots 0 .. len[b] - n + i (the new tokens' own K and V must be in the cache:
- * cb_paged_append). out[r][h] = softmax(scale * q[r][h] . K) V with key head
+ * cb_paged_append). out[r][h] = softmax(scale * q[r][h] . K) V (scale > 0) with key head
  * h / (heads / kv_heads). heads is a multiple of kv_heads, at most 128 times it. q and out:
  * [rows][heads][128]; out must not overlap q. lse (nullable, [rows][heads]): the base-2
  * log-sum-exp of the scaled scores, as cb_attention_fwd_lse_f16. A row that sees no slot
- * gets out = 0 and lse = -inf. workspace: 16-byte aligned; its contents do not matter and none are kept, but
- * calls (and replays of captured graphs) that may run at the same time need one each. */
+ * gets out = 0 and lse = -inf. workspace: 16-byte aligned; its contents do not matter and
+ * none are kept, but calls (and replays of captured graphs) that may run at the same time
+ * need one each. */
 cb_status cb_paged_attention(const cb_paged_kv* kv, const void* q, int64_t q_stride,
                              int32_t heads, float scale, void* out, int64_t out_stride,
                              float* lse, void* workspace, size_t workspace_bytes, void* stream);

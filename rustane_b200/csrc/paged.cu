@@ -32,6 +32,10 @@ constexpr int64_t INT_LIMIT = std::numeric_limits<int32_t>::max();
 // ------------------------------------------------------------------------ checks
 bool aligned(const void* p, uintptr_t a) { return (reinterpret_cast<uintptr_t>(p) & (a - 1)) == 0; }
 
+constexpr float LOG2_E = 1.4426950408889634f;
+// The kernels take scale * log2(e), which has to be finite too.
+bool scale_ok(float scale) { return scale > 0.0f && std::isfinite(scale * LOG2_E); }
+
 bool dtype_ok(int32_t d) { return d == CB_DTYPE_F16 || d == CB_DTYPE_BF16; }
 
 // Sizes of a descriptor (no pointers).
@@ -60,8 +64,10 @@ bool heads_ok(const cb_paged_kv* kv, int32_t heads) {
          (int64_t)kv->max_new * heads <= INT_LIMIT;
 }
 
-// A token array: [rows][width] elements of two bytes.
-bool array_ok(const void* p, int64_t stride, int64_t width) {
+// A token array: [rows][width] elements of two bytes. One without rows may be null, as that of
+// an empty tensor.
+bool array_ok(const void* p, int64_t rows, int64_t stride, int64_t width) {
+  if (rows == 0) return true;
   return p && aligned(p, 16) && stride >= width && stride % 8 == 0 && stride <= (int64_t(1) << 40);
 }
 
@@ -237,7 +243,7 @@ cb_status launch_attention(const cb_paged_kv* kv, const T* q, int64_t q_stride, 
   if (!make_cache_map(&tk, kv->k, kv, box) || !make_cache_map(&tv, kv->v, kv, box))
     return CB_ERR_UNSUPPORTED;
   const PagedKV d = device_kv(kv);
-  const float scale_log2 = scale * 1.4426950408889634f;
+  const float scale_log2 = scale * LOG2_E;
   float* part_lse = workspace + p.workers * 2 * p.rows * PG_HD;
   const ShareParts parts{workspace, part_lse,
                          reinterpret_cast<ShareJoin*>(part_lse + p.workers * 2 * p.rows)};
@@ -283,7 +289,7 @@ cb_status launch_weights(const cb_paged_kv* kv, const T* q, int64_t q_stride, in
                          float scale, const float* lse, float* weights, cudaStream_t st) {
   const int group = heads / kv->kv_heads;
   const PagedKV d = device_kv(kv);
-  const float scale_log2 = scale * 1.4426950408889634f;
+  const float scale_log2 = scale * LOG2_E;
   if ((int64_t)kv->max_new * group <= PR_ROWS) {
     // two CTAs per SM; no more than there are blocks of slots
     const double blocks = step_bound(kv, group, PR_ROWS, PR_BLOCK);
@@ -393,8 +399,8 @@ cb_status cb_rope(const cb_rope_config* rope, int32_t dtype, const void* x, int6
       tokens < 0 || inverse < 0 || inverse > 1 || !rope_config_ok(rope, head_dim))
     return CB_ERR_INVALID_ARG;
   const int64_t width = (int64_t)heads * head_dim;
-  if (!positions || !aligned(positions, 4) || width > INT_LIMIT || !array_ok(x, x_stride, width) ||
-      !array_ok(y, y_stride, width))
+  if ((tokens > 0 && !positions) || !aligned(positions, 4) || width > INT_LIMIT ||
+      !array_ok(x, tokens, x_stride, width) || !array_ok(y, tokens, y_stride, width))
     return CB_ERR_INVALID_ARG;
   if (tokens == 0) return CB_OK;
   if (!(x == y && x_stride == y_stride) &&
@@ -431,13 +437,13 @@ cb_status cb_paged_append(const cb_paged_kv* kv, const cb_rope_config* rope, int
   if (!q != !q_out || (q && !heads_ok(kv, heads))) return CB_ERR_INVALID_ARG;
   if (!q) heads = 0;
   const int64_t q_width = (int64_t)heads * PG_HD, kv_width = (int64_t)kv->kv_heads * PG_HD;
-  if (q && (!array_ok(q, q_stride, q_width) || !array_ok(q_out, q_out_stride, q_width)))
+  const int64_t rows = kv->rows;
+  if (q && (!array_ok(q, rows, q_stride, q_width) || !array_ok(q_out, rows, q_out_stride, q_width)))
     return CB_ERR_INVALID_ARG;
-  if (!array_ok(k, k_stride, kv_width) || !array_ok(v, v_stride, kv_width) ||
+  if (!array_ok(k, rows, k_stride, kv_width) || !array_ok(v, rows, v_stride, kv_width) ||
       !aligned(positions, 4) || !aligned(weights, 4) || !aligned(slot_positions, 4))
     return CB_ERR_INVALID_ARG;
-  if (kv->rows == 0 || kv->max_new == 0) return CB_OK;
-  const int64_t rows = kv->rows;
+  if (rows == 0 || kv->max_new == 0) return CB_OK;
   if (q && !(q == q_out && q_stride == q_out_stride) &&
       arrays_overlap(q, q_stride, q_width, q_out, q_out_stride, q_width, rows))
     return CB_ERR_INVALID_ARG;
@@ -485,8 +491,8 @@ cb_status cb_paged_attention(const cb_paged_kv* kv, const void* q, int64_t q_str
   if (!kv_sizes_ok(kv) || !kv_pointers_ok(kv, true) || !heads_ok(kv, heads))
     return CB_ERR_INVALID_ARG;
   const int64_t width = (int64_t)heads * PG_HD;
-  if (!(scale > 0.0f) || !std::isfinite(scale) || !array_ok(q, q_stride, width) ||
-      !array_ok(out, out_stride, width) || !aligned(lse, 4) || !aligned(workspace, 16))
+  if (!scale_ok(scale) || !array_ok(q, kv->rows, q_stride, width) ||
+      !array_ok(out, kv->rows, out_stride, width) || !aligned(lse, 4) || !aligned(workspace, 16))
     return CB_ERR_INVALID_ARG;
   const size_t need = plan_attention(kv, heads).bytes();
   if (!workspace || workspace_bytes < need) return CB_ERR_INVALID_ARG;
@@ -510,8 +516,8 @@ cb_status cb_paged_attention_weights(const cb_paged_kv* kv, const void* q, int64
                                      float* weights, void* stream) {
   if (!kv_sizes_ok(kv) || !kv_pointers_ok(kv, true) || !heads_ok(kv, heads))
     return CB_ERR_INVALID_ARG;
-  if (!(scale > 0.0f) || !std::isfinite(scale) || !array_ok(q, q_stride, (int64_t)heads * PG_HD) ||
-      !lse || !weights || !aligned(lse, 4) || !aligned(weights, 4))
+  if (!scale_ok(scale) || !array_ok(q, kv->rows, q_stride, (int64_t)heads * PG_HD) ||
+      (kv->rows > 0 && !lse) || !weights || !aligned(lse, 4) || !aligned(weights, 4))
     return CB_ERR_INVALID_ARG;
   if (kv->rows == 0 || kv->max_new == 0) return CB_OK;
   const cb_status s =

@@ -143,6 +143,22 @@ def test_evict_refuses_an_output_over_the_other_input(bridge_lib, change):
     assert _evict(bridge_lib, _kv(), **change) == BAD
 
 
+def test_calls_without_rows_take_null_token_arrays(bridge_lib):
+    kv = _kv(rows=0, max_new=0)
+    assert _attention(bridge_lib, kv, q=None, out=None, lse=None) == 0
+    assert _weights(bridge_lib, kv, q=None, lse=None) == 0
+    assert _append(bridge_lib, kv, q=None, qo=None, k=None, v=None, pos=None) == 0
+    assert _rope(bridge_lib, _config(), x=None, y=None, pos=None, tokens=0) == 0
+    assert _attention(bridge_lib, kv, ws=None) == BAD
+    assert _weights(bridge_lib, kv, w=None) == BAD
+
+
+@pytest.mark.parametrize("scale", [3e38, math.inf, -0.1])
+def test_scales_whose_base_2_form_is_not_finite_are_refused(bridge_lib, scale):
+    assert _attention(bridge_lib, _kv(), scale=scale) == BAD
+    assert _weights(bridge_lib, _kv(), scale=scale) == BAD
+
+
 def test_more_than_128_query_heads_to_a_key_head_are_refused(bridge_lib):
     kv = _kv(kv_heads=1)
     assert _attention(bridge_lib, kv, heads=129, q_stride=1 << 16, out_stride=1 << 16) == BAD
