@@ -17,7 +17,7 @@
 // per scheduler and took 1.4 times as long; steps of 64 rows with two CTAs an SM likewise: a
 // step costs a warp some 60 instructions whatever its rows.)
 // 3 chunks of up to 1024 on 8192 slots, 32 / 8 heads, bf16: 153 us, 0.69 PFLOP/s. A step of 512
-// slots and 128 rows takes 2.6 us, about 4800 cycles: 3072 of MUFU, 2900 issue slots of each
+// slots and 128 rows takes 2.6 us, about 4800 cycles: 3100 of MUFU, 2900 issue slots of each
 // scheduler, 2048 of products, which its four warps of sums overlap only in part; and 296 CTAs of
 // unequal length on 148 SMs leave a tail of 12 %.
 #pragma once
