@@ -583,7 +583,10 @@ cb_status cb_paged_evict_workspace(const cb_paged_kv* kv, int32_t budget, size_t
  * counts as the smallest; among equals the lowest slot), budget in all; sinks + recent <=
  * budget. The kept slots behind the budget move into the slots below it that became free,
  * both in ascending order; the other kept slots stay where they are (attention does not
- * depend on the slots' order). len_out[b] = min(len[b], budget). weights_out and
+ * depend on the slots' order). len_out[b] = min(len[b], budget). A slot below the budget whose
+ * page is absent takes no row: it keeps its place and counts, and of such a sequence's slots
+ * behind the budget only those that must stay move, in the places of the lightest (if more
+ * must stay than there are places, the lowest slots of them do). weights_out and
  * positions_out get the values of all slots below len_out[b]; they may be the input arrays
  * themselves (not overlap them in another way). K and V change in place. Slots from
  * len_out[b] on are left as they were. len_out must not overlap len. The sequences of the

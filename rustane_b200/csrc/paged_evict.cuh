@@ -1,8 +1,11 @@
 // Eviction from a paged cache by accumulated attention weight.
 //
 // One cluster of CTAs per (sequence, key head). Every slot gets a 32-bit key whose unsigned
-// order is the order of keeping: all ones for the positions that must stay, else the
-// weight's bits made monotone (NaN lowest). Which slots go:
+// order is the order of keeping: EV_MUST for the positions that must stay, else the
+// weight's bits made monotone (NaN lowest). A slot below the budget whose page is absent can
+// take no row: it keeps its place (EV_HELD, above all others), and in such a sequence the
+// slots behind the budget that need not stay come last (0), so that a row that must stay
+// never moves to where it would be lost. Which slots go:
 //   - up to EV_FEW of them (a decode step drops one): the smallest key, of equals the highest
 //     slot, is looked for that many times;
 //   - more: the budget-th largest key is found eleven bits a pass by a histogram in shared
@@ -40,6 +43,9 @@ __device__ __forceinline__ uint32_t evict_key(float w) {
   const uint32_t bits = __float_as_uint(w + 0.0f);  // -0 counts as 0
   return bits >> 31 ? ~bits : bits | 0x80000000u;
 }
+
+constexpr uint32_t EV_MUST = 0xfffffffeu;  // (of a weight: at most 0xff800000, infinity)
+constexpr uint32_t EV_HELD = 0xffffffffu;
 
 constexpr int EV_FEW = 8;
 constexpr int EV_BINS = 2048;
@@ -124,6 +130,7 @@ __global__ void __launch_bounds__(THREADS)
   // ---- the keys. Written to another array, weights and positions of every slot below the
   // new length are copied at once (a hole's are overwritten when its mover comes).
   uint32_t key[PER];
+  bool held = false;  // a slot below the new length is absent
   {
     const int recent_from = __ldg(a.next_position + b) - a.recent;
     constexpr int BATCH = PER < 8 ? PER : 8;  // loads in flight
@@ -146,8 +153,9 @@ __global__ void __launch_bounds__(THREADS)
       for (int e = 0; e < BATCH; ++e) {
         const int s = base + (e0 + e) * THREADS + t;
         const bool must = p[e] < a.sinks || (a.recent > 0 && p[e] >= recent_from);
-        // 0: no slot, or one that is absent (kept last)
-        key[e0 + e] = at[e] < 0 ? 0u : must ? 0xffffffffu : evict_key(w[e]);
+        // 0: no slot, or an absent one behind the new length (never kept: as many others are there)
+        key[e0 + e] = at[e] < 0 ? (s < new_len ? EV_HELD : 0u) : must ? EV_MUST : evict_key(w[e]);
+        held |= at[e] < 0 && s < new_len;
         if (at[e] >= 0 && s < new_len) {
           if (copy_w) a.weights_out[at[e]] = w[e];
           if (copy_p) a.positions_out[at[e]] = p[e];
@@ -156,6 +164,14 @@ __global__ void __launch_bounds__(THREADS)
     }
   }
   if (n <= a.budget) return;  // everything stays (the whole cluster ends here)
+  if (ctas > 1)  // the other CTAs' slots too
+    for (int s = t << kv.page_shift; s < new_len; s += THREADS << kv.page_shift)
+      held |= kv.page_id(b, s) < 0;
+  if (__syncthreads_or(held)) {
+#pragma unroll
+    for (int e = 0; e < PER; ++e)
+      if (base + e * THREADS + t >= new_len && key[e] != EV_MUST) key[e] = 0u;
+  }
 
   auto cluster_barrier = [&] {
     __syncwarp();
@@ -234,7 +250,7 @@ __global__ void __launch_bounds__(THREADS)
         if (sm.few[j] < new_len && lower == nth) dst = sm.few[j];
       }
       const int src_id = kv.page_id(b, src), dst_id = dst >= 0 ? kv.page_id(b, dst) : -1;
-      if (src_id < 0 || dst_id < 0) continue;  // a slot that is absent
+      if (src_id < 0 || dst_id < 0) continue;  // (neither is: absent slots stay out of both)
       const int from = kv.page_row(src_id, head, src), at = kv.page_row(dst_id, head, dst);
       *pool(at) = *pool(from);
       if (lane == 0) a.weights_out[at] = a.weights[from];
@@ -418,7 +434,7 @@ __global__ void __launch_bounds__(THREADS)
     if (lane < 16 && i0 + lane < moves) {
       const int src = __ldcg(movers + i0 + lane), dst = __ldcg(holes + i0 + lane);
       const int src_id = kv.page_id(b, src), dst_id = kv.page_id(b, dst);
-      if (src_id >= 0 && dst_id >= 0) {  // else a slot that is absent
+      if (src_id >= 0 && dst_id >= 0) {  // (both are: absent slots are in neither list)
         from = kv.page_row(src_id, head, src);
         at = kv.page_row(dst_id, head, dst);
       }

@@ -1,0 +1,108 @@
+"""GPU tests of the paged-cache operators at the edges of what their calls allow, against
+64-bit forms. Tolerances are derived beside each test."""
+import ctypes as C
+import math
+
+import pytest
+import torch
+
+import paged_ref as R
+from paged_ref import Cache, ptr, stream
+from rustane_b200 import bridge as B
+
+pytestmark = pytest.mark.gpu
+
+
+# ------------------------------------------------------------- eviction and absent pages
+def _evict(lib, c, w, wo, p, po, nxt, budget, sinks, recent, lo):
+    d, size = c.desc(), C.c_size_t()
+    assert lib.cb_paged_evict_workspace(C.byref(d), budget, C.byref(size)) == 0
+    ws = torch.empty(size.value, dtype=torch.uint8, device="cuda")
+    rc = lib.cb_paged_evict(C.byref(d), ptr(w), ptr(wo), ptr(p), ptr(po), ptr(nxt), budget, sinks,
+                            recent, ptr(lo), ptr(ws), size.value, stream())
+    torch.cuda.synchronize()
+    return rc
+
+
+def _evict_absent_ref(w, p, absent, nxt, budget, sinks, recent):
+    """{slot below the new length: the slot whose contents it gets} of one sequence and key
+    head. Where a slot below the budget is absent, only slots that must stay move."""
+    n = len(w)
+    new = min(n, budget)
+    slots = [s for s in range(n) if not absent[s]]
+    if n <= budget:
+        return {s: s for s in slots}
+    held = any(absent[:new])
+
+    def order(s):
+        must = p[s] < sinks or (recent > 0 and p[s] >= nxt - recent)
+        rank = 0 if must else 3 if held and s >= new else 2 if math.isnan(w[s]) else 1
+        return rank, -w[s] if rank == 1 else 0.0, s
+    keep = set(sorted(slots, key=order)[:new - sum(absent[:new])])
+    movers = [s for s in slots if s >= new and s in keep]
+    source = {s: s if s in keep else movers.pop(0) for s in slots if s < new}
+    assert not movers
+    return source
+
+
+ABSENT = [
+    # lens, kv_heads, page, budget, sinks, recent, absent pages of each sequence
+    ([64, 64], 1, 16, 48, 0, 16, [[1], []]),
+    ([64, 64, 64], 2, 16, 48, 4, 8, [[1], [3], [0, 2]]),
+    ([52, 50, 49], 2, 16, 48, 2, 10, [[1], [3], [0, 1, 2]]),      # few slots go
+    ([64, 64], 1, 16, 48, 8, 40, [[1], [0]]),                     # more must stay than have room
+    ([64, 40], 1, 16, 48, 0, 48, [[0, 1, 2], [1]]),               # nothing below the budget is there
+    ([700, 700], 3, 64, 300, 4, 100, [[0, 4, 9], [10]]),
+    ([6000, 5500], 2, 64, 2000, 4, 900, [[3, 17, 90], [93]]),     # two CTAs
+    ([5006, 5003], 1, 32, 5000, 4, 60, [[7], [156]]),             # few, two CTAs
+    ([20000], 1, 128, 8000, 4, 3000, [[0, 30, 62, 100]]),         # eight CTAs
+]
+
+
+@pytest.mark.parametrize("in_place", [False, True])
+@pytest.mark.parametrize("lens,kv_heads,page,budget,sinks,recent,gone", ABSENT)
+def test_evict_keeps_what_must_stay_beside_absent_pages(bridge_lib, lens, kv_heads, page, budget,
+                                                        sinks, recent, gone, in_place):
+    c = Cache(lens, [0] * len(lens), kv_heads, kv_heads, page, "f16", seed=sum(lens))
+    shape = (c.pages, kv_heads, page)
+    g = torch.Generator(device="cuda").manual_seed(budget)
+    w = (torch.rand(shape, device="cuda", generator=g) * 50).floor() / 8
+    odd = torch.randint(0, 20, shape, device="cuda", generator=g)
+    for i, x in enumerate((math.nan, math.inf, -math.inf, -1.5)):
+        w[odd == i] = x
+    p = torch.zeros(shape, device="cuda", dtype=torch.int32)
+    for b in range(c.batch):
+        for h in range(kv_heads):
+            at = c.place(b, torch.arange(lens[b], device="cuda"))
+            p[at[0], h, at[1]] = torch.randperm(lens[b], device="cuda", generator=g).int()
+    nxt = c.len.clone()
+    for b, pages in enumerate(gone):
+        for i, j in enumerate(pages):
+            c.table[b, j] = (-1, c.pages, -2 ** 31, 2 ** 31 - 1)[i]
+    wo = w if in_place else torch.full_like(w, 9.0)
+    po = p if in_place else torch.full_like(p, 9)
+    want = {"k": c.k.clone(), "v": c.v.clone(), "w": wo.clone(), "p": po.clone()}
+    for b in range(c.batch):
+        absent = [s // page in gone[b] for s in range(lens[b])]
+        for h in range(kv_heads):
+            pos = c.slots(p, b, h).tolist()
+            source = _evict_absent_ref(c.slots(w, b, h).tolist(), pos, absent, lens[b], budget,
+                                       sinks, recent)
+            # what the call promises, apart from how: present positions that must stay do, as
+            # far as there is room
+            must = {x for x, a in zip(pos, absent)
+                    if not a and (x < sinks or x >= lens[b] - recent)}
+            if lens[b] > budget:
+                stays = {pos[s] for s in source.values()}
+                assert must <= stays or stays <= must
+            to = c.place(b, torch.tensor(list(source), device="cuda", dtype=torch.long))
+            fro = c.place(b, torch.tensor(list(source.values()), device="cuda", dtype=torch.long))
+            for name, new, old in (("k", c.k, c.k), ("v", c.v, c.v), ("w", w, w), ("p", p, p)):
+                want[name][to[0], h, to[1]] = old[fro[0], h, fro[1]]
+    lo = torch.full_like(c.len, -1)
+    assert _evict(bridge_lib, c, w, wo, p, po, nxt, budget, sinks, recent, lo) == 0
+    assert lo.tolist() == [min(n, budget) for n in lens]
+    for name, got in (("k", c.k), ("v", c.v)):
+        assert torch.equal(got.view(torch.int16), want[name].view(torch.int16)), name
+    assert torch.equal(wo.view(torch.int32), want["w"].view(torch.int32))
+    assert torch.equal(po, want["p"])
