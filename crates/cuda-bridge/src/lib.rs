@@ -190,6 +190,8 @@ pub mod ffi {
         pub fn cb_paged_attention_workspace(kv: *const cb_paged_kv, heads: i32, bytes: *mut usize) -> cb_status;
         pub fn cb_paged_attention(kv: *const cb_paged_kv, q: *const c_void, q_stride: i64, heads: i32, scale: f32, out: *mut c_void, out_stride: i64, lse: *mut f32, workspace: *mut c_void, workspace_bytes: usize, stream: *mut c_void) -> cb_status;
         pub fn cb_paged_attention_weights(kv: *const cb_paged_kv, q: *const c_void, q_stride: i64, heads: i32, scale: f32, lse: *const f32, weights: *mut f32, stream: *mut c_void) -> cb_status;
+        pub fn cb_paged_check_device_error(expired: *mut i32, stream: *mut c_void) -> cb_status;
+        pub fn cb_selftest_paged_timeout(kv: *const cb_paged_kv, q: *const c_void, q_stride: i64, heads: i32, scale: f32, out: *mut c_void, out_stride: i64, lse: *mut f32, weights: *mut f32, workspace: *mut c_void, workspace_bytes: usize, stream: *mut c_void) -> cb_status;
         pub fn cb_paged_evict_workspace(kv: *const cb_paged_kv, budget: i32, bytes: *mut usize) -> cb_status;
         pub fn cb_paged_evict(kv: *const cb_paged_kv, weights: *const f32, weights_out: *mut f32, positions: *const i32, positions_out: *mut i32, next_position: *const i32, budget: i32, sinks: i32, recent: i32, len_out: *mut i32, workspace: *mut c_void, workspace_bytes: usize, stream: *mut c_void) -> cb_status;
     }

@@ -467,7 +467,10 @@ cb_status cb_lm_head_ce_f16_noalloc(const void* xf, const void* embed, const uin
  * do not exist, and of a sequence with more than max_new new tokens the rows behind
  * max_new are left alone. Rows behind the last sequence (padding) are neither read nor
  * written. A batch whose descriptor allows more work than a launch can count (about 2^29
- * blocks of 16 slots) is CB_ERR_UNSUPPORTED. */
+ * blocks of 16 slots) is CB_ERR_UNSUPPORTED.
+ *
+ * The kernels' waits are bounded (2 s). After one that ran out, rows of out and lse, or slots of
+ * weights, that were not finished are NaN, and cb_paged_check_device_error reports it. */
 
 #define CB_DTYPE_F16 1
 #define CB_DTYPE_BF16 2
@@ -572,6 +575,22 @@ cb_status cb_paged_attention(const cb_paged_kv* kv, const void* q, int64_t q_str
 cb_status cb_paged_attention_weights(const cb_paged_kv* kv, const void* q, int64_t q_stride,
                                      int32_t heads, float scale, const float* lse,
                                      float* weights, void* stream);
+
+/* Synchronises `stream`, writes to *expired (host) how many blocks or warps of this section's
+ * kernels had a wait run out on the current device, and clears the count: CB_OK for none, else
+ * CB_ERR_DEVICE_TIMEOUT. Not to be captured. */
+cb_status cb_paged_check_device_error(int32_t* expired, void* stream);
+
+/* Self-test of the bounded waits: cb_paged_attention_weights, then cb_paged_attention of this
+ * step, by kernels whose loads are never issued and whose waits run out after 1 ms. Arguments
+ * as of these calls (dtype CB_DTYPE_F16; lse is read by the first and written by the second).
+ * Afterwards every row of out and lse is NaN and, where kernels with waits add up
+ * the weights (more than 16 query rows per key head), so is every slot that a row sees; the
+ * next cb_paged_check_device_error returns CB_ERR_DEVICE_TIMEOUT. */
+cb_status cb_selftest_paged_timeout(const cb_paged_kv* kv, const void* q, int64_t q_stride,
+                                    int32_t heads, float scale, void* out, int64_t out_stride,
+                                    float* lse, float* weights, void* workspace,
+                                    size_t workspace_bytes, void* stream);
 
 /* Bytes of workspace that cb_paged_evict needs (host call, no GPU; reads batch, kv_heads
  * and max_len). */

@@ -61,7 +61,7 @@ EXPORTED = [
     "cb_prefill", "cb_decode_step", "cb_decode_position",
     "cb_rope_frequencies", "cb_rope", "cb_paged_append", "cb_paged_attention_workspace",
     "cb_paged_attention", "cb_paged_attention_weights", "cb_paged_evict_workspace",
-    "cb_paged_evict",
+    "cb_paged_evict", "cb_paged_check_device_error", "cb_selftest_paged_timeout",
 ]
 
 
@@ -184,6 +184,9 @@ def load_library(path: Path | None = None) -> C.CDLL:
         "cb_paged_attention_workspace": (i32, [pkv, i32, psize]),
         "cb_paged_attention": (i32, [pkv, vp, i64, i32, f32, vp, i64, vp, vp, C.c_size_t, vp]),
         "cb_paged_attention_weights": (i32, [pkv, vp, i64, i32, f32, vp, vp, vp]),
+        "cb_paged_check_device_error": (i32, [pi32, vp]),
+        "cb_selftest_paged_timeout": (i32, [pkv, vp, i64, i32, f32, vp, i64, vp, vp, vp,
+                                            C.c_size_t, vp]),
         "cb_paged_evict_workspace": (i32, [pkv, i32, psize]),
         "cb_paged_evict": (i32, [pkv, vp, vp, vp, vp, vp, i32, i32, i32, vp, vp, C.c_size_t,
                                  vp]),

@@ -231,7 +231,7 @@ cudaError_t launch_pdl(void (*kernel)(Params...), dim3 grid, int threads, cudaSt
   return cudaLaunchKernelEx(&cfg, kernel, Params(args)...);
 }
 
-template <typename T>
+template <typename T, bool LOADS>
 cb_status launch_attention(const cb_paged_kv* kv, const T* q, int64_t q_stride, int32_t heads,
                            float scale, T* out, int64_t out_stride, float* lse, float* workspace,
                            cudaStream_t st) {
@@ -250,16 +250,18 @@ cb_status launch_attention(const cb_paged_kv* kv, const T* q, int64_t q_stride, 
   cudaError_t e;
   if (p.tc) {
     static std::atomic<uint64_t> done{0};
-    if ((e = allow_smem(paged_tile_kernel<T>, PT_SMEM, done)) != cudaSuccess) return status_of(e);
-    paged_tile_kernel<T><<<p.ctas, PT_THREADS, PT_SMEM, st>>>(
+    if ((e = allow_smem(paged_tile_kernel<T, LOADS>, PT_SMEM, done)) != cudaSuccess)
+      return status_of(e);
+    paged_tile_kernel<T, LOADS><<<p.ctas, PT_THREADS, PT_SMEM, st>>>(
         tk, tv, d, q, q_stride, heads, scale_log2, out, out_stride, lse, parts, box);
     if ((e = cudaPeekAtLastError()) != cudaSuccess) return status_of(e);
     e = launch_pdl(paged_join_kernel<T>, dim3(p.ctas, PT_ROWS / PJ_ROWS), PJ_WARPS * 32, st, parts,
                    heads, group, out, out_stride, lse);
   } else {
     static std::atomic<uint64_t> done{0};
-    if ((e = allow_smem(paged_rows_kernel<T>, PR_SMEM, done)) != cudaSuccess) return status_of(e);
-    paged_rows_kernel<T><<<p.ctas, PR_WARPS * 32, PR_SMEM, st>>>(
+    if ((e = allow_smem(paged_rows_kernel<T, LOADS>, PR_SMEM, done)) != cudaSuccess)
+      return status_of(e);
+    paged_rows_kernel<T, LOADS><<<p.ctas, PR_WARPS * 32, PR_SMEM, st>>>(
         tk, tv, d, q, q_stride, heads, scale_log2, out, out_stride, lse, parts);
     if ((e = cudaPeekAtLastError()) != cudaSuccess) return status_of(e);
     const int tile_rows = (int)std::min<int64_t>(PR_ROWS, (int64_t)kv->max_new * group);
@@ -284,7 +286,7 @@ bool make_q_map(CUtensorMap* map, const void* q, int64_t q_stride, int heads, in
              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-template <typename T>
+template <typename T, bool LOADS>
 cb_status launch_weights(const cb_paged_kv* kv, const T* q, int64_t q_stride, int32_t heads,
                          float scale, const float* lse, float* weights, cudaStream_t st) {
   const int group = heads / kv->kv_heads;
@@ -308,9 +310,9 @@ cb_status launch_weights(const cb_paged_kv* kv, const T* q, int64_t q_stride, in
       !make_q_map(&tq, q, q_stride, heads, kv->rows, group, tokens))
     return CB_ERR_UNSUPPORTED;
   static std::atomic<uint64_t> done{0};
-  const cudaError_t e = allow_smem(paged_weights_tile_kernel<T>, WT_SMEM, done);
+  const cudaError_t e = allow_smem(paged_weights_tile_kernel<T, LOADS>, WT_SMEM, done);
   if (e != cudaSuccess) return status_of(e);
-  paged_weights_tile_kernel<T><<<(unsigned)grid, WT_THREADS, WT_SMEM, st>>>(
+  paged_weights_tile_kernel<T, LOADS><<<(unsigned)grid, WT_THREADS, WT_SMEM, st>>>(
       tk, tq, d, heads, scale_log2, lse, weights, blocks, box, tokens);
   return status_of(cudaPeekAtLastError());
 }
@@ -485,9 +487,13 @@ cb_status cb_paged_attention_workspace(const cb_paged_kv* kv, int32_t heads, siz
   return CB_OK;
 }
 
-cb_status cb_paged_attention(const cb_paged_kv* kv, const void* q, int64_t q_stride,
-                             int32_t heads, float scale, void* out, int64_t out_stride,
-                             float* lse, void* workspace, size_t workspace_bytes, void* stream) {
+}  // extern "C"
+
+template <bool LOADS>
+static cb_status paged_attention(const cb_paged_kv* kv, const void* q, int64_t q_stride,
+                                 int32_t heads, float scale, void* out, int64_t out_stride,
+                                 float* lse, void* workspace, size_t workspace_bytes,
+                                 void* stream) {
   if (!kv_sizes_ok(kv) || !kv_pointers_ok(kv, true) || !heads_ok(kv, heads))
     return CB_ERR_INVALID_ARG;
   const int64_t width = (int64_t)heads * PG_HD;
@@ -505,15 +511,20 @@ cb_status cb_paged_attention(const cb_paged_kv* kv, const void* q, int64_t q_str
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   float* ws = static_cast<float*>(workspace);
   if (kv->dtype == CB_DTYPE_F16)
-    return launch_attention(kv, static_cast<const __half*>(q), q_stride, heads, scale,
-                            static_cast<__half*>(out), out_stride, lse, ws, st);
-  return launch_attention(kv, static_cast<const __nv_bfloat16*>(q), q_stride, heads, scale,
-                          static_cast<__nv_bfloat16*>(out), out_stride, lse, ws, st);
+    return launch_attention<__half, LOADS>(kv, static_cast<const __half*>(q), q_stride, heads,
+                                           scale, static_cast<__half*>(out), out_stride, lse, ws,
+                                           st);
+  if constexpr (LOADS)
+    return launch_attention<__nv_bfloat16, true>(kv, static_cast<const __nv_bfloat16*>(q), q_stride,
+                                                 heads, scale, static_cast<__nv_bfloat16*>(out),
+                                                 out_stride, lse, ws, st);
+  return CB_ERR_UNSUPPORTED;
 }
 
-cb_status cb_paged_attention_weights(const cb_paged_kv* kv, const void* q, int64_t q_stride,
-                                     int32_t heads, float scale, const float* lse,
-                                     float* weights, void* stream) {
+template <bool LOADS>
+static cb_status paged_weights(const cb_paged_kv* kv, const void* q, int64_t q_stride,
+                               int32_t heads, float scale, const float* lse, float* weights,
+                               void* stream) {
   if (!kv_sizes_ok(kv) || !kv_pointers_ok(kv, true) || !heads_ok(kv, heads))
     return CB_ERR_INVALID_ARG;
   if (!scale_ok(scale) || !array_ok(q, kv->rows, q_stride, (int64_t)heads * PG_HD) ||
@@ -525,10 +536,55 @@ cb_status cb_paged_attention_weights(const cb_paged_kv* kv, const void* q, int64
   if (s != CB_OK) return s;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   if (kv->dtype == CB_DTYPE_F16)
-    return launch_weights(kv, static_cast<const __half*>(q), q_stride, heads, scale, lse, weights,
-                          st);
-  return launch_weights(kv, static_cast<const __nv_bfloat16*>(q), q_stride, heads, scale, lse,
-                        weights, st);
+    return launch_weights<__half, LOADS>(kv, static_cast<const __half*>(q), q_stride, heads, scale,
+                                         lse, weights, st);
+  if constexpr (LOADS)
+    return launch_weights<__nv_bfloat16, true>(kv, static_cast<const __nv_bfloat16*>(q), q_stride,
+                                               heads, scale, lse, weights, st);
+  return CB_ERR_UNSUPPORTED;
+}
+
+extern "C" {
+
+cb_status cb_paged_attention(const cb_paged_kv* kv, const void* q, int64_t q_stride,
+                             int32_t heads, float scale, void* out, int64_t out_stride,
+                             float* lse, void* workspace, size_t workspace_bytes, void* stream) {
+  return paged_attention<true>(kv, q, q_stride, heads, scale, out, out_stride, lse, workspace,
+                               workspace_bytes, stream);
+}
+
+cb_status cb_paged_attention_weights(const cb_paged_kv* kv, const void* q, int64_t q_stride,
+                                     int32_t heads, float scale, const float* lse,
+                                     float* weights, void* stream) {
+  return paged_weights<true>(kv, q, q_stride, heads, scale, lse, weights, stream);
+}
+
+cb_status cb_paged_check_device_error(int32_t* expired, void* stream) {
+  if (!expired) return CB_ERR_INVALID_ARG;
+  cb_status s = check_device({});
+  if (s != CB_OK) return s;
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  *expired = 0;
+  cudaError_t e = cudaMemcpyFromSymbolAsync(expired, paged_expired, sizeof(int32_t), 0,
+                                            cudaMemcpyDeviceToHost, st);
+  if (e == cudaSuccess) e = cudaStreamSynchronize(st);
+  if (e == cudaSuccess && *expired != 0) {
+    const int none = 0;
+    e = cudaMemcpyToSymbolAsync(paged_expired, &none, sizeof(none), 0, cudaMemcpyHostToDevice, st);
+    if (e == cudaSuccess) e = cudaStreamSynchronize(st);
+    s = CB_ERR_DEVICE_TIMEOUT;
+  }
+  return e == cudaSuccess ? s : status_of(e);
+}
+
+cb_status cb_selftest_paged_timeout(const cb_paged_kv* kv, const void* q, int64_t q_stride,
+                                    int32_t heads, float scale, void* out, int64_t out_stride,
+                                    float* lse, float* weights, void* workspace,
+                                    size_t workspace_bytes, void* stream) {
+  const cb_status s = paged_weights<false>(kv, q, q_stride, heads, scale, lse, weights, stream);
+  if (s != CB_OK) return s;
+  return paged_attention<false>(kv, q, q_stride, heads, scale, out, out_stride, lse, workspace,
+                                workspace_bytes, stream);
 }
 
 static size_t evict_list(const cb_paged_kv* kv, int32_t budget) {

@@ -58,7 +58,7 @@ __device__ __forceinline__ float quad_max(float x) {
 }
 
 // Parts: o [2 workers][16 rows][128], lse [2 workers][16]; worker = warp * gridDim + CTA.
-template <typename T>
+template <typename T, bool LOADS>
 __global__ void __launch_bounds__(PR_WARPS * 32, 1)
     paged_rows_kernel(const __grid_constant__ CUtensorMap tmK,
                       const __grid_constant__ CUtensorMap tmV, const PagedKV kv,
@@ -97,12 +97,14 @@ __global__ void __launch_bounds__(PR_WARPS * 32, 1)
     const int row = id >= 0 ? kv.page_row(id, ahead.head, next_j * PR_BLOCK) : kv.cache_rows();
     uint8_t* dst = ring + stage * PR_STAGE_BYTES;
     sh.absent[warp][stage] = id < 0;
-    mbar_arrive_expect_tx(&full[stage], PR_STAGE_BYTES);
-    tma_load_2d(dst, &tmK, &full[stage], 0, row);
-    tma_load_2d(dst + 2048, &tmK, &full[stage], 64, row);
-    tma_load_2d(dst + 4096, &tmV, &full[stage], 0, row);
-    tma_load_2d(dst + 6144, &tmV, &full[stage], 64, row);
-    ++loaded;
+    if constexpr (LOADS) {
+      mbar_arrive_expect_tx(&full[stage], PR_STAGE_BYTES);
+      tma_load_2d(dst, &tmK, &full[stage], 0, row);
+      tma_load_2d(dst + 2048, &tmK, &full[stage], 64, row);
+      tma_load_2d(dst + 4096, &tmV, &full[stage], 0, row);
+      tma_load_2d(dst + 6144, &tmV, &full[stage], 64, row);
+      ++loaded;
+    }
     if (++next_j == ahead.j1) {
       more = ahead.next(kv, group);
       next_j = ahead.j0;
@@ -166,11 +168,12 @@ __global__ void __launch_bounds__(PR_WARPS * 32, 1)
     float m[2] = {-CUDART_INF_F, -CUDART_INF_F}, l[2] = {0.f, 0.f};
     bool odd_v = false;  // an infinity or NaN was taken out of V
 
-    for (int jb = j0; jb < j1; ++jb, ++g) {
+    for (int jb = j0; ok && jb < j1; ++jb, ++g) {
       const int stage = g % PR_STAGES;
       const int key0 = jb * PR_BLOCK;
-      if (ok) ok = mbar_wait(&full[stage], (g / PR_STAGES) & 1, &sh.failed);
-      __syncwarp();
+      ok = __all_sync(0xffffffffu,
+                      paged_wait<LOADS>(&full[stage], (g / PR_STAGES) & 1, &sh.failed));
+      if (!ok) break;
       const uint32_t kb = smem_u32(ring + stage * PR_STAGE_BYTES), vb = kb + 4096;
       const bool absent = sh.absent[warp][stage] != 0;
       float s[2][4] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
@@ -286,9 +289,10 @@ __global__ void __launch_bounds__(PR_WARPS * 32, 1)
     for (int j = 0; j < 2; ++j) {
       l[j] = quad_sum(l[j]);
       const int r = r0 + 8 * j;
+      if (!ok) l[j] = CUDART_NAN_F;  // a wait ran out, here or in a segment before
       const float inv = l[j] == 0.f ? 0.f : 1.0f / l[j];  // a row that sees nothing: 0
       const float row_lse = l[j] == 0.f ? -CUDART_INF_F : m[j] + log2f(l[j]);
-      if (r < rows && ok) {
+      if (r < rows) {
         if (whole) {
           T* po = out + row_of[j] * out_stride + (int64_t)head_of[j] * PG_HD + c2;
 #pragma unroll
@@ -312,6 +316,11 @@ __global__ void __launch_bounds__(PR_WARPS * 32, 1)
     if (lane == 0) go_on = w.next(kv, group);
     go_on = __any_sync(0xffffffffu, go_on);
   } while (go_on);
+  if (!ok && lane == 0) {
+    for (uint32_t x = g; x < loaded; ++x)
+      paged_drain<LOADS>(&full[x % PR_STAGES], (x / PR_STAGES) & 1);
+    paged_report_timeout();
+  }
 }
 
 // Joins the parts of the tiles that begin in a worker's share and go on behind it:

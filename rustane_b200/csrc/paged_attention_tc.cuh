@@ -168,7 +168,7 @@ struct PtShared {  // at PT_SHARE_OFF
 static_assert(sizeof(PtShared) <= PT_SMEM - 1024 - PT_SHARE_OFF, "shared memory");
 
 // Parts: o [2 gridDim][128][256 rows], lse [2 gridDim][256].
-template <typename T>
+template <typename T, bool LOADS>
 __global__ void __launch_bounds__(PT_THREADS, 1)
     paged_tile_kernel(const __grid_constant__ CUtensorMap tmK,
                       const __grid_constant__ CUtensorMap tmV, const PagedKV kv,
@@ -251,9 +251,10 @@ __global__ void __launch_bounds__(PT_THREADS, 1)
     regs_dec<72>();
     if (warp == 0) {
       // ---------------- producer
-      uint32_t g = 0;  // steps loaded
-      bool ok = true;
-      do {
+      uint32_t g = 0;               // steps loaded
+      uint32_t k_of = 0, v_of = 0;  // of K and of V
+      bool ok = LOADS;
+      if (LOADS) do {
         const int n = w.j1 - w.j0;
         const int b = w.b, head = w.head, end = w.seq.end, first = w.j0 * PT_KEYS;
         int id = pt_step_id<PT_KEYS>(kv, b, first, end, box_rows, lane);
@@ -272,23 +273,32 @@ __global__ void __launch_bounds__(PT_THREADS, 1)
           for (uint32_t parts_gone = __ballot_sync(0xffffffffu, gone); parts_gone;
                parts_gone &= parts_gone - 1)
             absent |= ((1u << (box_rows / 16)) - 1) << ((__ffs(parts_gone) - 1) / 2 * (box_rows / 16));
-          if (!(ok = mbar_wait(&k_empty[buf], free_parity, failed))) break;
+          ok = __all_sync(0xffffffffu, paged_wait<LOADS>(&k_empty[buf], free_parity, failed));
+          if (!ok) break;
           if (lane == 0) absent_of[g & 3] = absent;
           pt_load_step<PT_KEYS>(&tmK, smem + PT_K_OFF + buf * PT_STEP_BYTES, &k_full[buf], kv, head,
                                 key0, id, box_rows, lane);
-          if (!(ok = mbar_wait(&v_empty[buf], free_parity, failed))) break;
+          k_of = g + 1;
+          ok = __all_sync(0xffffffffu, paged_wait<LOADS>(&v_empty[buf], free_parity, failed));
+          if (!ok) break;
           pt_load_step<PT_KEYS>(&tmV, smem + PT_V_OFF + buf * PT_STEP_BYTES, &v_full[buf], kv, head,
                                 key0, id, box_rows, lane);
+          v_of = g + 1;
           id = next;
         }
-      } while (__all_sync(0xffffffffu, ok) && next_segment());
+      } while (ok && next_segment());
+      // the last steps' loads (of a CTA that ends as it should they have long been used)
+      for (uint32_t x = k_of < PT_BUFS ? 0 : k_of - PT_BUFS; x < k_of; ++x)
+        paged_drain<LOADS>(&k_full[x % PT_BUFS], (x / PT_BUFS) & 1);
+      for (uint32_t x = v_of < PT_BUFS ? 0 : v_of - PT_BUFS; x < v_of; ++x)
+        paged_drain<LOADS>(&v_full[x % PT_BUFS], (x / PT_BUFS) & 1);
     } else if (warp == 1) {
       // ---------------- matrix instructions
       constexpr uint32_t idesc_s = pt_idesc<T>(PT_KEYS, false), idesc_pv = pt_idesc<T>(128, true);
       const uint32_t leader = pt_elect();
       const uint32_t t0 = __shfl_sync(0xffffffffu, tmem, 0);
       auto wait = [&](uint64_t* bar, uint32_t parity) -> bool {
-        const bool there = __all_sync(0xffffffffu, mbar_wait(bar, parity, failed));
+        const bool there = __all_sync(0xffffffffu, paged_wait<LOADS>(bar, parity, failed));
         tc_fence_after();
         return there;
       };
@@ -362,7 +372,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1)
         ++seg;
       } while (ok && next_segment());
       pt_commit(leader, drain);  // nothing is in flight when TMEM is given back
-      mbar_wait(drain, 0, failed);
+      paged_drain<LOADS>(drain, 0);
     }
   } else {
     regs_inc<216>();
@@ -395,9 +405,8 @@ __global__ void __launch_bounds__(PT_THREADS, 1)
       float m = -CUDART_INF_F, l = 0.f;
       for (int j = 0; j < n_s; ++j, ++gs) {
         const int key0 = key_first + j * PT_KEYS;
-        ok = mbar_wait(&s_full[s], gs & 1, failed);
-        __syncwarp();
-        if (!__all_sync(0xffffffffu, ok)) break;
+        ok = __all_sync(0xffffffffu, paged_wait<LOADS>(&s_full[s], gs & 1, failed));
+        if (!ok) break;
         tc_fence_after();
         uint32_t u[4][32];
 #pragma unroll
@@ -454,7 +463,9 @@ __global__ void __launch_bounds__(PT_THREADS, 1)
           // not every row sees every slot of this step: V of slots behind the sequence reads as
           // 0, infinities and NaN of the others too (a thread per slot)
           const uint32_t g = g0 + j;
-          ok = mbar_wait(&v_full[g % PT_BUFS], (g / PT_BUFS) & 1, failed);
+          ok = __all_sync(0xffffffffu,
+                          paged_wait<LOADS>(&v_full[g % PT_BUFS], (g / PT_BUFS) & 1, failed));
+          if (!ok) break;
           uint8_t* v = smem + PT_V_OFF + (g % PT_BUFS) * PT_STEP_BYTES + r * 128;
           if (r >= seq.end - key0) {
 #pragma unroll 4
@@ -515,9 +526,8 @@ __global__ void __launch_bounds__(PT_THREADS, 1)
       const float inv = l == 0.f ? 0.f : 1.0f / l;
       const float row_lse = l == 0.f ? -CUDART_INF_F : m + log2f(l);
       const bool some = n_s > 0 && l != 0.f;
-      if (ok) ok = mbar_wait(&o_full[s], seg & 1, failed);
-      __syncwarp();
-      if (!__all_sync(0xffffffffu, ok)) break;
+      if (ok) ok = __all_sync(0xffffffffu, paged_wait<LOADS>(&o_full[s], seg & 1, failed));
+      if (!ok) break;
       tc_fence_after();
       if (*odd_v && n_s > 0) {
         // O += the infinities and NaN that this row sees, of all slots that either tile may
@@ -620,9 +630,32 @@ __global__ void __launch_bounds__(PT_THREADS, 1)
       g0 += w.j1 - w.j0;
       ++seg;
     } while (next_segment());
+    if (!ok) {
+      // a wait ran out: NaN for the rows of this segment and of all behind it
+      tmem_st_wait();
+      do {
+        const int f = w.tile * PT_ROWS + s * PT_SUB + r, i = f / group;
+        const bool valid = i < w.seq.n;
+        if (!w.whole()) {  // (the join gives a row NaN for one such part)
+          const int part = 2 * blockIdx.x + (seg == 0 ? 0 : 1);
+          if (valid) parts.lse[part * PT_ROWS + s * PT_SUB + r] = CUDART_NAN_F;
+          if (w.j0 == 0 && threadIdx.x == 128)
+            parts.join[blockIdx.x] = w.join(sh.table, blockIdx.x, part, group);
+        } else if (valid) {
+          const int64_t row = (int64_t)w.seq.row0 + i;
+          const int h = w.head * group + f - i * group;
+          if (lse) lse[row * heads + h] = CUDART_NAN_F;
+          for (int c = 0; c < PG_HD / 8; ++c)
+            reinterpret_cast<uint4*>(out + row * out_stride + (int64_t)h * PG_HD)[c] =
+                make_uint4(0x7fff7fffu, 0x7fff7fffu, 0x7fff7fffu, 0x7fff7fffu);
+        }
+        ++seg;
+      } while (next_segment());
+    }
     tc_fence_before();
   }
   __syncthreads();
+  if (threadIdx.x == 0 && *failed != 0) paged_report_timeout();
   if (warp == 1) {
     tc_fence_after();
     tmem_dealloc(tmem, PT_TMEM_COLS);

@@ -53,6 +53,26 @@ __device__ __forceinline__ PagedSeq paged_seq(const PagedKV& kv, int b) {
   return PagedSeq{lo, min(hi - lo, kv.max_new), len - (hi - lo), min(len, kv.max_len)};
 }
 
+// Every wait of these kernels is bounded. One that runs out ends its CTA's work: what the CTA had
+// still to write becomes NaN (never what the arrays held before), its copies in flight are
+// waited for, and it is counted in the device's word, which cb_paged_check_device_error reads
+// (rows kernel: a count per warp). LOADS = false is the self-test: nothing is ever loaded, so
+// the waits run out, after 1 ms.
+__device__ int paged_expired;
+
+template <bool LOADS>
+__device__ __forceinline__ bool paged_wait(uint64_t* bar, uint32_t parity, int* failed) {
+  return mbar_wait_for(bar, parity, failed, LOADS ? CB_WAIT_LIMIT_NS : 1000000ull);
+}
+// Before a CTA ends: for what is still on its way, also after another wait has run out.
+template <bool LOADS>
+__device__ __forceinline__ void paged_drain(uint64_t* bar, uint32_t parity) {
+  paged_wait<LOADS>(bar, parity, nullptr);
+}
+__device__ __forceinline__ void paged_report_timeout() {
+  atomicAdd(&paged_expired, 1);
+}
+
 // Programmatic dependent launch, in its two halves: a kernel lets the next one on the stream
 // start (it then waits in pdl_wait for this one's end and memory).
 __device__ __forceinline__ void pdl_launch_dependents() {

@@ -52,7 +52,7 @@ __device__ __forceinline__ void tma_load_3d_plain(void* smem_dst, const CUtensor
 
 // Grid: ((sequence * blocks of WT_KEYS slots) + block) * kv_heads + key head. tmQ: q as
 // [rows][heads][128] in boxes of step_tokens x group x 64.
-template <typename T>
+template <typename T, bool LOADS>
 __global__ void __launch_bounds__(WT_THREADS, 1)
     paged_weights_tile_kernel(const __grid_constant__ CUtensorMap tmK,
                               const __grid_constant__ CUtensorMap tmQ, const PagedKV kv, int heads,
@@ -124,9 +124,9 @@ __global__ void __launch_bounds__(WT_THREADS, 1)
 
   if (warp == 0) {
     // ---------------- producer
-    if (lane == 0) mbar_arrive_expect_tx(k_full, 32768 * tiles);
+    if (LOADS && lane == 0) mbar_arrive_expect_tx(k_full, 32768 * tiles);
     __syncwarp();
-    for (int s = 0; s < tiles; ++s) {
+    for (int s = 0; LOADS && s < tiles; ++s) {
       const int k = key0 + s * 128;
       const int id = pt_step_id<128>(kv, b, k, seq.end, box_rows, lane);
       const int part = lane >> 1, half = lane & 1;
@@ -136,16 +136,21 @@ __global__ void __launch_bounds__(WT_THREADS, 1)
                     half * 64, row);
       }
     }
-    if (lane == 0) {
-      for (int j = 0; j < steps; ++j) {
+    if (LOADS && lane == 0) {
+      int j = 0;
+      for (; j < steps; ++j) {
         const int buf = j % WT_Q_BUFS;
-        if (!mbar_wait(&q_empty[buf], ((j / WT_Q_BUFS) & 1) ^ 1u, failed)) break;
+        if (!paged_wait<LOADS>(&q_empty[buf], ((j / WT_Q_BUFS) & 1) ^ 1u, failed)) break;
         uint8_t* dst = smem + WT_Q_OFF + buf * WT_Q_BYTES;
         const int row = seq.row0 + i0 + j * step_tokens;
         mbar_arrive_expect_tx(&q_full[buf], step_rows * 256);
         tma_load_3d_plain(dst, &tmQ, &q_full[buf], 0, head * group, row);
         tma_load_3d_plain(dst + WT_Q_BYTES / 2, &tmQ, &q_full[buf], 64, head * group, row);
       }
+      // what is still on its way (in a CTA that ends as it should it has been used by then)
+      paged_drain<LOADS>(k_full, 0);
+      for (int x = max(0, j - WT_Q_BUFS); x < j; ++x)
+        paged_drain<LOADS>(&q_full[x % WT_Q_BUFS], (x / WT_Q_BUFS) & 1);
     }
   } else if (warp == 1) {
     // ---------------- matrix instructions
@@ -153,7 +158,7 @@ __global__ void __launch_bounds__(WT_THREADS, 1)
     const uint32_t leader = pt_elect();
     const uint32_t t0 = __shfl_sync(0xffffffffu, tmem, 0);
     auto wait = [&](uint64_t* bar, uint32_t parity) -> bool {
-      const bool there = __all_sync(0xffffffffu, mbar_wait(bar, parity, failed));
+      const bool there = __all_sync(0xffffffffu, paged_wait<LOADS>(bar, parity, failed));
       tc_fence_after();
       return there;
     };
@@ -177,7 +182,7 @@ __global__ void __launch_bounds__(WT_THREADS, 1)
       pt_commit(leader, &q_empty[buf]);
     }
     pt_commit(leader, drain);
-    mbar_wait(drain, 0, failed);
+    paged_drain<LOADS>(drain, 0);
   } else if (warp < 4) {
     // ---------------- log-sum-exps and limits of the steps' rows: a warp takes every other
     // step and loads its next one before it waits for the buffer (one step after another,
@@ -206,9 +211,9 @@ __global__ void __launch_bounds__(WT_THREADS, 1)
         lm[e] = lim[e];
       }
       if (j + 2 < steps) load(j + 2);
-      const bool ok = mbar_wait(&l_empty[buf], ((j / WT_L_BUFS) & 1) ^ 1u, failed);
-      __syncwarp();
-      if (!__all_sync(0xffffffffu, ok)) break;
+      if (!__all_sync(0xffffffffu, paged_wait<LOADS>(&l_empty[buf], ((j / WT_L_BUFS) & 1) ^ 1u,
+                                                     failed)))
+        break;
       float* dst = reinterpret_cast<float*>(smem + WT_L_OFF + buf * WT_ROWS * 8);
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
@@ -233,8 +238,9 @@ __global__ void __launch_bounds__(WT_THREADS, 1)
       const bool whole = first + step_tokens <= seq.n && key0 + s * 128 + 128 <= seq.limit(first);
       const float4* nl = reinterpret_cast<const float4*>(smem + WT_L_OFF + buf * WT_ROWS * 8);
       const int4* lim = reinterpret_cast<const int4*>(nl + WT_ROWS / 4);
-      if (!mbar_wait(&l_full[buf], (j / WT_L_BUFS) & 1, failed) ||
-          !mbar_wait(&s_full[s], j & 1, failed)) { ok = false; break; }
+      ok = __all_sync(0xffffffffu, paged_wait<LOADS>(&l_full[buf], (j / WT_L_BUFS) & 1, failed) &&
+                                       paged_wait<LOADS>(&s_full[s], j & 1, failed));
+      if (!ok) break;
       tc_fence_after();
       uint32_t u[2][32];  // 32 query rows at a time, the next ones on their way
       tmem_ld_32x32b_x32(t_s, u[0]);
@@ -283,7 +289,8 @@ __global__ void __launch_bounds__(WT_THREADS, 1)
       __syncwarp();
       if (lane == 0) mbar_arrive(&l_empty[buf]);
     }
-    if (ok && key < seq.limit(seq.n - 1)) {
+    if (!ok) acc[0].x = CUDART_NAN_F;  // a wait ran out
+    if (key < seq.limit(seq.n - 1)) {
       const int id = kv.page_id(b, key);
       if (id >= 0)
         atomicAdd(weights + kv.page_row(id, head, key),
@@ -292,6 +299,7 @@ __global__ void __launch_bounds__(WT_THREADS, 1)
   }
   tc_fence_before();
   __syncthreads();
+  if (threadIdx.x == 0 && *failed != 0) paged_report_timeout();
   if (warp == 1) {
     tc_fence_after();
     tmem_dealloc(tmem, WT_TMEM_COLS);
