@@ -110,7 +110,8 @@ __global__ void __launch_bounds__(WT_THREADS, 1)
     tmem_relinquish();
   }
   // Rows behind a step's (where 128 is no multiple of the group) are 0 and count with a
-  // log-sum-exp of infinity, weight 0, so that steps need no masks for them.
+  // log-sum-exp of infinity, weight 0. (The masks count for them all the same: 0 times a key's
+  // infinity is NaN.)
   for (int i = threadIdx.x; i < WT_Q_BUFS * 2 * (WT_ROWS - step_rows) * 8; i += WT_THREADS) {
     const int half = i / ((WT_ROWS - step_rows) * 8), in_half = i - half * (WT_ROWS - step_rows) * 8;
     *reinterpret_cast<uint4*>(smem + WT_Q_OFF + half * (WT_Q_BYTES / 2) + step_rows * 128 +
@@ -234,8 +235,9 @@ __global__ void __launch_bounds__(WT_THREADS, 1)
     for (int j = 0; j < steps; ++j) {
       const int buf = j % WT_L_BUFS;
       const int first = i0 + j * step_tokens;
-      // whole steps whose rows all see the tile's slots need no masks
+      // whole steps whose rows all see the tile's slots need no masks, in 32 rows without padding
       const bool whole = first + step_tokens <= seq.n && key0 + s * 128 + 128 <= seq.limit(first);
+      const int unmasked = whole ? step_rows / 32 : 0;
       const float4* nl = reinterpret_cast<const float4*>(smem + WT_L_OFF + buf * WT_ROWS * 8);
       const int4* lim = reinterpret_cast<const int4*>(nl + WT_ROWS / 4);
       ok = __all_sync(0xffffffffu, paged_wait<LOADS>(&l_full[buf], (j / WT_L_BUFS) & 1, failed) &&
@@ -255,7 +257,7 @@ __global__ void __launch_bounds__(WT_THREADS, 1)
           __syncwarp();
           if (lane == 0) mbar_arrive(&s_empty[s]);
         }
-        if (whole) {
+        if (c < unmasked) {
 #pragma unroll
           for (int e = 0; e < 32; e += 4) {
             const float4 y = nl[c * 8 + e / 4];

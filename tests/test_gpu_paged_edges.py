@@ -106,3 +106,31 @@ def test_evict_keeps_what_must_stay_beside_absent_pages(bridge_lib, lens, kv_hea
         assert torch.equal(got.view(torch.int16), want[name].view(torch.int16)), name
     assert torch.equal(wo.view(torch.int32), want["w"].view(torch.int32))
     assert torch.equal(po, want["p"])
+
+
+# ------------------------------------------- keys with infinities in the weights of a chunk
+@pytest.mark.parametrize("heads", [3, 5, 7, 100, 4, 128])
+def test_weights_of_an_infinite_key_do_not_depend_on_the_group(bridge_lib, heads):
+    """A key with one infinite element scores minus infinity with queries whose element there
+    is negative: its slot gets 0 from them, also where the rows of a step are not all taken."""
+    c = Cache([600], [150], heads, 1, 32, "bf16", seed=heads)
+    q = c.tokens(heads * 128, scale=1.5)
+    q.unflatten(1, (heads, 128))[:150, :, 9] = -0.5
+    scale = 128 ** -0.5
+    _, lse64, _, _ = R.attention_ref(c, q, scale)
+    lse = torch.zeros(c.rows, heads, device="cuda")
+    lse[:150] = lse64.float()
+    clean, w = (torch.zeros(c.pages, 1, 32, device="cuda") for _ in range(2))
+    d = c.desc()
+    for x in (clean, w):
+        assert bridge_lib.cb_paged_attention_weights(C.byref(d), ptr(q), q.stride(0), heads, scale,
+                                                     ptr(lse), ptr(x), stream()) == 0
+        torch.cuda.synchronize()
+        for slot, value in ((5, math.inf), (70, -math.inf), (590, math.inf)):
+            at = c.place(0, torch.tensor([slot], device="cuda"))
+            c.k[at[0], 0, at[1], 9] = value
+    want = clean.clone()
+    for slot, total in ((5, 0.0), (70, math.inf), (590, 0.0)):
+        at = c.place(0, torch.tensor([slot], device="cuda"))
+        want[at[0], 0, at[1]] = total
+    assert torch.equal(w, want)
