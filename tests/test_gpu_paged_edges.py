@@ -134,3 +134,40 @@ def test_weights_of_an_infinite_key_do_not_depend_on_the_group(bridge_lib, heads
         at = c.place(0, torch.tensor([slot], device="cuda"))
         want[at[0], 0, at[1]] = total
     assert torch.equal(w, want)
+
+
+# ------------------------------------------------------------- sums of many small weights
+def _one_heavy_slot(n, new, batch, heads, behind, dtype):
+    """Every sequence sees the same n slots, slot 0 with a score of `behind` (base 2) above
+    the equal others and V = 0, the others' V = 1. (Many sequences, so that one worker walks all
+    slots of one.) Returns out, lse, the others' sums and the error of a score."""
+    c = Cache([n], [new], heads, 1, 64, dtype, seed=1, pad=0)
+    c.k[c.live], c.v[c.live] = 0.0, 1.0
+    first = c.place(0, torch.tensor([0], device="cuda"))
+    c.k[first[0], 0, first[1]], c.v[first[0], 0, first[1]] = 1.0, 0.0
+    c.table = c.table.expand(batch, -1).contiguous()
+    c.len = c.len.expand(batch).contiguous()
+    c.row_start = torch.arange(batch + 1, device="cuda", dtype=torch.int32) * new
+    c.batch, c.rows = batch, batch * new
+    q = torch.ones(c.rows, heads * 128, device="cuda", dtype=c.dt)
+    out = torch.zeros_like(q)
+    lse = torch.zeros(c.rows, heads, device="cuda")
+    assert R.attention(B.load_library(), c, q, behind / (128 * R.LOG2E), out, lse) == 0
+    others = torch.arange(n - new, n, dtype=torch.float64, device="cuda")
+    # a score: its accumulation and scaling in 32 bits (paged_ref.attention_ref)
+    delta = behind / R.LOG2E * 2.0 ** -19 + 2.0 ** -20 * (1 + behind / R.LOG2E)
+    return (out.view(batch, new, -1).double(), lse.view(batch, new, -1).double(),
+            (others * 2.0 ** -behind)[:, None], delta)
+
+
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("heads,new,batch", [(1, 1, 2400), (32, 1, 300), (2, 40, 150)])
+@pytest.mark.parametrize("behind", [18.0, 20.3, 23.1, 25.6])
+def test_the_log_sum_exp_counts_many_small_weights(bridge_lib, heads, new, batch, behind, dtype):
+    """The sum itself, in 32 bits: off by half a step for each of its last additions (a step of
+    128 keys each at most: n / 128 of them, and 32 within the first), not for each slot."""
+    n = 30000
+    _, lse, small, delta = _one_heavy_slot(n, new, batch, heads, behind, dtype)
+    want = behind + torch.log2(1 + small)
+    tol = delta * R.LOG2E + 2.0 ** -19 + (n / 128 + 32) * 2.0 ** -24 * R.LOG2E
+    assert float((lse - want).abs().max()) <= tol
