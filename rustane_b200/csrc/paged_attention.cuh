@@ -167,6 +167,7 @@ __global__ void __launch_bounds__(PR_WARPS * 32, 1)
     for (int i = 0; i < 16; ++i)
 #pragma unroll
       for (int j = 0; j < 4; ++j) o[i][j] = 0.f;
+    // the running maximum, less P_UP, and sum
     float m[2] = {-CUDART_INF_F, -CUDART_INF_F}, l[2] = {0.f, 0.f};
     float l_over[2] = {0.f, 0.f};  // what l's roundings have added to it
     bool odd_v = false;  // an infinity or NaN was taken out of V
@@ -202,8 +203,9 @@ __global__ void __launch_bounds__(PR_WARPS * 32, 1)
       bool grew = false;
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
-        const float mx = quad_max(fmaxf(fmaxf(s[0][2 * j], s[0][2 * j + 1]),
-                                        fmaxf(s[1][2 * j], s[1][2 * j + 1]))) * scale_log2;
+        const float mx = fmaf(quad_max(fmaxf(fmaxf(s[0][2 * j], s[0][2 * j + 1]),
+                                             fmaxf(s[1][2 * j], s[1][2 * j + 1]))),
+                              scale_log2, -H::P_UP);
         const float mn = fmaxf(m[j], mx);
         base[j] = mn == -CUDART_INF_F ? 0.f : mn;
         grew |= mn > m[j];
@@ -236,8 +238,9 @@ __global__ void __launch_bounds__(PR_WARPS * 32, 1)
         l_over[j] = (sum - l[j]) - term;
         l[j] = sum;
       }
-      // P rounds to the cache's type (the matrix instruction takes one type for both sides):
-      // at most half a step of each weight, the size of the output's own rounding.
+      // P rounds to the cache's type (the matrix instruction takes one type for both sides): at
+      // most half a step of each weight, the size of the output's own rounding (fp16: or 2^-40 of
+      // the largest weight).
       const uint32_t pf[4] = {H::pack(s[0][0], s[0][1]), H::pack(s[0][2], s[0][3]),
                               H::pack(s[1][0], s[1][1]), H::pack(s[1][2], s[1][3])};
       uint32_t v_mask[2] = {0xffffffffu, 0xffffffffu};
@@ -302,7 +305,8 @@ __global__ void __launch_bounds__(PR_WARPS * 32, 1)
       const int r = r0 + 8 * j;
       if (!ok) l[j] = CUDART_NAN_F;  // a wait ran out, here or in a segment before
       const float inv = l[j] == 0.f ? 0.f : 1.0f / l[j];  // a row that sees nothing: 0
-      const float row_lse = l[j] == 0.f ? -CUDART_INF_F : m[j] + log2f(l[j]);
+      const float row_lse =
+          l[j] == 0.f ? -CUDART_INF_F : m[j] + H::P_UP + log2f(l[j] * exp2f(-H::P_UP));
       if (r < rows) {
         if (whole) {
           T* po = out + row_of[j] * out_stride + (int64_t)head_of[j] * PG_HD + c2;

@@ -15,7 +15,7 @@
 //   warps 4-7    softmax of tile A, one thread per query row: 128 scores of a step in
 //   warps 8-11   registers (tile B likewise), running maximum and sum in 32 bits, P written
 //                over S. O in TMEM is rescaled only when the maximum has grown by 2^8 (P stays
-//                below 2^8, which both types hold).
+//                below 2^8, or in fp16, whose small weights are taken 2^7 up, below 2^15).
 // A tile's S(j+1) is issued behind its PV(j), so "S(j+1) is full" also says that O may be
 // rescaled and that P(j) is no longer read. Steps of 64 keys with two S buffers a tile, and
 // two threads per row, hide the products' latency as well, but a step costs a warp about 60
@@ -51,6 +51,9 @@ constexpr int PT_SHARE_OFF = PT_BAR_OFF + 256;
 constexpr int PT_SMEM = PT_SHARE_OFF + SHARE_CHUNK * 8 + 64 + PT_THREADS / 32 * 80 + 1024;
 constexpr uint32_t PT_TMEM_COLS = 512;  // S_A, S_B, O_A, O_B: 128 columns each
 constexpr float PT_RESCALE = 8.0f;
+// Binary places that P is taken up: what PT_RESCALE leaves of the type's.
+template <typename T>
+constexpr float PT_UP = Half16<T>::P_UP > 0.0f ? Half16<T>::P_UP - PT_RESCALE : 0.0f;
 
 template <typename T>
 __device__ __forceinline__ constexpr uint32_t pt_idesc(int n, bool b_mn) {
@@ -402,7 +405,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1)
       // every row of the tile sees the slots below this
       const int lim_all = seq.limit(f_sub / group);
       const int n_s = sub_steps(s);
-      float m = -CUDART_INF_F, l = 0.f;
+      float m = -CUDART_INF_F, l = 0.f;  // the running maximum, less PT_UP, and sum
       for (int j = 0; j < n_s; ++j, ++gs) {
         const int key0 = key_first + j * PT_KEYS;
         ok = __all_sync(0xffffffffu, paged_wait<LOADS>(&s_full[s], gs & 1, failed));
@@ -437,7 +440,8 @@ __global__ void __launch_bounds__(PT_THREADS, 1)
             mx[c] = fmax3(mx[c], __uint_as_float(u[c][e]), __uint_as_float(u[c][e + 1]));
           mx[c] = fmaxf(mx[c], __uint_as_float(u[c][31]));
         }
-        const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * scale_log2;
+        const float top =
+            fmaf(fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])), scale_log2, -PT_UP<T>);
         float corr = 1.0f;
         bool need = false;
         if (j == 0) {
@@ -507,7 +511,8 @@ __global__ void __launch_bounds__(PT_THREADS, 1)
             x.y = exp2_mufu(x.y);
             sum[e & 1] = fadd2(sum[e & 1], x);
             // P rounds to the cache's type: at most half a step of each weight, the size of
-            // the output's own rounding
+            // the output's own rounding (fp16: or 2^-32 of the largest weight, over 2^20
+            // slots less than that rounding)
             p[e] = H::pack(x.x, x.y);
           }
           tmem_st_32x32b_x16(t_s + c * 16, p);
@@ -524,7 +529,8 @@ __global__ void __launch_bounds__(PT_THREADS, 1)
       // ---------------- the segment's output
       const int h = w.head * group + f - i * group;
       const float inv = l == 0.f ? 0.f : 1.0f / l;
-      const float row_lse = l == 0.f ? -CUDART_INF_F : m + log2f(l);
+      const float row_lse =
+          l == 0.f ? -CUDART_INF_F : m + PT_UP<T> + log2f(l * exp2f(-PT_UP<T>));
       const bool some = n_s > 0 && l != 0.f;
       if (ok) ok = __all_sync(0xffffffffu, paged_wait<LOADS>(&o_full[s], seg & 1, failed));
       if (!ok) break;

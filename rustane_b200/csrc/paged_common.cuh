@@ -128,6 +128,10 @@ template <typename T>
 struct Half16;
 template <>
 struct Half16<__half> {
+  // P of an attention is taken that many binary places up, as far as the type goes: fp16's
+  // normal range ends at 2^-14, and weights below it lose up to 2^-25 each of the largest one,
+  // which over a long cache adds up to more than an output's rounding.
+  static constexpr float P_UP = 15.0f;
   static __device__ __forceinline__ float2 unpack(uint32_t w) {
     return __half22float2(*reinterpret_cast<const __half2*>(&w));
   }
@@ -145,6 +149,7 @@ struct Half16<__half> {
 };
 template <>
 struct Half16<__nv_bfloat16> {
+  static constexpr float P_UP = 0.0f;  // (normal down to 2^-126)
   static __device__ __forceinline__ float2 unpack(uint32_t w) {
     return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
   }

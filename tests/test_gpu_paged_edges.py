@@ -171,3 +171,16 @@ def test_the_log_sum_exp_counts_many_small_weights(bridge_lib, heads, new, batch
     want = behind + torch.log2(1 + small)
     tol = delta * R.LOG2E + 2.0 ** -19 + (n / 128 + 32) * 2.0 ** -24 * R.LOG2E
     assert float((lse - want).abs().max()) <= tol
+
+
+@pytest.mark.parametrize("heads,new,batch", [(1, 1, 2400), (32, 1, 300), (2, 40, 150)])
+@pytest.mark.parametrize("behind", [20.3, 25.6])
+def test_many_small_weights_in_fp16_add_up(bridge_lib, heads, new, batch, behind):
+    """Each weight is far below fp16's normal range beside the largest, their sum is not. A
+    weight is off by half a step of the type or by 2^-32 of the largest one."""
+    n = 30000
+    out, _, small, delta = _one_heavy_slot(n, new, batch, heads, behind, "f16")
+    want = small / (1 + small)
+    tol = 2 * 2.0 ** -11 * want + (2 * delta + 2.0 ** -18) * want + n * 2.0 ** -32 + 2.0 ** -25
+    over = (out - want).abs() - tol
+    assert float(over.max()) <= 0.0, (float(out.min()), float(out.max()), float(want[0, 0]))
