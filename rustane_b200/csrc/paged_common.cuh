@@ -84,9 +84,10 @@ __device__ __forceinline__ void pdl_wait() {
 
 // 2^x of two numbers on the FMA pipes, for kernels whose exponentials keep the MUFU busy
 // (16 results a clock and SM). x = n + f with n the nearest whole number: 2^f on [-1/2, 1/2] by
-// the polynomial of degree 5 with the least largest relative error (Remez's exchange: 2.6e-7,
-// ex2.approx has 2.4e-7), times 2^n built in the exponent field.
-// Results below 2^-126 are 0, as ex2.approx.ftz's, from 2^128 on infinite; NaN stays NaN.
+// the polynomial of degree 5 with the least largest relative error (Remez's exchange; 2.8e-7, with
+// 32-bit steps 3.4e-7, where ex2.approx has 2.4e-7), times 2^n built in the exponent field.
+// Results below 2^-126 are 0, as ex2.approx.ftz's; NaN stays NaN. n ends at 127: up to 2^128 the
+// polynomial is taken on to f = 1, where it is off by 7e-5, and behind that it overflows.
 __device__ __forceinline__ float max_nan(float a, float b) {
   float r;
   asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
@@ -97,19 +98,21 @@ __device__ __forceinline__ float min_nan(float a, float b) {
   asm("min.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
   return r;
 }
-__device__ __forceinline__ float2 fmul2(float2 a, float2 b) {
+__device__ __forceinline__ float2 fmul2_ftz(float2 a, float2 b) {
   uint64_t r;
-  asm("mul.rn.f32x2 %0, %1, %2;"
+  asm("mul.rn.ftz.f32x2 %0, %1, %2;"
       : "=l"(r)
       : "l"(*reinterpret_cast<uint64_t*>(&a)), "l"(*reinterpret_cast<uint64_t*>(&b)));
   return *reinterpret_cast<float2*>(&r);
 }
 __device__ __forceinline__ float2 exp2_poly2(float2 x) {
   constexpr float MAGIC = 12582912.0f;  // 1.5 x 2^23: adding it rounds to a whole number
-  // n = -127 makes an exponent field of 0, exactly 0, and n = 128 one of 255, infinity
-  x.x = min_nan(max_nan(x.x, -127.0f), 128.0f);
-  x.y = min_nan(max_nan(x.y, -127.0f), 128.0f);
-  const float2 t = fadd2(x, make_float2(MAGIC, MAGIC));
+  // n = -127 makes an exponent field of 0, exactly 0
+  x.x = max_nan(x.x, -127.0f);
+  x.y = max_nan(x.y, -127.0f);
+  float2 t = fadd2(x, make_float2(MAGIC, MAGIC));
+  t.x = min_nan(t.x, MAGIC + 127.0f);
+  t.y = min_nan(t.y, MAGIC + 127.0f);
   const float2 n = fadd2(t, make_float2(-MAGIC, -MAGIC));
   const float2 f = ffma2(n, make_float2(-1.0f, -1.0f), x);
   auto both = [](float c) { return make_float2(c, c); };
@@ -120,7 +123,7 @@ __device__ __forceinline__ float2 exp2_poly2(float2 x) {
   p = ffma2(p, f, both(1.0f));
   const float2 scale = make_float2(__uint_as_float((__float_as_uint(t.x) << 23) + 0x3f800000u),
                                    __uint_as_float((__float_as_uint(t.y) << 23) + 0x3f800000u));
-  return fmul2(p, scale);
+  return fmul2_ftz(p, scale);
 }
 
 // ------------------------------------------------------------------ the 16-bit types

@@ -184,3 +184,53 @@ def test_many_small_weights_in_fp16_add_up(bridge_lib, heads, new, batch, behind
     tol = 2 * 2.0 ** -11 * want + (2 * delta + 2.0 ** -18) * want + n * 2.0 ** -32 + 2.0 ** -25
     over = (out - want).abs() - tol
     assert float(over.max()) <= 0.0, (float(out.min()), float(out.max()), float(want[0, 0]))
+
+
+# ----------------------------------------------- the exponential of the weights of a chunk
+def test_exponentials_of_the_weights_over_their_whole_range(bridge_lib):
+    """With q = 0 and one row of a step that counts (log-sum-exp -x, the others infinite) a
+    slot's weight is 2^x. The columns of a step take 2^x from the special-function unit (relative
+    error 2^-22) or from a polynomial (3.4e-7): each within that, 0 below 2^-126, infinite from
+    2^128 on. Between 2^127.5 and there the polynomial is off by up to 7e-5."""
+    n, heads, page = 8192, 128, 16
+    dev = "cuda"
+    own = 7 + torch.arange(n, device=dev, dtype=torch.int32)
+    table = torch.cat([torch.arange(7, device=dev, dtype=torch.int32).expand(n, 7), own[:, None]], 1)
+    table = table.contiguous()
+    length = torch.full((n,), 128, device=dev, dtype=torch.int32)
+    start = torch.arange(n + 1, device=dev, dtype=torch.int32)
+    pages = n + 7
+    k = torch.zeros(pages, 1, page, 128, device=dev, dtype=torch.float16)
+    q = torch.zeros(n, heads * 128, device=dev, dtype=torch.float16)
+    kv = B.cb_paged_kv(k.data_ptr(), k.data_ptr(), table.data_ptr(), length.data_ptr(),
+                       start.data_ptr(), B.CB_DTYPE_F16, pages, 1, page, n, 8, 128, n, 1)
+    row = torch.arange(n, device=dev)
+    g = torch.Generator(device=dev).manual_seed(1)
+    special = [-126.0, -126.2, -126.49, -126.51, -127.0, -127.6, -149.0, -1e30, -math.inf,
+               math.nextafter(-126.0, 0.0), 127.49, 127.51, 127.6, 127.99, 128.0, 128.01, 129.0,
+               1e30, math.inf, math.nan, 0.0, -0.5, 0.5, 1.0, -1.0]
+    for lo, hi in ((-127.0, -125.0), (126.5, 128.5), (-130.0, 129.0), (-1.0, 1.0), (-40.0, 2.0)):
+        x = lo + (hi - lo) * torch.rand(n, device=dev, generator=g)
+        x = torch.cat([torch.tensor(special, device=dev).repeat_interleave(8), x])[:n].float()
+        lse = torch.full((n, heads), math.inf, device=dev)
+        col = (row * 37 + row // 8) % 128
+        col[:8 * len(special)] = (row % 8)[:8 * len(special)]  # every special value in 8 columns
+        lse[row, col] = -x
+        w = torch.zeros(pages, 1, page, device=dev)
+        assert bridge_lib.cb_paged_attention_weights(C.byref(kv), ptr(q), q.stride(0), heads, 1.0,
+                                                     ptr(lse), ptr(w), stream()) == 0
+        torch.cuda.synchronize()
+        got = w[own.long(), 0]
+        assert bool(((got == got[:, :1]) | got.isnan()).all())  # all slots of a page alike
+        got = got[:, 0]
+        nan = x.isnan()
+        assert bool(got[nan].isnan().all()) and not bool(got[~nan].isnan().any())
+        assert bool((got[x < -126.0] == 0).all())
+        assert bool(torch.isinf(got[x >= 128.001]).all())
+        usual = (x >= -126.0) & (x <= 127.5)
+        want = torch.exp2(x.double())
+        error = ((got.double() - want).abs() / want)
+        assert float(error[usual].max()) <= 3.4e-7
+        top = (x > 127.5) & (x < 128.0)
+        if bool(top.any()):
+            assert float(error[top].max()) <= 7e-5
