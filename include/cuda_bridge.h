@@ -459,6 +459,8 @@ cb_status cb_lm_head_ce_f16_noalloc(const void* xf, const void* embed, const uin
  *
  * All pointers are device memory of the current device (CB_ERR_INVALID_ARG otherwise),
  * token arrays and caches 16-byte aligned, strides counted in elements and multiples of 8.
+ * What a call writes lies apart from everything else that it reads or writes, but for what its
+ * comment allows (CB_ERR_INVALID_ARG otherwise; token arrays may be columns of one wider array).
  * Work is enqueued on `stream` (NULL = default stream) without allocation or
  * synchronisation; a call without rows (rows, max_new or tokens 0) does nothing, and with
  * rows or tokens 0 its token arrays may be NULL. Device-side values are held to the

@@ -88,6 +88,40 @@ bool ranges_overlap(const void* a, int64_t a_bytes, const void* b, int64_t b_byt
   return pa < pb + b_bytes && pb < pa + a_bytes;
 }
 
+// What a call reads or writes, from its first to its last byte; a token array by its rows.
+struct Span {
+  const void* p;
+  int64_t bytes;
+};
+Span token_span(const void* p, int64_t rows, int64_t stride, int64_t width) {
+  return Span{p, ((rows - 1) * stride + width) * 2};
+}
+Span meta_span(const void* p, const cb_paged_kv* kv) {  // [pages][kv_heads][page_size]
+  return Span{p, (int64_t)kv->pages * kv->kv_heads * kv->page_size * 4};
+}
+Span pool_span(const void* p, const cb_paged_kv* kv) {
+  return Span{p, (int64_t)kv->pages * kv->kv_heads * kv->page_size * PG_HD * 2};
+}
+Span table_span(const cb_paged_kv* kv) {
+  return Span{kv->table, (int64_t)kv->batch * kv->table_stride * 4};
+}
+Span len_span(const cb_paged_kv* kv) { return Span{kv->len, kv->batch * 4ll}; }
+Span row_start_span(const cb_paged_kv* kv) { return Span{kv->row_start, (kv->batch + 1ll) * 4}; }
+
+// Whether an output meets another output or an input (those of one call; null ones are absent).
+bool outputs_meet(std::initializer_list<Span> outputs, std::initializer_list<Span> inputs) {
+  auto meet = [](const Span& a, const Span& b) {
+    return a.p && b.p && ranges_overlap(a.p, a.bytes, b.p, b.bytes);
+  };
+  for (const Span* o = outputs.begin(); o != outputs.end(); ++o) {
+    for (const Span* x = o + 1; x != outputs.end(); ++x)
+      if (meet(*o, *x)) return true;
+    for (const Span& x : inputs)
+      if (meet(*o, x)) return true;
+  }
+  return false;
+}
+
 // The current device is a B200 and every (non-null) pointer is memory of it.
 cb_status check_device(std::initializer_list<const void*> pointers) {
   int dev = 0;
@@ -408,6 +442,9 @@ cb_status cb_rope(const cb_rope_config* rope, int32_t dtype, const void* x, int6
   if (!(x == y && x_stride == y_stride) &&
       arrays_overlap(x, x_stride, width, y, y_stride, width, tokens))
     return CB_ERR_INVALID_ARG;
+  if (outputs_meet({token_span(y, tokens, y_stride, width)},
+                   {Span{positions, tokens * 4ll}, Span{rope->inv_freq, rope->rot_dim * 4ll}}))
+    return CB_ERR_INVALID_ARG;
   const cb_status s = check_device({x, y, positions, rope->inv_freq});
   if (s != CB_OK) return s;
   const int piece = rope->rot_dim % 16 == 0 && head_dim % 16 == 0 ? 8 : 4;
@@ -451,6 +488,21 @@ cb_status cb_paged_append(const cb_paged_kv* kv, const cb_rope_config* rope, int
     return CB_ERR_INVALID_ARG;
   if (q && (arrays_overlap(q_out, q_out_stride, q_width, k, k_stride, kv_width, rows) ||
             arrays_overlap(q_out, q_out_stride, q_width, v, v_stride, kv_width, rows)))
+    return CB_ERR_INVALID_ARG;
+  const Span q_out_span = q ? token_span(q_out, rows, q_out_stride, q_width) : Span{};
+  const Span inv_freq{rope ? rope->inv_freq : nullptr, rope ? rope->rot_dim * 4ll : 0};
+  const Span read[] = {table_span(kv), len_span(kv), row_start_span(kv),
+                       Span{positions, rows * 4}, inv_freq};
+  const Span tokens[] = {q ? token_span(q, rows, q_stride, q_width) : Span{},
+                         token_span(k, rows, k_stride, kv_width),
+                         token_span(v, rows, v_stride, kv_width)};
+  const Span written[] = {pool_span(kv->k, kv), pool_span(kv->v, kv)};
+  if (outputs_meet({q_out_span, meta_span(weights, kv), meta_span(slot_positions, kv)},
+                   {read[0], read[1], read[2], read[3], read[4], written[0], written[1]}) ||
+      outputs_meet({meta_span(weights, kv), meta_span(slot_positions, kv)},
+                   {tokens[0], tokens[1], tokens[2]}) ||
+      outputs_meet({written[0]}, {read[0], read[1], read[2], read[3], read[4]}) ||
+      outputs_meet({written[1]}, {read[0], read[1], read[2], read[3], read[4]}))
     return CB_ERR_INVALID_ARG;
   const cb_status s =
       check_device({kv->k, kv->v, kv->table, kv->len, kv->row_start, rope ? rope->inv_freq : nullptr,
@@ -505,6 +557,13 @@ static cb_status paged_attention(const cb_paged_kv* kv, const void* q, int64_t q
   if (kv->rows == 0 || kv->max_new == 0) return CB_OK;
   if (arrays_overlap(q, q_stride, width, out, out_stride, width, kv->rows))
     return CB_ERR_INVALID_ARG;
+  const Span lse_span{lse, (int64_t)kv->rows * heads * 4}, ws_span{workspace, (int64_t)need};
+  const Span q_span = token_span(q, kv->rows, q_stride, width);
+  if (outputs_meet({token_span(out, kv->rows, out_stride, width), lse_span, ws_span},
+                   {pool_span(kv->k, kv), pool_span(kv->v, kv), table_span(kv), len_span(kv),
+                    row_start_span(kv)}) ||
+      outputs_meet({lse_span, ws_span}, {q_span}))
+    return CB_ERR_INVALID_ARG;
   const cb_status s = check_device({kv->k, kv->v, kv->table, kv->len, kv->row_start, q, out, lse,
                                     workspace});
   if (s != CB_OK) return s;
@@ -531,6 +590,11 @@ static cb_status paged_weights(const cb_paged_kv* kv, const void* q, int64_t q_s
       (kv->rows > 0 && !lse) || !weights || !aligned(lse, 4) || !aligned(weights, 4))
     return CB_ERR_INVALID_ARG;
   if (kv->rows == 0 || kv->max_new == 0) return CB_OK;
+  if (outputs_meet({meta_span(weights, kv)},
+                   {pool_span(kv->k, kv), table_span(kv), len_span(kv), row_start_span(kv),
+                    token_span(q, kv->rows, q_stride, (int64_t)heads * PG_HD),
+                    Span{lse, (int64_t)kv->rows * heads * 4}}))
+    return CB_ERR_INVALID_ARG;
   const cb_status s =
       check_device({kv->k, kv->table, kv->len, kv->row_start, q, lse, weights});
   if (s != CB_OK) return s;
@@ -613,13 +677,19 @@ cb_status cb_paged_evict(const cb_paged_kv* kv, const float* weights, float* wei
   size_t need = 0;
   cb_paged_evict_workspace(kv, budget, &need);
   if (workspace_bytes < need) return CB_ERR_INVALID_ARG;
-  const int64_t meta = (int64_t)kv->pages * kv->kv_heads * kv->page_size * 4;
-  if ((weights != weights_out && ranges_overlap(weights, meta, weights_out, meta)) ||
-      (positions != positions_out && ranges_overlap(positions, meta, positions_out, meta)) ||
-      ranges_overlap(len_out, kv->batch * 4ll, kv->len, kv->batch * 4ll) ||
-      ranges_overlap(weights_out, meta, positions_out, meta) ||
-      ranges_overlap(weights_out, meta, positions, meta) ||
-      ranges_overlap(weights, meta, positions_out, meta))
+  const Span w_in = meta_span(weights, kv), p_in = meta_span(positions, kv);
+  const Span w_out = meta_span(weights_out, kv), p_out = meta_span(positions_out, kv);
+  const Span lens_out{len_out, kv->batch * 4ll}, ws{workspace, (int64_t)need};
+  const Span next{next_position, kv->batch * 4ll};
+  if ((weights != weights_out && outputs_meet({w_out}, {w_in})) ||
+      (positions != positions_out && outputs_meet({p_out}, {p_in})) ||
+      outputs_meet({w_out}, {p_in}) || outputs_meet({p_out}, {w_in}) ||
+      outputs_meet({lens_out, ws}, {w_in, p_in}) ||
+      outputs_meet({w_out, p_out, lens_out, ws},
+                   {len_span(kv), table_span(kv), next, pool_span(kv->k, kv),
+                    pool_span(kv->v, kv)}) ||
+      outputs_meet({pool_span(kv->k, kv)}, {w_in, p_in, len_span(kv), table_span(kv), next}) ||
+      outputs_meet({pool_span(kv->v, kv)}, {w_in, p_in, len_span(kv), table_span(kv), next}))
     return CB_ERR_INVALID_ARG;
   if (kv->max_len > EV_MAX_LEN) return CB_ERR_UNSUPPORTED;
   const cb_status s = check_device({kv->k, kv->v, kv->table, kv->len, weights, weights_out,
