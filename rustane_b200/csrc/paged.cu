@@ -65,10 +65,11 @@ bool heads_ok(const cb_paged_kv* kv, int32_t heads) {
 }
 
 // A token array: [rows][width] elements of two bytes. One without rows may be null, as that of
-// an empty tensor.
+// an empty tensor. No memory has 2^60 elements: the bytes up to its end fit 64 bits.
 bool array_ok(const void* p, int64_t rows, int64_t stride, int64_t width) {
   if (rows == 0) return true;
-  return p && aligned(p, 16) && stride >= width && stride % 8 == 0 && stride <= (int64_t(1) << 40);
+  return p && aligned(p, 16) && stride >= width && stride % 8 == 0 &&
+         stride <= (int64_t(1) << 40) && (double)rows * (double)stride < 0x1p60;
 }
 
 // Whether two token arrays share an element. Columns of one wider array do not.

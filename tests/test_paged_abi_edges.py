@@ -79,3 +79,16 @@ def test_arrays_side_by_side_are_not_refused(bridge_lib):
     assert _reached(_append(bridge_lib, kv, q=6 * A, qs=1024, qo=6 * A, qos=1024, k=6 * A + row,
                             ks=1024, v=6 * A + row + 512, vs=1024, pos=None, w=None, sp=None))
     assert _reached(_attention(bridge_lib, _kv(v=A)))                     # one pool read as both
+
+
+@pytest.mark.parametrize("rows", [1 << 23, (1 << 29) - 1])
+def test_token_arrays_longer_than_any_memory_are_refused(bridge_lib, rows):
+    """(rows - 1) * stride elements of two bytes pass 2^63: no address arithmetic on them."""
+    kv, s = _kv(rows=rows), 1 << 40
+    assert _attention(bridge_lib, kv, q_stride=s) == BAD
+    assert _attention(bridge_lib, kv, out_stride=s) == BAD
+    assert _weights(bridge_lib, kv, qs=s) == BAD
+    for name in ("qs", "qos", "ks", "vs"):
+        assert _append(bridge_lib, kv, **{name: s}) == BAD
+    assert _rope(bridge_lib, _config(), xs=s, tokens=rows) == BAD
+    assert _rope(bridge_lib, _config(), ys=s, tokens=rows) == BAD
