@@ -395,6 +395,7 @@ cb_status cb_rope_frequencies(int32_t rot_dim, const cb_rope_scaling* scaling, d
     return CB_ERR_INVALID_ARG;
   double base = s.base;
   if (s.kind == CB_ROPE_SCALE_BASE) base *= std::pow(s.factor, (double)rot_dim / (rot_dim - 2));
+  if (!std::isfinite(base)) return CB_ERR_INVALID_ARG;
   double lo = 0.0, hi = 0.0;
   if (s.kind == CB_ROPE_SCALE_PARTS) {
     if (!(s.original_len > 0.0) || !(s.slow_turns > 0.0) || !(s.fast_turns >= s.slow_turns) ||

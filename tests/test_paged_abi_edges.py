@@ -92,3 +92,12 @@ def test_token_arrays_longer_than_any_memory_are_refused(bridge_lib, rows):
         assert _append(bridge_lib, kv, **{name: s}) == BAD
     assert _rope(bridge_lib, _config(), xs=s, tokens=rows) == BAD
     assert _rope(bridge_lib, _config(), ys=s, tokens=rows) == BAD
+
+
+@pytest.mark.parametrize("base,factor", [(10000.0, 1e306), (1e300, 1e10), (1e308, 2.0)])
+def test_a_scaled_base_that_is_not_finite_is_refused(bridge_lib, base, factor):
+    """All frequencies but the first would be 0."""
+    s = B.cb_rope_scaling(base, B.CB_ROPE_SCALE_BASE, factor, 0.0, 0.0, 0.0)
+    inv = (C.c_double * 32)(*[7.0] * 32)
+    assert bridge_lib.cb_rope_frequencies(64, C.byref(s), inv, None) == BAD
+    assert list(inv) == [7.0] * 32
