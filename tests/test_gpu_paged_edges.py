@@ -234,3 +234,108 @@ def test_exponentials_of_the_weights_over_their_whole_range(bridge_lib):
         top = (x > 127.5) & (x < 128.0)
         if bool(top.any()):
             assert float(error[top].max()) <= 7e-5
+
+
+# ----------------------------------------------------------- bounds wider than what there is
+@pytest.mark.parametrize("lens,news,heads,kv_heads,page", [
+    ([700, 3, 0, 259], [1, 1, 0, 1], 8, 2, 32), ([400, 129, 64, 2], [129, 0, 1, 2], 4, 4, 128),
+    ([5000, 20, 3000], [1, 1, 2], 8, 4, 16), ([90, 0, 17], [0, 0, 0], 4, 2, 16)])
+def test_a_step_below_the_descriptors_bounds(bridge_lib, lens, news, heads, kv_heads, page):
+    """What a graph captured for larger steps meets: max_len, max_new, rows and the table's rows
+    far above the step's, ids behind a sequence's pages outside the pool. Up to a step in
+    which no sequence has a token."""
+    c = Cache(lens, news, heads, kv_heads, page, "bf16", seed=7, pad=600, max_len=40000, max_new=512,
+              table_stride=40000 // page + 1)
+    total, scale = c.starts[-1], 128 ** -0.5
+    q = c.tokens(heads * 128)
+    out = torch.full((c.rows, heads * 128), 3.0, device="cuda", dtype=c.dt)
+    lse = torch.full((c.rows, heads), 3.0, device="cuda")
+    assert R.attention(bridge_lib, c, q, scale, out, lse) == 0
+    want, want_lse, tol, lse_tol = R.attention_ref(c, q, scale)
+    over = (out[:total].unflatten(1, (heads, 128)).double() - want).abs() - tol
+    assert total == 0 or float(over.max()) <= 0
+    assert total == 0 or float(((lse[:total].double() - want_lse).abs() - lse_tol).max()) <= 0
+    assert bool((out[total:] == 3.0).all()) and bool((lse[total:] == 3.0).all())
+    w = torch.rand(c.pages, kv_heads, page, device="cuda")
+    ref, w_tol = R.weights_ref(c, q, scale, lse, w)
+    d = c.desc()
+    assert bridge_lib.cb_paged_attention_weights(C.byref(d), ptr(q), q.stride(0), heads, scale,
+                                                 ptr(lse), ptr(w), stream()) == 0
+    torch.cuda.synchronize()
+    assert float(((w.double() - ref).abs() - w_tol).max()) <= 0
+    # append and evict of the same step: rows, and slots behind the sequences, as they were
+    k, v = c.tokens(kv_heads * 128), c.tokens(kv_heads * 128)
+    pool = c.k.clone()
+    q_out = torch.full_like(q, 3.0)
+    assert bridge_lib.cb_paged_append(C.byref(d), None, heads, ptr(q), q.stride(0), ptr(q_out),
+                                      q_out.stride(0), ptr(k), k.stride(0), ptr(v), v.stride(0),
+                                      None, None, None, stream()) == 0
+    torch.cuda.synchronize()
+    assert torch.equal(q_out[:total], q[:total]) and bool((q_out[total:] == 3.0).all())
+    for b in range(c.batch):
+        at = c.place(b, torch.arange(lens[b] - news[b], lens[b], device="cuda"))
+        rows = k[c.starts[b]:c.starts[b + 1]].unflatten(1, (kv_heads, 128))
+        for h in range(kv_heads):
+            pool[at[0], h, at[1]] = rows[:, h]
+    assert torch.equal(c.k.view(torch.int16), pool.view(torch.int16))
+    p = torch.zeros(w.shape, device="cuda", dtype=torch.int32)
+    lo = torch.full_like(c.len, -1)
+    assert _evict(bridge_lib, c, w, w, p, p, c.len, 40000, 0, 0, lo) == 0
+    assert lo.tolist() == lens and torch.equal(c.k.view(torch.int16), pool.view(torch.int16))
+
+
+FIRST_CALLS = """
+import ctypes as C, sys, torch
+sys.path[:0] = [{root!r}, {root!r} + "/tests"]
+import paged_ref as R
+from paged_ref import Cache, ptr
+from rustane_b200 import bridge as B
+lib = B.load_library()
+for lens, news, heads in (([300, 40], [1, 1], 4), ([300, 140], [120, 33], 4)):
+    c = Cache(lens, news, heads, 2, 16, "f16")
+    q, k, v = c.tokens(512), c.tokens(256), c.tokens(256)
+    out, q_out = torch.zeros_like(q), torch.zeros_like(q)
+    lse = torch.zeros(c.rows, heads, device="cuda")
+    w = torch.zeros(c.pages, 2, 16, device="cuda")
+    p = torch.zeros(c.pages, 2, 16, device="cuda", dtype=torch.int32)
+    pos = torch.zeros(c.rows, device="cuda", dtype=torch.int32)
+    inv = torch.ones(64, device="cuda", dtype=torch.float64)
+    lo = torch.zeros_like(c.len)
+    d, size, esize = c.desc(), C.c_size_t(), C.c_size_t()
+    assert lib.cb_paged_attention_workspace(C.byref(d), heads, C.byref(size)) == 0
+    assert lib.cb_paged_evict_workspace(C.byref(d), 64, C.byref(esize)) == 0
+    ws = torch.zeros(size.value + esize.value + 64, dtype=torch.uint8, device="cuda")
+    ews = ws[-(-size.value // 16) * 16:]
+    rope = B.cb_rope_config(inv.data_ptr(), 128, B.CB_ROPE_HALF, 1.0)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        st = C.c_void_p(torch.cuda.current_stream().cuda_stream)
+        assert lib.cb_rope(C.byref(rope), 1, ptr(q), 512, ptr(out), 512, ptr(pos), c.rows, 4, 128, 0, st) == 0
+        assert lib.cb_paged_append(C.byref(d), C.byref(rope), heads, ptr(q), 512, ptr(q_out), 512, ptr(k),
+                                   256, ptr(v), 256, None, ptr(w), ptr(p), st) == 0
+        assert lib.cb_paged_attention(C.byref(d), ptr(q_out), 512, heads, 0.1, ptr(out), 512, ptr(lse),
+                                      ptr(ws), size.value, st) == 0
+        assert lib.cb_paged_attention_weights(C.byref(d), ptr(q_out), 512, heads, 0.1, ptr(lse), ptr(w), st) == 0
+        assert lib.cb_paged_evict(C.byref(d), ptr(w), ptr(w), ptr(p), ptr(p), ptr(c.len), 64, 0, 0,
+                                  ptr(lo), ptr(ews), esize.value, st) == 0
+    graph.replay()
+    torch.cuda.synchronize()
+    assert lo.tolist() == [min(n, 64) for n in lens]
+    total = c.starts[-1]
+    got = out[:total].unflatten(1, (heads, 128)).double()
+    assert bool(torch.isfinite(got).all()) and float(got.abs().max()) > 0
+    assert bool(torch.isfinite(lse[:total]).all())
+print("captured first calls: fine")
+"""
+
+
+def test_the_first_calls_of_a_process_may_be_captured(bridge_lib):
+    """No call needs one outside a capture before it."""
+    import subprocess
+    import sys
+    from pathlib import Path
+    root = str(Path(__file__).resolve().parents[1])
+    r = subprocess.run([sys.executable, "-c", FIRST_CALLS.format(root=root)], capture_output=True,
+                       text=True, timeout=300)
+    assert r.returncode == 0 and "fine" in r.stdout, r.stdout + r.stderr
