@@ -466,10 +466,10 @@ cb_status cb_lm_head_ce_f16_noalloc(const void* xf, const void* embed, const uin
  * rows or tokens 0 its token arrays may be NULL. Device-side values are held to the
  * descriptor: a page id outside 0 .. pages - 1 stands for slots that are absent (not
  * written, not seen by any query), slots from max_len on are absent, rows from `rows` on
- * do not exist, and of a sequence with more than max_new new tokens the rows behind
- * max_new are left alone. Rows behind the last sequence (padding) are neither read nor
- * written. A batch whose descriptor allows more work than a launch can count (about 2^29
- * blocks of 16 slots) is CB_ERR_UNSUPPORTED.
+ * do not exist (a sequence's new tokens end there), and of a sequence with more than max_new
+ * new tokens the rows behind max_new are left alone. What rows behind the last sequence
+ * (padding) hold does not matter, and they are not written. A batch whose descriptor allows
+ * more work than a launch can count (about 2^29 blocks of 16 slots) is CB_ERR_UNSUPPORTED.
  *
  * The kernels' waits are bounded (2 s). After one that ran out, rows of out and lse, or slots of
  * weights, that were not finished are NaN, and cb_paged_check_device_error reports it. */

@@ -232,12 +232,13 @@ struct AttentionPlan {
   }
 };
 
-// More than 16 query rows per key head go to the tcgen05 kernel. Both sides measured (us; bf16,
-// 8 key heads):  rows per key head     8    16    24    32    64   128
-//   4 x 8192 slots,  16-row kernel  37.3  41.3  52.1  54.0  85.5   150
-//                    tcgen05        46.3  47.7  47.9  47.8  48.9  49.2
-//   32 x 2048 slots, 16-row kernel  59.2  65.8   106   109   194   334
-//                    tcgen05        73.4  76.0  77.5  78.1  79.4  80.9
+// More than 16 query rows per key head go to the tcgen05 kernel. Both sides measured (us, the L2
+// flushed before each call; bf16, 8 key heads):
+//                rows per key head     8    16    24    32    64   128
+//   4 x 8192 slots,  16-row kernel    47    49    66    68   100   160
+//                    tcgen05          53    53    55    53    55    55
+//   32 x 2048 slots, 16-row kernel    74    78   119   121   199   360
+//                    tcgen05          82    84    86    86    88    88
 AttentionPlan plan_attention(const cb_paged_kv* kv, int32_t heads) {
   AttentionPlan p;
   const int group = heads / kv->kv_heads;

@@ -15,11 +15,11 @@
 // blocks of 16 keys through a ring that TMA fills, running ahead over the borders of tiles, and
 // meets no other warp until the join. (A CTA per tile and part of the keys, whose four warps
 // joined in shared memory, left the SMs idle at every CTA's start and end and in the last
-// wave: 4.4 TB/s on few long sequences, 4.6 on many short ones.)
+// wave: 76 us for the first case below, where this form then took 65.)
 //
-// Measured: 4 x up to 32768 slots, 32 / 8 heads, bf16, 331 MB: 66.7 us, 5.0 TB/s; 64 x up to 512
-// slots, 12 / 12 heads, f16, 111 MB: 25.6 us. About 6 us of each are the walk to a worker's first
-// block and the join; between them the reads run at 7 TB/s but for the slowest SM's tail.
+// Measured: 4 x up to 32768 slots, 32 / 8 heads, bf16, 331 MB: 66.9 us, 4.9 TB/s; 64 x up to 512
+// slots, 12 / 12 heads, f16, 111 MB: 25.8 us, 4.3 TB/s. The walk to a worker's first block comes
+// before the reads, the slowest SM's tail and the join (alone and cold: 12 and 7 us) behind them.
 //
 // A weight of 0 does not keep an infinity or NaN out of a product. V of slots behind the
 // sequence's end, which may hold anything, reads as 0; and of the slots that only later ones of
@@ -439,8 +439,8 @@ __global__ void __launch_bounds__(PR_WARPS * 32)
 // The dot product may take the head's elements in any order: lane c of a quad takes the
 // 16-byte pieces c, c + 4, ... of both operands, so a quad reads whole 64-byte runs and K goes
 // to registers directly. Bound by the reads of K: a warp is a worker as in the attention
-// kernel, with one block of 16 slots on its way while it works on another. 16 x up to 4097 slots,
-// 32 / 8 heads, f16, 83 MB: 19.1 to 19.9 us, 4.2 TB/s.
+// kernel, with one block of 16 slots on its way while it works on another (K in registers: 128 of
+// them, and a few spills). 16 x up to 4097 slots, 32 / 8 heads, f16, 83 MB: 19.1 us, 4.3 TB/s.
 constexpr int PW_WARPS = 8;  // two CTAs per SM
 struct PwShared {
   PrShares::Walk walk[PW_WARPS];

@@ -18,14 +18,14 @@
 //                below 2^8, or in fp16, whose small weights are taken 2^7 up, below 2^15).
 // A tile's S(j+1) is issued behind its PV(j), so "S(j+1) is full" also says that O may be
 // rescaled and that P(j) is no longer read. Steps of 64 keys with two S buffers a tile, and
-// two threads per row, hide the products' latency as well, but a step costs a warp about 60
-// instructions whatever its keys: both took 2.3 us for 128 keys. Where there are at most 128
-// rows, tile B rests: to give it the same rows and every other step won 3 % (24 rows on 32 x 2048
-// slots, 8 key heads: 77.5 to 75.0 us; the loads' latency is the pace there, 2 us a step).
+// two threads per row, hide the products' latency as well, but a step costs a warp some sixty
+// instructions whatever its keys: both were slower. Where there are at most 128 rows, tile B
+// rests: to give it the same rows and every other step won 3 % when tried and was not kept.
 //
-// Measured (bf16): 2 x 2048 new tokens on 16384 slots, 40 / 8 heads, 1.29 TFLOP: 1.19 to 1.23 ms,
-// 1050 TFLOP/s at the power cap's 1.57 GHz. 8 chunks of up to 512 on 2048 (f16, 12 / 12 heads):
-// 51.5 us, about 5 to the first product, 4 to 6 per tile and 5 for the join.
+// Measured (bf16): 2 x 2048 new tokens on 16384 slots, 40 / 8 heads, 1.29 TFLOP: 1.18 to 1.31 ms
+// on different GPUs, 980 to 1090 TFLOP/s at the power cap's 1.57 GHz. 8 chunks of up to 512 on
+// 2048 (f16, 12 / 12 heads): 51.8 us; at most 16 steps a tile do not hide a tile's own cost (its
+// Q, the pipeline's start, its output), and the join (alone and cold) takes 10 us.
 //
 // Infinities and NaN in V of slots that not every row sees are taken out and added afterwards to
 // the rows that see them (see paged_attention.cuh).
@@ -110,7 +110,7 @@ __device__ __forceinline__ void pt_commit(uint32_t leader, uint64_t* bar) {
 
 // Loads a warp's 32 query rows f0 + r (r = first .. first + 31) of a key head into a K-major
 // swizzled tile; rows behind the sequence's last are zero. Half a warp takes a row, so a load
-// meets whole lines (a row per lane took 2.6 us for the block's 256 rows).
+// meets whole lines.
 template <typename T>
 __device__ __forceinline__ void pt_load_q(uint8_t* tile, const T* __restrict__ q, int64_t q_stride,
                                           const PagedSeq& seq, int head, int group, int f0,
@@ -159,9 +159,8 @@ __device__ __forceinline__ int pt_step_id(const PagedKV& kv, int b, int key0, in
   return (lane >> 1) * box_rows < KEYS && key < end ? kv.page_id(b, key) : -1;
 }
 
-// A tile counts three steps for its Q, its pipeline's start and its output (a step takes 1.9 us,
-// a tile 4 to 6 us beside its steps; ragged prompts: 58.6 us with two, 51.6 with three, 53.8
-// with four).
+// A tile counts three steps for its Q, its pipeline's start and its output (ragged prompts: 58.6
+// us with two, 51.6 with three, 53.8 with four).
 using PtShares = PagedShares<PT_ROWS, PT_KEYS, 3, 5>;
 
 struct PtShared {  // at PT_SHARE_OFF

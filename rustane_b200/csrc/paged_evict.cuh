@@ -19,8 +19,8 @@
 // Reading the weights and positions and moving the rows is the work that cannot be left out;
 // a long sequence gets several CTAs (they share the counts through distributed shared
 // memory), because one SM moves rows at a small part of the memory's rate.
-// 4 x up to 32768 slots to 8192, 8 heads, bf16: 45 us, 20 of them the moves at the memory's rate,
-// the others the latency of three passes and the numbering. 64 x 513 slots to 512, 12 heads: 5.7 us.
+// 4 x up to 32768 slots to 8192, 8 heads, bf16: 44.5 us, 20 of them the moves at the memory's rate,
+// the others the latency of the passes and the numbering. 64 x 513 slots to 512, 12 heads: 5.6 us.
 #pragma once
 #include "paged_common.cuh"
 
@@ -294,7 +294,7 @@ __global__ void __launch_bounds__(THREADS)
   // ---- the budget-th largest key T: the histogram of the keys within [T, T + 2^(shift + 11))
   // (all of them at first), the bin that holds it, and on within that bin. Of the other CTAs'
   // histograms only the sums over 32 bins and then the 32 bins in question are read (all of
-  // them would be 64 KB a CTA and pass: 3 to 20 us over the SMs' network).
+  // them would be 64 KB a CTA and pass over the SMs' network).
   uint32_t T = 0;
   uint32_t want = (uint32_t)a.budget;  // that many of the range's largest keys stay
   bool exact = false;                  // all keys >= T stay

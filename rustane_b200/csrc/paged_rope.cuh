@@ -9,9 +9,9 @@
 // PIECE is 8 (16-byte accesses) where rot_dim and the head's size are multiples of 16, else 4.
 // The angle is formed in 64 bits as a fraction of a turn (at position 10^6 a 32-bit product
 // would be off by 0.06 rad), reduced to [-1/2, 1/2] there, and only then rounded to 32 bits.
-// Measured: 16384 tokens x 12 heads of 128, interleaved, f16, 101 MB: 20.8 us, 4.9 TB/s (a plain
-// device copy of as much: 35 us); appending 12 prompts of up to 1000 tokens, 32 / 8 heads, bf16,
-// 191 MB: 39 us, 4.9 TB/s; one token of 64 sequences: 3.7 us, a launch and three dependent reads.
+// Measured: 16384 tokens x 12 heads of 128, interleaved, f16, 101 MB: 20.7 us, 4.9 TB/s (torch's
+// copy of as much: 35 us); appending 12 prompts of up to 1000 tokens, 32 / 8 heads, bf16, 191 MB:
+// 38.4 us, 5.0 TB/s; one token of 64 sequences: 3.7 us, a launch and three dependent reads.
 #pragma once
 #include "paged_common.cuh"
 
